@@ -136,6 +136,12 @@ int balance_loss(const void* logits, int dtype, const int* top_experts, int64_t 
 int gates_backward(const void* logits, int dtype, const int64_t* sorted_experts, const int64_t* pair_pos, const float* d_gates,
                    const float* share, const float* d_loss, float alpha, int64_t batch, int64_t seq, int E, int top_k, void* d_logits,
                    cudaStream_t st);
+int64_t linear_ce_state_bytes(int64_t T);
+int64_t linear_ce_workspace_bytes(int64_t T, int64_t V, int64_t d, int pass);
+int linear_ce_forward(const void* x, int64_t ldx, const void* w, int64_t ldw, int dtype, const int64_t* target, int64_t ignore, int64_t T, int64_t V,
+                      int64_t d, int reduction, float* loss, void* state, void* workspace, int64_t workspace_bytes, cudaStream_t st);
+int linear_ce_backward(const void* x, int64_t ldx, const void* w, int64_t ldw, int dtype, const float* grad, int64_t T, int64_t V, int64_t d,
+                       int reduction, const void* state, void* dx, void* dw, void* workspace, int64_t workspace_bytes, cudaStream_t st);
 int update_bias(const int64_t* counts, float* bias, int E, float expected, float gamma, cudaStream_t st);
 int64_t moe_route_workspace_ints(int64_t T, int E);
 int moe_route(const void* logits, int logits_dtype, const float* bias, int64_t T, int E, int top_k, int* workspace, int* top_experts,
@@ -355,6 +361,21 @@ int cinn_lightning_indexer(const void* q, const void* k, const void* w, int dtyp
                            int64_t Lk, int64_t H, int64_t d, const int64_t* q_strides, const int64_t* k_strides,
                            const int64_t* w_strides, void* stream) {
     return cinn::lightning_indexer(q, k, w, dtype, out, B, Lq, Lk, H, d, q_strides, k_strides, w_strides, (cudaStream_t)stream);
+}
+
+int64_t cinn_linear_ce_state_bytes(int64_t T) { return cinn::linear_ce_state_bytes(T); }
+int64_t cinn_linear_ce_workspace_bytes(int64_t T, int64_t V, int64_t d, int pass) { return cinn::linear_ce_workspace_bytes(T, V, d, pass); }
+int cinn_linear_ce_forward(const void* x, int64_t ldx, const void* w, int64_t ldw, int dtype, const int64_t* target, int64_t ignore_index,
+                           int64_t T, int64_t V, int64_t d, int reduction, float* loss, void* state, void* workspace,
+                           int64_t workspace_bytes, void* stream) {
+    return cinn::linear_ce_forward(x, ldx, w, ldw, dtype, target, ignore_index, T, V, d, reduction, loss, state, workspace, workspace_bytes,
+                                   (cudaStream_t)stream);
+}
+int cinn_linear_ce_backward(const void* x, int64_t ldx, const void* w, int64_t ldw, int dtype, const float* grad, int64_t T, int64_t V,
+                            int64_t d, int reduction, const void* state, void* dx, void* dw, void* workspace, int64_t workspace_bytes,
+                            void* stream) {
+    return cinn::linear_ce_backward(x, ldx, w, ldw, dtype, grad, T, V, d, reduction, state, dx, dw, workspace, workspace_bytes,
+                                    (cudaStream_t)stream);
 }
 
 int cinn_scatter_rows(const void* in, const int64_t* idx, void* out, int64_t n_rows, int64_t n_dst, int64_t row_bytes,

@@ -742,6 +742,7 @@ static inline int gemm_sms() {
     const int lim = g_gemm_sm_limit.load(std::memory_order_relaxed), all = sm_count();
     return (lim > 0 && lim < all) ? lim : all;
 }
+int gemm_sm_count() { return gemm_sms(); }
 bool gemm_sms_capped() { return g_gemm_sm_limit.load(std::memory_order_relaxed) > 0 && gemm_sms() < sm_count(); }
 int set_gemm_sm_limit(int n) { return g_gemm_sm_limit.exchange(n < 0 ? 0 : n); }
 
@@ -1155,11 +1156,12 @@ int read_moe_status(int* out, int reset);
 int read_indexer_status(int* out, int reset);
 int read_attn_status(int* out, int reset);
 int read_linear_few_status(int* out, int reset);
+int read_loss_status(int* out, int reset);
 
 // One word for the caller: the GEMM's code if it has one, else the quantisers', the exchange kernels', the indexer's,
-// the attention's, the few-row linear's.
+// the attention's, the few-row linear's, the cross entropy's.
 int read_device_status(int* out, int reset) {
-    int v = 0, q = 0, m = 0, x = 0, a = 0, f = 0;
+    int v = 0, q = 0, m = 0, x = 0, a = 0, f = 0, l = 0;
     CINN_CHECK_CUDA(cudaMemcpyFromSymbol(&v, g_device_status, sizeof(int)));
     if (reset && v != 0) {
         int z = 0;
@@ -1175,7 +1177,9 @@ int read_device_status(int* out, int reset) {
     if (rc) return rc;
     rc = read_linear_few_status(&f, reset);
     if (rc) return rc;
-    *out = v != 0 ? v : (q != 0 ? q : (m != 0 ? m : (x != 0 ? x : (a != 0 ? a : f))));
+    rc = read_loss_status(&l, reset);
+    if (rc) return rc;
+    *out = v != 0 ? v : (q != 0 ? q : (m != 0 ? m : (x != 0 ? x : (a != 0 ? a : (f != 0 ? f : l)))));
     return CINN_OK;
 }
 

@@ -1,0 +1,107 @@
+// Output projection + cross entropy (csrc/loss.cu): forward and backward as one native call each, and as a native autograd node.
+#include "host.h"
+
+namespace cinnhost {
+
+namespace {
+
+// rows of d elements as the kernels read them: contiguous, 16 bytes apart, on a 16-byte boundary
+Tensor rows_of(const Tensor& t) {
+    const bool fine = t.stride(1) == 1 && t.stride(0) % 8 == 0 && t.stride(0) >= t.size(1) && (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15) == 0;
+    return fine ? t : t.clone(at::MemoryFormat::Contiguous);
+}
+int64_t pitch(const Tensor& t) { return t.size(0) > 1 ? t.stride(0) : t.size(1); }
+
+// x (T, d), w (V, d) of one 16-bit type, d a multiple of 8; target (T,) int64; reduction 0 none, 1 mean, 2 sum.
+// -> loss (fp32, (T,) or ()), what the backward takes of the forward
+std::tuple<Tensor, Tensor> ce_forward(const Tensor& x, const Tensor& w, const Tensor& target, int64_t ignore, int64_t reduction) {
+    c10::cuda::CUDAGuard guard(x.device());
+    const int64_t T = x.size(0), d = x.size(1), V = w.size(0);
+    Tensor loss = reduction ? empty({}, at::kFloat, x.device()) : empty({T}, at::kFloat, x.device());
+    Tensor state = empty({api.cinn_linear_ce_state_bytes(T)}, at::kByte, x.device());
+    const int64_t need = api.cinn_linear_ce_workspace_bytes(T, V, d, 0);
+    Tensor ws = empty({need}, at::kByte, x.device());
+    check(api.cinn_linear_ce_forward(x.data_ptr(), pitch(x), w.data_ptr(), pitch(w), tag_of(x.scalar_type()), target.data_ptr<int64_t>(), ignore, T, V, d,
+                                     (int)reduction, f32(loss), state.data_ptr(), ws.data_ptr(), need, stream()), "cinn_linear_ce_forward");
+    return {loss, state};
+}
+
+std::tuple<Tensor, Tensor> ce_backward(const Tensor& grad, const Tensor& x, const Tensor& w, const Tensor& state, int64_t reduction, bool want_x, bool want_w) {
+    c10::cuda::CUDAGuard guard(x.device());
+    const int64_t T = x.size(0), d = x.size(1), V = w.size(0);
+    Tensor g = grad.to(at::kFloat).contiguous(), dx, dw;
+    if (want_x) dx = empty({T, d}, x.scalar_type(), x.device());
+    if (want_w) dw = empty({V, d}, w.scalar_type(), x.device());
+    const int64_t need = api.cinn_linear_ce_workspace_bytes(T, V, d, (want_x ? 1 : 0) | (want_w ? 2 : 0) | 4);
+    Tensor ws = empty({need}, at::kByte, x.device());
+    check(api.cinn_linear_ce_backward(x.data_ptr(), pitch(x), w.data_ptr(), pitch(w), tag_of(x.scalar_type()), f32(g), T, V, d, (int)reduction,
+                                      state.data_ptr(), want_x ? dx.data_ptr() : nullptr, want_w ? dw.data_ptr() : nullptr, ws.data_ptr(), need, stream()),
+          "cinn_linear_ce_backward");
+    return {dx, dw};
+}
+
+struct CrossEntropyNode : public torch::autograd::Function<CrossEntropyNode> {
+    static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& x_in, const Tensor& w_in, const Tensor& target, int64_t ignore,
+                          int64_t reduction) {
+        const Tensor x = rows_of(x_in), w = rows_of(w_in);
+        const auto [loss, state] = ce_forward(x, w, target, ignore, reduction);
+        ctx->save_for_backward({x, w, state});
+        ctx->saved_data["reduction"] = reduction;
+        return loss;
+    }
+    static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
+        auto s = ctx->get_saved_variables();
+        Tensor dx, dw;
+        as_python_error([&] {
+            require(!at::GradMode::is_enabled(), "linear_cross_entropy has no second derivative (create_graph=True)");
+            std::tie(dx, dw) = ce_backward(grads[0], s[0], s[1], s[2], ctx->saved_data["reduction"].toInt(), ctx->needs_input_grad(0),
+                                           ctx->needs_input_grad(1));
+        });
+        return {dx, dw, Tensor(), Tensor(), Tensor()};
+    }
+};
+
+// the operands in the type they are multiplied in, padded to whole 16 bytes; differentiable
+std::tuple<Tensor, Tensor, Tensor> ce_operands(const Tensor& x_in, const Tensor& w_in, const Tensor& target_in) {
+    require(x_in.is_cuda() && w_in.is_cuda() && target_in.is_cuda(), "Inputs must be on CUDA");
+    require(x_in.device() == w_in.device() && x_in.device() == target_in.device(), "linear_cross_entropy: x, weight and target must be on the same device");
+    require(x_in.dim() >= 1 && w_in.dim() == 2 && x_in.size(-1) == w_in.size(1), "linear_cross_entropy: x is (..., d) and weight (vocabulary, d)");
+    require(w_in.size(0) > 0 && w_in.size(1) > 0, "linear_cross_entropy: weight must not be empty");
+    require(target_in.scalar_type() == at::kLong || target_in.scalar_type() == at::kInt, "linear_cross_entropy: targets are int64 or int32");
+    require(target_in.sizes() == x_in.sizes().slice(0, x_in.dim() - 1), "linear_cross_entropy: target has one entry for every row of x");
+    Tensor x = x_in.reshape({-1, x_in.size(-1)}), w = w_in;
+    if (at::autocast::is_autocast_enabled(at::kCUDA)) {
+        const auto type = at::autocast::get_autocast_dtype(at::kCUDA);
+        x = x.to(type);
+        w = w.to(type);
+    }
+    const auto type = x.scalar_type();
+    require(type == w.scalar_type() && (type == at::kBFloat16 || type == at::kHalf),
+            "linear_cross_entropy multiplies 16-bit operands: x and weight must both be bfloat16 or both float16 (or autocast must make them so)");
+    const int64_t odd = x.size(1) % 8;
+    if (odd) {
+        x = at::constant_pad_nd(x, {0, 8 - odd});
+        w = at::constant_pad_nd(w, {0, 8 - odd});
+    }
+    return {x, w, target_in.reshape({-1}).to(at::kLong).contiguous()};
+}
+
+}  // namespace
+
+void bind_loss(pybind11::module_& m) {
+    m.def("linear_ce_operands", &ce_operands);
+    m.def("linear_ce_forward", [](const Tensor& x, const Tensor& w, const Tensor& target, int64_t ignore, int64_t reduction) {
+        return ce_forward(rows_of(x), rows_of(w), target, ignore, reduction);
+    });
+    m.def("linear_ce_backward", [](const Tensor& grad, const Tensor& x, const Tensor& w, const Tensor& state, int64_t reduction, bool want_x, bool want_w) {
+        return ce_backward(grad, rows_of(x), rows_of(w), state, reduction, want_x, want_w);
+    });
+    m.def("linear_cross_entropy", [](const Tensor& x_in, const Tensor& w_in, const Tensor& target_in, int64_t ignore, int64_t reduction) {
+        const auto [x, w, target] = ce_operands(x_in, w_in, target_in);
+        const Tensor loss = takes_node(x, w) ? CrossEntropyNode::apply(x, w, target, ignore, reduction)
+                                             : std::get<0>(ce_forward(rows_of(x), rows_of(w), target, ignore, reduction));
+        return reduction ? loss : loss.view(target_in.sizes());
+    });
+}
+
+}  // namespace cinnhost

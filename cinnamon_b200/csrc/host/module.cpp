@@ -8,6 +8,7 @@ void bind_linear(pybind11::module_& m);
 void bind_attention(pybind11::module_& m);
 void bind_moe(pybind11::module_& m);
 void bind_moe_train(pybind11::module_& m);
+void bind_loss(pybind11::module_& m);
 }  // namespace cinnhost
 
 PYBIND11_MODULE(_host, m) {
@@ -36,4 +37,5 @@ PYBIND11_MODULE(_host, m) {
     bind_attention(m);
     bind_moe(m);
     bind_moe_train(m);
+    bind_loss(m);
 }

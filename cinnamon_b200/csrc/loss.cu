@@ -1,0 +1,971 @@
+// Output projection and softmax cross entropy in one operator, forward and backward, without the logits in memory.
+//
+//   z = x W^T                      x (T, d), W (V, d), 16-bit operands, fp32 sums in tensor memory
+//   loss_t = log sum_v e^z_tv - z_t,target(t)
+//   dz_tv = g_t (e^(z_tv - lse_t) - [v = target(t)]),   dx = dz W,   dW = dz^T x
+//
+// Forward: a tile of 256 tokens x 256 words is multiplied by a pair of SMs and read out of tensor memory once, into a running
+// maximum and sum per token (two fp32 numbers); tiles of one run of words are joined in registers, runs by a small pass
+// at the end.  Backward: the words in pieces; a piece's product is made again, turned into dz in the epilogue and rounded to
+// the operands' type (bf16, or fp16 times 2^14, so that small probabilities keep their bits), and two products over the
+// piece add up dx (fp32, in L2) and write the piece's rows of dW.  So the work is 2 T V d forward and 6 T V d backward, one T V d more than
+// with kept logits, and the memory is that of one piece.
+//
+// Tokens whose target is ignored take part in nothing: the others' rows are gathered first (where none is ignored, x is read
+// as it is), so that what stands in ignored rows, infinities and NaN as well, reaches neither gradient, and half a batch of
+// prompts costs half.
+//
+// Sums, maxima and the two statistics per token are fp32; the logarithm of the sum is kept apart from the maximum, since
+// their sum would round away what e^(z - lse) - 1 of a well-predicted token is made of.
+#include "tcgen05.cuh"
+#include <algorithm>
+#include <cmath>
+
+namespace cinn {
+
+int gemm_sm_count();                       // SMs that the persistent kernels may take (gemm.cu)
+
+namespace ce {
+
+__device__ int g_status = 0;               // 0, or (role << 8) | reason of a bounded wait that ran out
+
+enum Mode { STATS = 0, SOFT = 1, DX = 2, DW = 3, DW_PART = 4 };
+
+constexpr int M = 256, N = 256;            // the pair's tile
+constexpr int KE = 64;                     // elements of a K block: 128 bytes
+constexpr int STAGES = 4;
+constexpr int SIDE = 128 * 128;            // bytes of one operand's stage in one CTA: 128 rows (or columns) x 64 elements
+constexpr int EPI = 8, COLS = 128;         // epilogue warps: four lane quarters x two halves of the columns
+constexpr int W_TMA = EPI, W_MMA = EPI + 1, W_STORE = EPI + 2;
+constexpr int THREADS = (EPI + 3) * 32;
+constexpr int BOX = 32 * 128;              // a TMA-store box: 32 rows of 128 bytes; two per epilogue warp
+constexpr int STAGE_BYTES = STAGES * 2 * SIDE;
+constexpr int C_BYTES = EPI * 2 * BOX;
+constexpr size_t SMEM_STATS = (size_t)STAGE_BYTES + 256 + 1024, SMEM = SMEM_STATS + C_BYTES;
+constexpr int GROUP = 16;                  // tiles of tokens that meet a run of words before the next ones do (L2)
+constexpr int SCAN = 1024;                 // tokens per CTA of the passes that gather
+constexpr float LOG2E = 1.4426950408889634f;
+constexpr float FP16_SCALE = 16384.0f;     // of dz in fp16: the smallest probability with all its bits is then 2^-28
+
+struct Params {
+    const int* n_valid;                    // rows in use (device)
+    int T, V, d;
+    int v0, vc;                            // the piece: its first word, how many
+    int parts;                             // STATS: runs of words per tile of tokens
+    int splits;                            // DX, DW_PART: pieces of the reduction, each with sums of its own
+    int rows_pad;                          // rows of one split's sums
+    int add;                               // DX: add to the sums of earlier pieces
+    int per_row;                           // SOFT: gradients per token (reduction "none")
+    int64_t part_ld;
+    float2* part;                          // STATS: (parts * 2, part_ld) maximum and sum
+    float* target_logit;
+    const int* target;                     // per row in use
+    const int* rows;                       // the token of every row in use
+    const float2* stat;                    // per row: maximum, log2 of the sum
+    const float* grad;                     // the loss's gradient: one number, or one per token
+    const unsigned* grad_max;              // the bits of the largest |gradient| (reduction "none")
+    int mean;
+};
+
+__device__ __forceinline__ bool wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, int code) {
+    return mbar_wait_bounded(bar, parity, abort_flag, code, &g_status);
+}
+__device__ __forceinline__ bool wait_warp(uint32_t bar, uint32_t parity, volatile int* abort_flag, int code) {
+    return __all_sync(0xffffffffu, wait(bar, parity, abort_flag, code));
+}
+__device__ __forceinline__ uint32_t cta_rank() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ uint32_t mapa(uint32_t addr, uint32_t rank) {
+    uint32_t r;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+    return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// relaxed: it hands over a buffer of tensor memory whose reads are complete (see gemm_pair.cuh)
+__device__ __forceinline__ void arrive_remote(uint32_t cluster_addr) {
+    asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
+__device__ __forceinline__ void load_2d(const CUtensorMap* map, uint32_t bar_cluster, uint32_t dst, int x, int y) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
+        ::"r"(dst), "l"(map), "r"(bar_cluster), "r"(x), "r"(y) : "memory");
+}
+__device__ __forceinline__ void add_2d(const CUtensorMap* map, uint32_t src, int x, int y) {
+    asm volatile("cp.reduce.async.bulk.tensor.2d.global.shared::cta.add.bulk_group [%0, {%2, %3}], [%1];"
+                 ::"l"(map), "r"(src), "r"(x), "r"(y) : "memory");
+}
+__device__ __forceinline__ void commit_pair(uint32_t own, uint32_t peer) {
+    asm volatile(
+        "{\n\t.reg .pred e;\n\t"
+        "elect.sync _|e, 0xffffffff;\n\t"
+        "@e tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t"
+        "@e tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%1];\n\t}"
+        ::"r"(own), "r"(peer) : "memory");
+}
+// The four steps of a K block by one election; low words of the descriptors, STEP in units of 16 bytes.
+template <int STEP_A, int STEP_B>
+__device__ __forceinline__ void mma_block(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, bool fresh) {
+    asm volatile(
+        "{\n\t.reg .pred p, e;\n\t.reg .b64 a, b;\n\t.reg .b32 x, y;\n\t"
+        "elect.sync _|e, 0xffffffff;\n\t"
+        "setp.ne.b32 p, %5, 0;\n\t"
+        "mov.b64 a, {%1, %4};\n\tmov.b64 b, {%2, %4};\n\t"
+        "@e tcgen05.mma.cta_group::2.kind::f16 [%0], a, b, %3, p;\n\t"
+        "add.u32 x, %1, %6;\n\tadd.u32 y, %2, %7;\n\tmov.b64 a, {x, %4};\n\tmov.b64 b, {y, %4};\n\t"
+        "@e tcgen05.mma.cta_group::2.kind::f16 [%0], a, b, %3, 1;\n\t"
+        "add.u32 x, %1, %8;\n\tadd.u32 y, %2, %9;\n\tmov.b64 a, {x, %4};\n\tmov.b64 b, {y, %4};\n\t"
+        "@e tcgen05.mma.cta_group::2.kind::f16 [%0], a, b, %3, 1;\n\t"
+        "add.u32 x, %1, %10;\n\tadd.u32 y, %2, %11;\n\tmov.b64 a, {x, %4};\n\tmov.b64 b, {y, %4};\n\t"
+        "@e tcgen05.mma.cta_group::2.kind::f16 [%0], a, b, %3, 1;\n\t}"
+        ::"r"(d), "r"(a), "r"(b), "r"(idesc), "r"(DESC_HI), "r"(fresh ? 0u : 1u), "n"(STEP_A), "n"(STEP_B), "n"(2 * STEP_A), "n"(2 * STEP_B),
+          "n"(3 * STEP_A), "n"(3 * STEP_B) : "memory");
+}
+__device__ __forceinline__ void ld32(uint32_t taddr, uint32_t (&r)[32]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, "
+        "%19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+          "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]),
+          "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]),
+          "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(taddr));
+}
+__device__ __forceinline__ void ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ float exp2_approx(float x) {          // relative error 2^-22; a result below 2^-126 is 0
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+template <bool BF16>
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+    if constexpr (BF16) {
+        const __nv_bfloat162 t = __floats2bfloat162_rn(a, b);
+        return *reinterpret_cast<const uint32_t*>(&t);
+    } else {
+        const __half2 t = __floats2half2_rn(a, b);
+        return *reinterpret_cast<const uint32_t*>(&t);
+    }
+}
+
+// What the gradients are multiplied by once their sums are complete: the loss's gradient (over the number of targets for a
+// mean), or the largest of the tokens' gradients, to which SOFT has related each.
+__device__ __forceinline__ float final_scale(const Params& p, bool bf16) {
+    const float s = p.per_row ? __uint_as_float(*p.grad_max) : p.mean ? *p.grad / (float)*p.n_valid : *p.grad;
+    return bf16 ? s : s * (1.0f / FP16_SCALE);
+}
+
+struct Unit { int m0, n_first, n_last, kb0, KB, split; };
+
+// Work of one cluster at a time: a tile (a run of them along the words for STATS).  Groups of GROUP row tiles, rows fastest inside.
+template <int MODE>
+__device__ __forceinline__ int unit_count(const Params& p, int valid) {
+    const int rows = MODE >= DW ? p.vc : valid, cols = MODE == STATS ? p.V : MODE == SOFT ? p.vc : p.d;
+    const int tiles = ((rows + M - 1) / M) * (MODE == STATS ? p.parts : (cols + N - 1) / N);
+    return (MODE == DX || MODE == DW_PART) ? tiles * p.splits : tiles;
+}
+template <int MODE>
+__device__ __forceinline__ Unit unit_at(const Params& p, int valid, int u) {
+    const int rows = MODE >= DW ? p.vc : valid, cols = MODE == STATS ? p.V : MODE == SOFT ? p.vc : p.d;
+    const int m_tiles = (rows + M - 1) / M, n_tiles = (cols + N - 1) / N, across = MODE == STATS ? p.parts : n_tiles;
+    const int red = MODE == DX ? p.vc : MODE >= DW ? valid : p.d, blocks = (red + KE - 1) / KE;
+    Unit r;
+    r.split = 0; r.kb0 = 0; r.KB = blocks;
+    if constexpr (MODE == DX || MODE == DW_PART) {
+        r.split = u / (m_tiles * across);
+        u -= r.split * (m_tiles * across);
+        r.kb0 = (int)((int64_t)blocks * r.split / p.splits);
+        r.KB = (int)((int64_t)blocks * (r.split + 1) / p.splits) - r.kb0;
+    }
+    const int g = u / (GROUP * across), first = g * GROUP, size = min(GROUP, m_tiles - first);
+    const int in = u - g * GROUP * across, n = in / size;
+    r.m0 = (first + in - n * size) * M;
+    if constexpr (MODE == STATS) {
+        r.n_first = (int)((int64_t)n_tiles * n / p.parts);
+        r.n_last = (int)((int64_t)n_tiles * (n + 1) / p.parts);
+    } else {
+        r.n_first = n; r.n_last = n + 1;
+    }
+    return r;
+}
+
+// A: x (STATS, SOFT) or dz (DX: as stored; DW: its transpose, MN-major);  B: W (STATS, SOFT: as stored; DX: MN-major) or x (DW, MN-major).
+// xg: x's rows in use, gathered; read in x's place where some token is ignored.
+template <int MODE, bool BF16>
+__global__ void __launch_bounds__(THREADS, 1)
+product_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b, const __grid_constant__ CUtensorMap tm_xg,
+               const __grid_constant__ CUtensorMap tm_c, const Params p) {
+    constexpr bool A_MN = MODE >= DW, B_MN = MODE >= DX;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+    uint8_t* smem_a = smem;
+    uint8_t* smem_b = smem + STAGES * SIDE;
+    uint8_t* c_stage = smem + STAGE_BYTES;
+    uint64_t* bars = reinterpret_cast<uint64_t*>(c_stage + (MODE == STATS ? 0 : C_BYTES));
+    // [0, S) full (used in the leader), [S, 2S) empty, then: tensor memory full (2), empty (2, leader), boxes staged, boxes taken
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * STAGES + 6);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t rank = cta_rank();
+    const uint32_t full0 = smem_u32(bars), empty0 = smem_u32(bars + STAGES);
+    const uint32_t tfull0 = smem_u32(bars + 2 * STAGES), tempty0 = smem_u32(bars + 2 * STAGES + 2);
+    const uint32_t staged = smem_u32(bars + 2 * STAGES + 4), taken = smem_u32(bars + 2 * STAGES + 5);
+
+    if (threadIdx.x == 0) *abort_flag = 0;
+    if (warp == W_TMA && lane == 0) {
+        for (int s = 0; s < STAGES; ++s) { mbar_init(full0 + 8 * s, 1); mbar_init(empty0 + 8 * s, 1); }
+        for (int b = 0; b < 2; ++b) { mbar_init(tfull0 + 8 * b, 1); mbar_init(tempty0 + 8 * b, 2 * EPI); }
+        mbar_init(staged, EPI);
+        mbar_init(taken, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == W_MMA) {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(512) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    }
+    pdl_wait();
+    if (warp == W_MMA) pdl_trigger();
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+    const int valid = *p.n_valid;
+    const int n_units = unit_count<MODE>(p, valid);
+    const int cluster = blockIdx.x >> 1, n_clusters = gridDim.x >> 1;
+
+    if (warp == W_TMA) {
+        // ------------------------------ TMA producer (both CTAs) ------------------------------
+        if (lane == 0) {
+            const uint32_t full_leader = mapa(full0, 0);
+            const CUtensorMap* map_a = (MODE <= SOFT && valid != p.T) ? &tm_xg : &tm_a;
+            const CUtensorMap* map_b = (MODE >= DW && valid != p.T) ? &tm_xg : &tm_b;
+            uint32_t it = 0;
+            bool alive = true;
+            for (int u = cluster; u < n_units && alive; u += n_clusters) {
+                const Unit w = unit_at<MODE>(p, valid, u);
+                for (int nt = w.n_first; nt < w.n_last && alive; ++nt) {
+                    const int ma = w.m0 + 128 * (int)rank, nb = nt * N + 128 * (int)rank;
+                    for (int kb = 0; kb < w.KB; ++kb, ++it) {
+                        const int s = it % STAGES;
+                        if (!wait(empty0 + 8 * s, (it / STAGES & 1) ^ 1, abort_flag, (11 << 8) | 1)) { alive = false; break; }
+                        if (rank == 0) mbar_expect_tx(full0 + 8 * s, 4 * SIDE);
+                        const uint32_t bar = full_leader + 8 * s, da = smem_u32(smem_a + s * SIDE), db = smem_u32(smem_b + s * SIDE);
+                        const int k = (w.kb0 + kb) * KE;
+                        if constexpr (!A_MN) {
+                            load_2d(map_a, bar, da, k, ma);
+                        } else {
+                            load_2d(map_a, bar, da, ma, k);
+                            load_2d(map_a, bar, da + SIDE / 2, ma + 64, k);
+                        }
+                        if constexpr (!B_MN) {
+                            load_2d(map_b, bar, db, k, p.v0 + nb);
+                        } else {
+                            const int y = MODE == DX ? p.v0 + k : k;
+                            load_2d(map_b, bar, db, nb, y);
+                            load_2d(map_b, bar, db + SIDE / 2, nb + 64, y);
+                        }
+                    }
+                }
+            }
+            if (!alive) {                  // abandoned: time for the copies already issued to land
+                const long long t0 = clock64();
+                while (clock64() - t0 < 2000000LL) { }
+            }
+        }
+    } else if (warp == W_MMA) {
+        // ------------------------------ MMA issuer (leader; a whole warp, one elected lane) ------------------------------
+        if (rank == 0) {
+            constexpr uint32_t idesc = make_idesc_f16(BF16, M, N, A_MN, B_MN);
+            // K-major: a step of 16 elements is 32 bytes of the row.  MN-major: 16 rows of 128 bytes; the second 64 columns are a panel
+            // of their own, SIDE / 2 bytes on (the leading offset).
+            constexpr uint32_t LEAD = (SIDE / 2) >> 4;
+            const uint32_t a0 = ((smem_u32(smem_a) >> 4) & 0x3FFF) | ((A_MN ? LEAD : 1u) << 16);
+            const uint32_t b0 = ((smem_u32(smem_b) >> 4) & 0x3FFF) | ((B_MN ? LEAD : 1u) << 16);
+            const uint32_t tfull_own = mapa(tfull0, 0), tfull_peer = mapa(tfull0, 1);
+            const uint32_t empty_own = mapa(empty0, 0), empty_peer = mapa(empty0, 1);
+            uint32_t it = 0, tile = 0;
+            bool alive = true;
+            for (int u = cluster; u < n_units && alive; u += n_clusters) {
+                const Unit w = unit_at<MODE>(p, valid, u);
+                for (int nt = w.n_first; nt < w.n_last && alive; ++nt, ++tile) {
+                    const uint32_t b = tile & 1;
+                    if (!wait_warp(tempty0 + 8 * b, (tile >> 1 & 1) ^ 1, abort_flag, (12 << 8) | 2)) { alive = false; break; }
+                    tc_fence_after();
+                    for (int kb = 0; kb < w.KB; ++kb, ++it) {
+                        const uint32_t s = it % STAGES;
+                        if (!wait_warp(full0 + 8 * s, it / STAGES & 1, abort_flag, (12 << 8) | 1)) { alive = false; break; }
+                        tc_fence_after();
+                        mma_block<A_MN ? 128 : 2, B_MN ? 128 : 2>(tmem + b * N, a0 + s * (SIDE >> 4), b0 + s * (SIDE >> 4), idesc, kb == 0);
+                        commit_pair(empty_own + 8 * s, empty_peer + 8 * s);
+                    }
+                    if (!alive) break;
+                    commit_pair(tfull_own + 8 * b, tfull_peer + 8 * b);
+                }
+            }
+            // every MMA issued above must have retired before tensor memory is freed
+            if (alive && tile) wait(tfull0 + 8 * ((tile - 1) & 1), (tile - 1) >> 1 & 1, abort_flag, (12 << 8) | 3);
+        }
+    } else if (warp == W_STORE) {
+        // ------------------------------ finished boxes to the TMA unit (both CTAs) ------------------------------
+        if constexpr (MODE != STATS) {
+            constexpr bool F32 = MODE == DX || MODE == DW_PART;
+            constexpr int PER = F32 ? 32 : 64, ROUNDS = COLS / (2 * PER);        // elements of a box's row; rounds of a tile
+            const int w = lane >> 1, q = w & 3, h = w >> 2;
+            const int out_cols = MODE == SOFT ? p.vc : p.d;
+            uint32_t round = 0;
+            bool alive = true;
+            for (int u = cluster; u < n_units && alive; u += n_clusters) {
+                const Unit t = unit_at<MODE>(p, valid, u);
+                const int row = t.m0 + 128 * (int)rank + q * 32;
+                for (int r = 0; r < ROUNDS; ++r, ++round) {
+                    const int col = t.n_first * N + h * COLS + (r * 2 + (lane & 1)) * PER;
+                    if (!wait_warp(staged, round & 1, abort_flag, (14 << 8) | 1)) { alive = false; break; }
+                    if (lane < 2 * EPI) {
+                        const uint32_t box = smem_u32(c_stage) + lane * BOX;
+                        if (col < out_cols && (MODE != DW || p.v0 + row < p.V)) {
+                            if constexpr (F32) {
+                                if (p.add) add_2d(&tm_c, box, col, t.split * p.rows_pad + row);
+                                else tma_store_2d(&tm_c, box, col, t.split * p.rows_pad + row);
+                            } else {
+                                tma_store_2d(&tm_c, box, col, (MODE == DW ? p.v0 : 0) + row);
+                            }
+                        }
+                        tma_store_commit();
+                        tma_store_wait_read();
+                    }
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(taken);
+                }
+            }
+            if (lane < 2 * EPI) tma_store_wait_all();
+        }
+    } else {
+        // ------------------------------ epilogue (both CTAs) ------------------------------
+        const int q = warp & 3, h = warp >> 2;
+        const uint32_t tempty_leader = mapa(tempty0, 0);
+        uint32_t tile = 0, round = 0;
+        bool alive = true;
+        float scale = 1.0f;
+        if constexpr (MODE == DW) scale = final_scale(p, BF16);
+        float rel_of = 1.0f;                               // SOFT, gradients per token: one over the largest
+        if constexpr (MODE == SOFT) {
+            if (p.per_row) {
+                const float most = __uint_as_float(*p.grad_max);
+                rel_of = most == 0.0f ? 0.0f : most;
+            }
+        }
+        for (int u = cluster; u < n_units && alive; u += n_clusters) {
+            const Unit w = unit_at<MODE>(p, valid, u);
+            const int row = w.m0 + 128 * (int)rank + q * 32 + lane;
+            const bool live = row < valid;
+            float mx = -INFINITY, sum = 0.0f, rel = 0.0f;
+            int target = -1;
+            if constexpr (MODE == STATS) {
+                if (live) target = p.target[row];
+            }
+            if constexpr (MODE == SOFT) {
+                if (live) {
+                    const float2 st = p.stat[row];
+                    mx = st.x; sum = st.y;
+                    target = p.target[row];
+                    rel = p.per_row ? (rel_of == 0.0f ? 0.0f : p.grad[p.rows[row]] / rel_of) : 1.0f;
+                    if (!BF16) rel *= FP16_SCALE;
+                }
+            }
+            for (int nt = w.n_first; nt < w.n_last; ++nt, ++tile) {
+                const uint32_t b = tile & 1;
+                if (!wait_warp(tfull0 + 8 * b, tile >> 1 & 1, abort_flag, (13 << 8) | 1)) { alive = false; break; }
+                tc_fence_after();
+                const uint32_t taddr = tmem + ((uint32_t)(q * 32) << 16) + b * N + h * COLS;
+                const int col0 = (MODE == STATS || MODE == SOFT ? p.v0 : 0) + nt * N + h * COLS;      // of this warp, among all words
+                if constexpr (MODE == STATS) {
+#pragma unroll 1
+                    for (int c = 0; c < COLS / 32; ++c) {
+                        uint32_t r[32];
+                        ld32(taddr + c * 32, r);
+                        ld_wait();
+                        const int at = col0 + c * 32;
+                        if (at >= p.V) break;
+                        const int hit = target - at;
+                        if ((unsigned)hit < 32u) {
+                            float z = 0.0f;
+#pragma unroll
+                            for (int j = 0; j < 32; ++j) z = j == hit ? __uint_as_float(r[j]) : z;
+                            p.target_logit[row] = z;
+                        }
+                        if (at + 32 > p.V) {               // words past the last one
+#pragma unroll
+                            for (int j = 0; j < 32; ++j)
+                                if (at + j >= p.V) r[j] = __float_as_uint(-INFINITY);
+                        }
+                        float top = mx;
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) top = fmaxf(top, __uint_as_float(r[j]));
+                        const float base = top == -INFINITY ? 0.0f : top;
+                        float part[4] = {sum * exp2_approx((mx - base) * LOG2E), 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) part[j & 3] += exp2_approx((__uint_as_float(r[j]) - base) * LOG2E);
+                        sum = (part[0] + part[1]) + (part[2] + part[3]);
+                        mx = top;
+                    }
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) arrive_remote(tempty_leader + 8 * b);
+                } else if constexpr (MODE == SOFT || MODE == DW) {
+                    const uint32_t slot = smem_u32(c_stage) + warp * 2 * BOX;
+                    if (!wait_warp(taken, (round & 1) ^ 1, abort_flag, (13 << 8) | 2)) { alive = false; break; }
+#pragma unroll
+                    for (int c = 0; c < COLS / 32; ++c) {
+                        uint32_t r[32];
+                        ld32(taddr + c * 32, r);
+                        ld_wait();
+                        if constexpr (MODE == SOFT) {
+                            const int hit = target - (col0 + c * 32);
+                            const int left = p.v0 + p.vc - (col0 + c * 32);        // words of the piece from here on
+#pragma unroll
+                            for (int j = 0; j < 32; ++j) r[j] = __float_as_uint(exp2_approx((__uint_as_float(r[j]) - mx) * LOG2E - sum));
+                            if ((unsigned)hit < 32u) {
+#pragma unroll
+                                for (int j = 0; j < 32; ++j)
+                                    if (j == hit) r[j] = __float_as_uint(__uint_as_float(r[j]) - 1.0f);
+                            }
+#pragma unroll
+                            for (int j = 0; j < 32; ++j) r[j] = __float_as_uint(__uint_as_float(r[j]) * rel);
+                            if (!live || left < 32) {
+#pragma unroll
+                                for (int j = 0; j < 32; ++j)
+                                    if (!live || j >= left) r[j] = 0u;
+                            }
+                        } else {
+#pragma unroll
+                            for (int j = 0; j < 32; ++j) r[j] = w.KB ? __float_as_uint(__uint_as_float(r[j]) * scale) : 0u;
+                        }
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {      // 16 bytes: 8 elements
+                            uint32_t v[4];
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) v[i] = pack2<BF16>(__uint_as_float(r[j * 8 + 2 * i]), __uint_as_float(r[j * 8 + 2 * i + 1]));
+                            const int chunk = (c & 1) * 4 + j;
+                            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};"
+                                         ::"r"(slot + (c >> 1) * BOX + lane * 128 + ((chunk ^ (lane & 7)) << 4)), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]) : "memory");
+                        }
+                    }
+                    tc_fence_before();
+                    fence_async_smem();
+                    __syncwarp();
+                    if (lane == 0) { arrive_remote(tempty_leader + 8 * b); mbar_arrive(staged); }
+                    ++round;
+                } else {
+                    const uint32_t slot = smem_u32(c_stage) + warp * 2 * BOX;
+#pragma unroll
+                    for (int half = 0; half < 2; ++half, ++round) {
+                        if (!wait_warp(taken, (round & 1) ^ 1, abort_flag, (13 << 8) | 2)) { alive = false; break; }
+#pragma unroll
+                        for (int c = 0; c < 2; ++c) {
+                            uint32_t r[32];
+                            ld32(taddr + half * 64 + c * 32, r);
+                            ld_wait();
+#pragma unroll
+                            for (int j = 0; j < 8; ++j) {
+                                if (!w.KB) r[4 * j] = r[4 * j + 1] = r[4 * j + 2] = r[4 * j + 3] = 0u;
+                                asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};"
+                                             ::"r"(slot + c * BOX + lane * 128 + ((j ^ (lane & 7)) << 4)), "r"(r[4 * j]), "r"(r[4 * j + 1]), "r"(r[4 * j + 2]), "r"(r[4 * j + 3]) : "memory");
+                            }
+                        }
+                        if (half == 1) tc_fence_before();
+                        fence_async_smem();
+                        __syncwarp();
+                        if (lane == 0) {
+                            if (half == 1) arrive_remote(tempty_leader + 8 * b);
+                            mbar_arrive(staged);
+                        }
+                    }
+                    if (!alive) break;
+                }
+            }
+            if constexpr (MODE == STATS) {
+                // (a part holds two halves of the columns, each a warp's)
+                const int across = p.parts, m_tiles = (valid + M - 1) / M;
+                const int g = u / (GROUP * across), size = min(GROUP, m_tiles - g * GROUP);
+                const int n = (u - g * GROUP * across) / size;
+                if (alive && live) p.part[(int64_t)(n * 2 + h) * p.part_ld + row] = make_float2(mx, sum);
+            }
+        }
+    }
+
+    // nobody leaves while the other CTA may still read this CTA's shared memory or signal its barriers
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync();
+    if (warp == W_MMA) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+    }
+}
+
+// ---------------------------------------------------------------------------------------------------------------------
+// rows in use
+// ---------------------------------------------------------------------------------------------------------------------
+struct State {                             // what the forward leaves for the backward (one allocation of the caller's)
+    int* n_valid;                          // [0] rows in use, [1] a ticket of the pass that adds up the losses
+    int* rows;                             // the token of every row in use
+    int* slot;                             // the row of every token; -1: ignored, -2: a target that is no word
+    int* target;                           // per row in use
+    float2* stat;                          // per row: maximum and log2 of the sum
+};
+
+__device__ __forceinline__ int slot_kind(int64_t t, int64_t ignore, int V) { return t == ignore ? -1 : (t < 0 || t >= V) ? -2 : 0; }
+
+__global__ void __launch_bounds__(SCAN)
+count_kernel(const int64_t* __restrict__ target, int T, int64_t ignore, int V, int* __restrict__ counts) {
+    pdl_wait();
+    pdl_trigger();
+    const int t = blockIdx.x * SCAN + threadIdx.x;
+    const int n = __syncthreads_count(t < T && slot_kind(target[t < T ? t : 0], ignore, V) == 0);
+    if (threadIdx.x == 0) counts[blockIdx.x] = n;
+}
+
+// counts: of all blocks; null with a single one
+__global__ void __launch_bounds__(SCAN)
+place_kernel(const int64_t* __restrict__ target, int T, int64_t ignore, int V, const int* __restrict__ counts, State s) {
+    pdl_wait();
+    pdl_trigger();
+    __shared__ int s_warp[32], s_base;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, t = blockIdx.x * SCAN + threadIdx.x;
+    int before = 0;
+    if (counts) {
+        int mine = 0;
+        for (int b = threadIdx.x; b < (int)blockIdx.x; b += SCAN) mine += counts[b];
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
+        if (lane == 0) s_warp[warp] = mine;
+        __syncthreads();
+        if (threadIdx.x == 0) {
+            int sum = 0;
+            for (int w = 0; w < 32; ++w) sum += s_warp[w];
+            s_base = sum;
+        }
+        __syncthreads();
+        before = s_base;
+    }
+    const int64_t goal = t < T ? target[t] : ignore;
+    const int kind = t < T ? slot_kind(goal, ignore, V) : -1;
+    const unsigned has = __ballot_sync(0xffffffffu, kind == 0);
+    if (lane == 0) s_warp[warp] = __popc(has);
+    __syncthreads();
+    int in_block = 0;
+    for (int w = 0; w < warp; ++w) in_block += s_warp[w];
+    const int row = before + in_block + __popc(has & ((1u << lane) - 1u));
+    if (t < T) s.slot[t] = kind == 0 ? row : kind;
+    if (kind == 0) { s.rows[row] = t; s.target[row] = (int)goal; }
+    if (blockIdx.x == gridDim.x - 1 && threadIdx.x == SCAN - 1) {
+        s.n_valid[0] = row + (kind == 0);
+        s.n_valid[1] = 0;
+    }
+}
+
+// x's rows in use, one after the other, and zeros up to a whole K block behind them (dz^T x reduces over rows: nothing else may
+// stand there).  Where every token is in use nothing is copied: x itself is read.
+__global__ void __launch_bounds__(256)
+gather_kernel(const uint4* __restrict__ x, int64_t ld, int T, int vecs, const int* __restrict__ n_valid, const int* __restrict__ rows,
+              uint4* __restrict__ out) {
+    pdl_wait();
+    pdl_trigger();
+    const int valid = *n_valid;
+    if (valid == T) return;
+    const int padded = (valid + KE - 1) / KE * KE;
+    const int64_t n = (int64_t)padded * vecs;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
+        const int r = (int)(i / vecs), c = (int)(i - (int64_t)r * vecs);
+        out[i] = r < valid ? x[(int64_t)rows[r] * ld + c] : make_uint4(0, 0, 0, 0);
+    }
+}
+
+// ---------------------------------------------------------------------------------------------------------------------
+// loss
+// ---------------------------------------------------------------------------------------------------------------------
+// Per token: the runs' maxima and sums joined, in their order; the loss; and for a sum or mean the blocks' sums, added up in 64 bits
+// and in their order by the block that comes last.
+__global__ void __launch_bounds__(128)
+loss_kernel(const float2* __restrict__ part, int64_t part_ld, int parts, const float* __restrict__ target_logit, State s, int T, int reduction,
+            double* __restrict__ block_sum, float* __restrict__ loss) {
+    pdl_wait();
+    pdl_trigger();
+    __shared__ double s_sum[4];
+    __shared__ bool s_last;
+    const int t = blockIdx.x * 128 + threadIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    double mine = 0.0;
+    if (t < T) {
+        const int row = s.slot[t];
+        float l = row == -2 ? NAN : 0.0f;
+        if (row >= 0) {
+            float mx = -INFINITY, sum = 0.0f;
+#pragma unroll 4
+            for (int i = 0; i < parts; ++i) {
+                const float2 v = part[(int64_t)i * part_ld + row];
+                const float top = fmaxf(mx, v.x), base = top == -INFINITY ? 0.0f : top;
+                sum = sum * exp2f((mx - base) * LOG2E) + v.y * exp2f((v.x - base) * LOG2E);
+                mx = top;
+            }
+            s.stat[row] = make_float2(mx, log2f(sum));
+            l = (mx - target_logit[row]) + logf(sum);
+        }
+        if (reduction == 0) loss[t] = l;
+        mine = l;
+    }
+    if (reduction == 0) return;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
+    if (lane == 0) s_sum[warp] = mine;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        block_sum[blockIdx.x] = (s_sum[0] + s_sum[1]) + (s_sum[2] + s_sum[3]);
+        __threadfence();
+        s_last = atomicAdd(&s.n_valid[1], 1) == (int)gridDim.x - 1;
+    }
+    __syncthreads();
+    if (!s_last) return;
+    __threadfence();
+    mine = 0.0;
+    for (int b = threadIdx.x; b < (int)gridDim.x; b += 128) mine += __ldcg(block_sum + b);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
+    if (lane == 0) s_sum[warp] = mine;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        const double total = (s_sum[0] + s_sum[1]) + (s_sum[2] + s_sum[3]);
+        *loss = (float)(reduction == 1 ? total / (double)s.n_valid[0] : total);
+    }
+}
+
+// ---------------------------------------------------------------------------------------------------------------------
+// gradients: what is left when the products are done
+// ---------------------------------------------------------------------------------------------------------------------
+// the largest |gradient| among the tokens in use, as bits (a NaN is larger than any number); *out starts at 0
+__global__ void __launch_bounds__(256)
+grad_max_kernel(const float* __restrict__ grad, const int* __restrict__ slot, int T, unsigned* __restrict__ out) {
+    pdl_wait();
+    pdl_trigger();
+    unsigned most = 0;
+    for (int t = blockIdx.x * 256 + threadIdx.x; t < T; t += gridDim.x * 256)
+        if (slot[t] >= 0) most = max(most, __float_as_uint(fabsf(grad[t])));
+    most = __reduce_max_sync(0xffffffffu, most);
+    if ((threadIdx.x & 31) == 0 && most) atomicMax(out, most);
+}
+
+// out[r] = scale * sum of the splits' sums of r's row, rounded once; slot (null: every row its own) -1 or -2: zeros
+template <bool BF16>
+__global__ void __launch_bounds__(256)
+finish_kernel(const float* __restrict__ sums, int splits, int64_t split_elems, int rows, int d, const int* __restrict__ slot, const Params p,
+              uint2* __restrict__ out) {
+    pdl_wait();
+    pdl_trigger();
+    const int vecs = d / 4;
+    const int64_t n = (int64_t)rows * vecs;
+    const float scale = final_scale(p, BF16);
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
+        const int r = (int)(i / vecs), c = (int)(i - (int64_t)r * vecs);
+        const int from = slot ? slot[r] : r;
+        float4 a = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (from >= 0) {
+            const float* at = sums + (int64_t)from * d + c * 4;
+            a = *reinterpret_cast<const float4*>(at);
+            for (int s = 1; s < splits; ++s) {
+                const float4 b = *reinterpret_cast<const float4*>(at + s * split_elems);
+                a.x += b.x; a.y += b.y; a.z += b.z; a.w += b.w;
+            }
+            a.x *= scale; a.y *= scale; a.z *= scale; a.w *= scale;
+        }
+        out[i] = make_uint2(pack2<BF16>(a.x, a.y), pack2<BF16>(a.z, a.w));
+    }
+}
+
+// ---------------------------------------------------------------------------------------------------------------------
+// plans
+// ---------------------------------------------------------------------------------------------------------------------
+static inline int64_t up(int64_t v, int64_t a) { return (v + a - 1) / a * a; }
+static inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+struct Plan {
+    int64_t T, V, d, Tp;                   // Tp: T in whole tiles
+    int clusters, parts;
+    int64_t vc;                            // words of a piece
+    int pieces, dx_splits, dw_splits;
+    int64_t dz_ld;
+};
+
+constexpr int64_t DZ_BYTES = 512LL << 20;  // most of a piece of dz: smaller pieces cost passes over dx, larger ones only memory
+
+static Plan make_plan(int64_t T, int64_t V, int64_t d) {
+    Plan r{};
+    r.T = T; r.V = V; r.d = d; r.Tp = up(T, M);
+    r.clusters = std::max(1, sm_count() / 2);          // (not those under a cap: sizes must not change between two calls)
+    const int64_t m_tiles = r.Tp / M, n_tiles = ceil_div(V, N), n_d = ceil_div(d, N);
+    // runs of words: as long as leaves every cluster some sixteen of them, for an even end
+    r.parts = (int)std::min<int64_t>(n_tiles, std::max<int64_t>(ceil_div(n_tiles, 16), ceil_div(16 * r.clusters, m_tiles)));
+    const int64_t fit = std::max<int64_t>(N, DZ_BYTES / (2 * r.Tp) / N * N);
+    r.pieces = (int)ceil_div(V, fit);
+    r.vc = up(ceil_div(V, r.pieces), N);   // equal pieces, in whole tiles
+    r.pieces = (int)ceil_div(V, r.vc);
+    r.dz_ld = up(std::min(r.vc, V), KE);
+    // reductions cut where their tiles would leave SMs idle, down to 16 K blocks a piece
+    auto cut = [&](int64_t tiles, int64_t blocks) {
+        return (int)std::max<int64_t>(1, std::min<int64_t>({(int64_t)r.clusters / std::max<int64_t>(1, tiles), blocks / 16, (int64_t)16}));
+    };
+    r.dx_splits = cut(m_tiles * n_d, ceil_div(std::min(r.vc, V), KE));
+    r.dw_splits = r.pieces > 1 ? 1 : cut(n_tiles * n_d, ceil_div(T, KE));
+    return r;
+}
+
+struct Carver {                            // sub-allocations of one workspace, 256 bytes apart
+    uint8_t* base;
+    int64_t used = 0;
+    void* take(int64_t bytes) { void* at = base ? base + used : nullptr; used += up(bytes, 256); return at; }
+};
+
+static State carve_state(void* mem, int64_t T, int64_t* bytes) {
+    Carver c{static_cast<uint8_t*>(mem)};
+    State s;
+    s.n_valid = static_cast<int*>(c.take(8));
+    s.rows = static_cast<int*>(c.take(4 * T));
+    s.slot = static_cast<int*>(c.take(4 * T));
+    s.target = static_cast<int*>(c.take(4 * T));
+    s.stat = static_cast<float2*>(c.take(8 * T));
+    if (bytes) *bytes = c.used;
+    return s;
+}
+
+struct Forward { int* counts; void* xg; float2* part; float* target_logit; double* block_sum; };
+static Forward carve_forward(void* mem, const Plan& r, int64_t* bytes) {
+    Carver c{static_cast<uint8_t*>(mem)};
+    Forward f;
+    f.counts = static_cast<int*>(c.take(4 * ceil_div(r.T, SCAN)));
+    f.xg = c.take(up(r.T, KE) * r.d * 2);
+    f.part = static_cast<float2*>(c.take(8LL * 2 * r.parts * r.Tp));
+    f.target_logit = static_cast<float*>(c.take(4 * r.T));
+    f.block_sum = static_cast<double*>(c.take(8 * ceil_div(r.T, 128)));
+    if (bytes) *bytes = c.used;
+    return f;
+}
+struct Backward { void *xg, *dz; float *dx, *dw; unsigned* grad_max; };
+static Backward carve_backward(void* mem, const Plan& r, bool want_dx, bool want_dw, int64_t* bytes) {
+    Carver c{static_cast<uint8_t*>(mem)};
+    Backward b;
+    b.grad_max = static_cast<unsigned*>(c.take(4));
+    b.xg = c.take(up(r.T, KE) * r.d * 2);
+    b.dz = c.take(r.Tp * r.dz_ld * 2);
+    b.dx = static_cast<float*>(c.take(want_dx ? 4 * r.dx_splits * r.Tp * r.d : 0));
+    b.dw = static_cast<float*>(c.take(want_dw && r.dw_splits > 1 ? 4 * r.dw_splits * up(r.V, M) * r.d : 0));
+    if (bytes) *bytes = c.used;
+    return b;
+}
+
+template <int MODE, bool BF16>
+static int launch(const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& xg, const CUtensorMap& c, const Params& p, cudaStream_t st) {
+    constexpr auto kern = product_kernel<MODE, BF16>;
+    constexpr size_t smem = MODE == STATS ? SMEM_STATS : SMEM;
+    int rc = allow_smem_once<kern>(smem);
+    if (rc) return rc;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(2 * std::max(1, gemm_sm_count() / 2)); cfg.blockDim = dim3(THREADS); cfg.dynamicSmemBytes = smem; cfg.stream = st;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = 2; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr; cfg.numAttrs = 2;
+    CINN_CHECK_CUDA(cudaLaunchKernelEx(&cfg, kern, a, b, xg, c, p));
+    CINN_CHECK_LAUNCH();
+    return CINN_OK;
+}
+
+static int map16(CUtensorMap* m, const void* base, int64_t inner, int64_t rows, int64_t ld, int box_rows, bool bf16) {
+    return encode_map_2d(m, base, (uint64_t)inner, (uint64_t)rows, (uint64_t)ld * 2, 64, (uint32_t)box_rows,
+                         bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
+static unsigned grid_for(int64_t items, int64_t per_block) { return (unsigned)std::max<int64_t>(1, std::min<int64_t>(ceil_div(items, per_block), 8LL * sm_count())); }
+
+static int check_shapes(const void* x, int64_t ldx, const void* w, int64_t ldw, int dtype, int64_t T, int64_t V, int64_t d, int reduction) {
+    CINN_CHECK_ARG(dtype == CINN_BF16 || dtype == CINN_F16, "linear_ce: operands are bf16 or fp16 (dtype tag %d)", dtype);
+    CINN_CHECK_ARG(T >= 0 && V >= 1 && d >= 1, "linear_ce: bad shape");
+    CINN_CHECK_ARG(T <= (1LL << 30) && V <= (1LL << 30) && d <= (1LL << 24) && (T / 256 + 1) * (V / 256 + 1) < (1LL << 31),
+                   "linear_ce: dimension too large");
+    CINN_CHECK_ARG(reduction >= 0 && reduction <= 2, "linear_ce: reduction %d (0 none, 1 mean, 2 sum)", reduction);
+    CINN_CHECK_ARG(d % 8 == 0 && ldx % 8 == 0 && ldw % 8 == 0 && ldx >= d && ldw >= d,
+                   "linear_ce: the row length (%lld) and pitches (%lld, %lld) must be multiples of 8 elements", (long long)d, (long long)ldx, (long long)ldw);
+    CINN_CHECK_ARG(T == 0 || (x && w), "linear_ce: null pointer");
+    CINN_CHECK_ARG(((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(w)) & 15) == 0, "linear_ce: operands must be 16-byte aligned");
+    return CINN_OK;
+}
+
+static int gather(const void* x, int64_t ldx, const Plan& r, const State& s, void* xg, cudaStream_t st) {
+    launch_dependent(gather_kernel, dim3(grid_for(r.T * (r.d / 8), 256)), dim3(256), 0, st, static_cast<const uint4*>(x), ldx / 8, (int)r.T,
+                     (int)(r.d / 8), s.n_valid, s.rows, static_cast<uint4*>(xg));
+    CINN_CHECK_LAUNCH();
+    return CINN_OK;
+}
+
+template <bool BF16>
+static int forward(const void* x, int64_t ldx, const void* w, int64_t ldw, const int64_t* target, int64_t ignore, const Plan& r, int reduction,
+                   float* loss, const State& s, const Forward& f, cudaStream_t st) {
+    const int blocks = (int)ceil_div(r.T, SCAN);
+    if (blocks > 1) {
+        launch_dependent(count_kernel, dim3(blocks), dim3(SCAN), 0, st, target, (int)r.T, ignore, (int)r.V, f.counts);
+        CINN_CHECK_LAUNCH();
+    }
+    launch_dependent(place_kernel, dim3(blocks), dim3(SCAN), 0, st, target, (int)r.T, ignore, (int)r.V, blocks > 1 ? f.counts : nullptr, s);
+    CINN_CHECK_LAUNCH();
+    int rc = gather(x, ldx, r, s, f.xg, st);
+    if (rc) return rc;
+    CUtensorMap ta, tb, tx;
+    if ((rc = map16(&ta, x, r.d, r.T, ldx, 128, BF16))) return rc;
+    if ((rc = map16(&tx, f.xg, r.d, up(r.T, KE), r.d, 128, BF16))) return rc;
+    if ((rc = map16(&tb, w, r.d, r.V, ldw, 128, BF16))) return rc;
+    Params p{};
+    p.n_valid = s.n_valid; p.T = (int)r.T; p.V = (int)r.V; p.d = (int)r.d; p.parts = r.parts;
+    p.part = f.part; p.part_ld = r.Tp; p.target_logit = f.target_logit; p.target = s.target;
+    if ((rc = launch<STATS, BF16>(ta, tb, tx, ta, p, st))) return rc;
+    launch_dependent(loss_kernel, dim3((unsigned)ceil_div(r.T, 128)), dim3(128), 0, st, f.part, r.Tp, 2 * r.parts, f.target_logit, s, (int)r.T,
+                     reduction, f.block_sum, loss);
+    CINN_CHECK_LAUNCH();
+    return CINN_OK;
+}
+
+template <bool BF16>
+static int backward(const void* x, int64_t ldx, const void* w, int64_t ldw, const float* grad, const Plan& r, int reduction, const State& s,
+                    void* dx, void* dw, const Backward& b, cudaStream_t st) {
+    int rc = gather(x, ldx, r, s, b.xg, st);
+    if (rc) return rc;
+    Params p{};
+    p.n_valid = s.n_valid; p.T = (int)r.T; p.V = (int)r.V; p.d = (int)r.d;
+    p.target = s.target; p.rows = s.rows; p.stat = s.stat; p.grad = grad; p.grad_max = b.grad_max;
+    p.per_row = reduction == 0; p.mean = reduction == 1;
+    if (p.per_row) {
+        CINN_CHECK_CUDA(cudaMemsetAsync(b.grad_max, 0, 4, st));
+        launch_dependent(grad_max_kernel, dim3(grid_for(r.T, 1024)), dim3(256), 0, st, grad, s.slot, (int)r.T, b.grad_max);
+        CINN_CHECK_LAUNCH();
+    }
+    CUtensorMap x_rows, xg_rows, x_cols, xg_cols, w_rows, w_cols, c_dw, c_dx;
+    if ((rc = map16(&x_rows, x, r.d, r.T, ldx, 128, BF16))) return rc;
+    if ((rc = map16(&xg_rows, b.xg, r.d, up(r.T, KE), r.d, 128, BF16))) return rc;
+    if ((rc = map16(&x_cols, x, r.d, r.T, ldx, 64, BF16))) return rc;
+    if ((rc = map16(&xg_cols, b.xg, r.d, up(r.T, KE), r.d, 64, BF16))) return rc;
+    if ((rc = map16(&w_rows, w, r.d, r.V, ldw, 128, BF16))) return rc;
+    if ((rc = map16(&w_cols, w, r.d, r.V, ldw, 64, BF16))) return rc;
+    auto sums = [&](CUtensorMap* m, float* base, int64_t rows) {
+        return encode_map_2d(m, base, (uint64_t)r.d, (uint64_t)rows, (uint64_t)r.d * 4, 32, 32, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, CU_TENSOR_MAP_SWIZZLE_128B);
+    };
+    if (dx && (rc = sums(&c_dx, b.dx, r.dx_splits * r.Tp))) return rc;
+    if (dw) {
+        if (r.dw_splits > 1) rc = sums(&c_dw, b.dw, r.dw_splits * up(r.V, M));
+        else rc = map16(&c_dw, dw, r.d, r.V, r.d, 32, BF16);
+        if (rc) return rc;
+    }
+    for (int i = 0; i < r.pieces; ++i) {
+        p.v0 = (int)(i * r.vc);
+        p.vc = (int)std::min<int64_t>(r.vc, r.V - p.v0);
+        CUtensorMap z_store, z_rows, z_cols;
+        if ((rc = map16(&z_store, b.dz, p.vc, r.Tp, r.dz_ld, 32, BF16))) return rc;
+        if ((rc = map16(&z_rows, b.dz, p.vc, r.Tp, r.dz_ld, 128, BF16))) return rc;
+        if ((rc = map16(&z_cols, b.dz, p.vc, r.Tp, r.dz_ld, 64, BF16))) return rc;
+        if ((rc = launch<SOFT, BF16>(x_rows, w_rows, xg_rows, z_store, p, st))) return rc;
+        if (dx) {
+            p.add = i > 0; p.splits = r.dx_splits; p.rows_pad = (int)r.Tp;
+            if ((rc = launch<DX, BF16>(z_rows, w_cols, xg_rows, c_dx, p, st))) return rc;
+        }
+        if (dw) {
+            p.add = 0; p.splits = r.dw_splits; p.rows_pad = (int)up(r.V, M);
+            rc = r.dw_splits > 1 ? launch<DW_PART, BF16>(z_cols, x_cols, xg_cols, c_dw, p, st)
+                                 : launch<DW, BF16>(z_cols, x_cols, xg_cols, c_dw, p, st);
+            if (rc) return rc;
+        }
+    }
+    if (dx) {
+        launch_dependent(finish_kernel<BF16>, dim3(grid_for(r.T * (r.d / 4), 256)), dim3(256), 0, st, b.dx, r.dx_splits, r.Tp * r.d, (int)r.T, (int)r.d,
+                         s.slot, p, static_cast<uint2*>(dx));
+        CINN_CHECK_LAUNCH();
+    }
+    if (dw && r.dw_splits > 1) {
+        launch_dependent(finish_kernel<BF16>, dim3(grid_for(r.V * (r.d / 4), 256)), dim3(256), 0, st, b.dw, r.dw_splits, up(r.V, M) * r.d, (int)r.V,
+                         (int)r.d, nullptr, p, static_cast<uint2*>(dw));
+        CINN_CHECK_LAUNCH();
+    }
+    return CINN_OK;
+}
+
+}  // namespace ce
+
+int64_t linear_ce_state_bytes(int64_t T) {
+    int64_t n = 0;
+    if (T > 0) ce::carve_state(nullptr, T, &n);
+    return n;
+}
+int64_t linear_ce_workspace_bytes(int64_t T, int64_t V, int64_t d, int pass) {
+    if (T <= 0 || V <= 0 || d <= 0) return 0;
+    int64_t n = 0;
+    const ce::Plan r = ce::make_plan(T, V, d);
+    if (pass == 0) ce::carve_forward(nullptr, r, &n);
+    else ce::carve_backward(nullptr, r, pass & 1, pass & 2, &n);
+    return n;
+}
+
+int linear_ce_forward(const void* x, int64_t ldx, const void* w, int64_t ldw, int dtype, const int64_t* target, int64_t ignore, int64_t T, int64_t V,
+                      int64_t d, int reduction, float* loss, void* state, void* workspace, int64_t workspace_bytes, cudaStream_t st) {
+    int rc = ce::check_shapes(x, ldx, w, ldw, dtype, T, V, d, reduction);
+    if (rc) return rc;
+    CINN_CHECK_ARG(loss || (T == 0 && reduction == 0), "linear_ce: null pointer");
+    if (T == 0) {
+        // a mean of nothing is NaN (all bits set), a sum 0
+        if (reduction) CINN_CHECK_CUDA(cudaMemsetAsync(loss, reduction == 1 ? 0xff : 0, 4, st));
+        return CINN_OK;
+    }
+    CINN_CHECK_ARG(target && state && workspace, "linear_ce: null pointer");
+    const ce::Plan r = ce::make_plan(T, V, d);
+    int64_t need = 0;
+    const ce::Forward f = ce::carve_forward(workspace, r, &need);
+    CINN_CHECK_ARG(workspace_bytes >= need, "linear_ce: workspace of %lld bytes, %lld are needed", (long long)workspace_bytes, (long long)need);
+    const ce::State s = ce::carve_state(state, T, nullptr);
+    return dtype == CINN_BF16 ? ce::forward<true>(x, ldx, w, ldw, target, ignore, r, reduction, loss, s, f, st)
+                              : ce::forward<false>(x, ldx, w, ldw, target, ignore, r, reduction, loss, s, f, st);
+}
+
+int linear_ce_backward(const void* x, int64_t ldx, const void* w, int64_t ldw, int dtype, const float* grad, int64_t T, int64_t V, int64_t d,
+                       int reduction, const void* state, void* dx, void* dw, void* workspace, int64_t workspace_bytes, cudaStream_t st) {
+    int rc = ce::check_shapes(x, ldx, w, ldw, dtype, T, V, d, reduction);
+    if (rc) return rc;
+    if (!dx && !dw) return CINN_OK;
+    if (T == 0) {
+        if (dw) CINN_CHECK_CUDA(cudaMemsetAsync(dw, 0, (size_t)(V * d * 2), st));
+        return CINN_OK;
+    }
+    CINN_CHECK_ARG(grad && state && workspace, "linear_ce: null pointer");
+    CINN_CHECK_ARG(((reinterpret_cast<uintptr_t>(dx) | reinterpret_cast<uintptr_t>(dw)) & 15) == 0, "linear_ce: gradients must be 16-byte aligned");
+    const ce::Plan r = ce::make_plan(T, V, d);
+    int64_t need = 0;
+    const ce::Backward b = ce::carve_backward(workspace, r, dx != nullptr, dw != nullptr, &need);
+    CINN_CHECK_ARG(workspace_bytes >= need, "linear_ce: workspace of %lld bytes, %lld are needed", (long long)workspace_bytes, (long long)need);
+    const ce::State s = ce::carve_state(const_cast<void*>(state), T, nullptr);
+    return dtype == CINN_BF16 ? ce::backward<true>(x, ldx, w, ldw, grad, r, reduction, s, dx, dw, b, st)
+                              : ce::backward<false>(x, ldx, w, ldw, grad, r, reduction, s, dx, dw, b, st);
+}
+
+int read_loss_status(int* out, int reset) {
+    int v = 0;
+    CINN_CHECK_CUDA(cudaMemcpyFromSymbol(&v, ce::g_status, sizeof(int)));
+    if (reset && v) {
+        const int z = 0;
+        CINN_CHECK_CUDA(cudaMemcpyToSymbol(ce::g_status, &z, sizeof(int)));
+    }
+    *out = v;
+    return CINN_OK;
+}
+
+}  // namespace cinn

@@ -839,6 +839,26 @@ def lightning_indexer_fused(q: torch.Tensor, k: torch.Tensor, w: torch.Tensor) -
     return _host.indexer(q, k, w)                         # one native call (csrc/host/attention.cpp)
 
 
+_REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}
+
+
+def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, target: torch.Tensor, ignore_index: int = -100,
+                         reduction: str = "mean") -> torch.Tensor:
+    """``F.cross_entropy(F.linear(x, weight).float(), target, ...)`` of an output projection (the reference's ``lm_head`` and
+    loss, src/train.py:345-356) without the logits in memory: forward and both gradients are made from ``x`` and ``weight``
+    tile by tile, so that beside inputs and gradients a call holds a piece of the vocabulary at a time (512 MiB at most, or 256
+    words for more than a million tokens).
+
+    ``x`` (..., d) and ``weight`` (vocabulary, d): both bfloat16 or both float16; under autocast they are cast to its type as for
+    ``F.linear``.  ``target`` (...): int64 or int32.  A target equal to ``ignore_index`` takes its token out: loss 0, a
+    gradient of zeros, no share in the mean or in ``weight``'s gradient, whatever its row of ``x`` holds (NaN too).  Any other
+    target outside the vocabulary makes its loss NaN and adds nothing to the gradients.  ``reduction``: "mean" over the targets
+    that count (NaN where there are none), "sum", or "none": the tokens' losses, of ``target``'s shape.  The loss is fp32; products
+    are summed in fp32, and the logits' gradient is rounded to the operands' type before the two products that follow."""
+    assert reduction in _REDUCTIONS, "reduction must be 'none', 'mean' or 'sum'"
+    return _host.linear_cross_entropy(x, weight, target, int(ignore_index), _REDUCTIONS[reduction])
+
+
 def gather_quantized_rows(x_fp8: torch.Tensor, x_scale: torch.Tensor, idx: torch.Tensor):
     """``(x_fp8[idx], x_scale[idx])`` in one pass: the dispatch gather of ``MoE.forward``
     (reference src/layers.py:140) on tokens quantised once before the gather."""

@@ -540,6 +540,26 @@ int cinn_moe_route_static(const float* logits, const float* bias, int64_t n_toke
                           int* top_experts, float* top_gates, int64_t* token_indices, float* sorted_scores,
                           int64_t* sorted_experts, int64_t* counts, int64_t* pair_pos, float* pair_gate, void* stream);
 
+/* Output projection and softmax cross entropy without the logits in memory (the reference: lm_head and
+ * F.cross_entropy, src/train.py:345-356).
+ *   z = x W^T, loss_t = log sum_v e^z_tv - z_t,target(t);  dx = dz W, dW = dz^T x with
+ *   dz_tv = grad_t (softmax(z_t)_v - [v = target(t)])
+ * x: (T, d) and w: (V, d) of one 16-bit type, rows contiguous, pitches ldx and ldw; d and the pitches multiples of 8, bases
+ * 16-byte aligned.  target: int64 (T,).  A token whose target is ignore_index has loss 0 and no part in anything, whatever
+ * its row of x holds; one whose target is no word (outside [0, V)) has the loss NaN and no part in the gradients.
+ * reduction 0: loss (T,), one per token; 1: the mean over the tokens with a target (NaN where there is none), 2: the sum.
+ * grad: (T,) or one number, fp32.  dx (T, d) and dw (V, d), contiguous, of the operands' type; either may be NULL.
+ * state: cinn_linear_ce_state_bytes(T), written by the forward for the backward.  workspace: scratch of
+ * cinn_linear_ce_workspace_bytes(T, V, d, pass): pass 0 = forward, 4 = backward, + 1 with dx, + 2 with dw. */
+int64_t cinn_linear_ce_state_bytes(int64_t T);
+int64_t cinn_linear_ce_workspace_bytes(int64_t T, int64_t V, int64_t d, int pass);
+int cinn_linear_ce_forward(const void* x, int64_t ldx, const void* w, int64_t ldw, int dtype, const int64_t* target,
+                           int64_t ignore_index, int64_t T, int64_t V, int64_t d, int reduction, float* loss, void* state,
+                           void* workspace, int64_t workspace_bytes, void* stream);
+int cinn_linear_ce_backward(const void* x, int64_t ldx, const void* w, int64_t ldw, int dtype, const float* grad, int64_t T,
+                            int64_t V, int64_t d, int reduction, const void* state, void* dx, void* dw, void* workspace,
+                            int64_t workspace_bytes, void* stream);
+
 /* Caps the number of SMs the persistent GEMM kernels (cinn_fp8_gemm, cinn_fp8_grouped_gemm*) occupy from now
  * on, process-wide; 0 = all of them (the default).  Returns the previous cap.  For callers that run other
  * kernels beside a GEMM on another stream, e.g. the send/receive kernels of an all-to-all, which otherwise wait
