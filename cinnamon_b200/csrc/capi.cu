@@ -136,6 +136,9 @@ int balance_loss(const void* logits, int dtype, const int* top_experts, int64_t 
 int gates_backward(const void* logits, int dtype, const int64_t* sorted_experts, const int64_t* pair_pos, const float* d_gates,
                    const float* share, const float* d_loss, float alpha, int64_t batch, int64_t seq, int E, int top_k, void* d_logits,
                    cudaStream_t st);
+int rotary(const void* const* in, void* const* out, const int64_t* in_strides, const int64_t* out_strides, const int64_t* heads, const int64_t* d,
+           const int64_t* start, int dtype, int64_t B, int64_t L, const int64_t* positions, int64_t pos_b, int64_t pos_l, const double* freq, int64_t pairs,
+           int interleaved, int inverse, float magnitude, cudaStream_t st);
 int64_t linear_ce_state_bytes(int64_t T);
 int64_t linear_ce_workspace_bytes(int64_t T, int64_t V, int64_t d, int pass);
 int linear_ce_forward(const void* x, int64_t ldx, const void* w, int64_t ldw, int dtype, const int64_t* target, int64_t ignore, int64_t T, int64_t V,
@@ -376,6 +379,13 @@ int cinn_linear_ce_backward(const void* x, int64_t ldx, const void* w, int64_t l
                             void* stream) {
     return cinn::linear_ce_backward(x, ldx, w, ldw, dtype, grad, T, V, d, reduction, state, dx, dw, workspace, workspace_bytes,
                                     (cudaStream_t)stream);
+}
+
+int cinn_rotary(const void* const* in, void* const* out, const int64_t* in_strides, const int64_t* out_strides, const int64_t* heads,
+                const int64_t* d, const int64_t* start, int dtype, int64_t B, int64_t L, const int64_t* positions, int64_t pos_stride_b,
+                int64_t pos_stride_l, const double* inv_freq, int64_t n_pairs, int interleaved, int inverse, float magnitude, void* stream) {
+    return cinn::rotary(in, out, in_strides, out_strides, heads, d, start, dtype, B, L, positions, pos_stride_b, pos_stride_l, inv_freq, n_pairs,
+                        interleaved, inverse, magnitude, (cudaStream_t)stream);
 }
 
 int cinn_scatter_rows(const void* in, const int64_t* idx, void* out, int64_t n_rows, int64_t n_dst, int64_t row_bytes,

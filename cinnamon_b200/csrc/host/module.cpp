@@ -9,6 +9,7 @@ void bind_attention(pybind11::module_& m);
 void bind_moe(pybind11::module_& m);
 void bind_moe_train(pybind11::module_& m);
 void bind_loss(pybind11::module_& m);
+void bind_rotary(pybind11::module_& m);
 }  // namespace cinnhost
 
 PYBIND11_MODULE(_host, m) {
@@ -38,4 +39,5 @@ PYBIND11_MODULE(_host, m) {
     bind_moe(m);
     bind_moe_train(m);
     bind_loss(m);
+    bind_rotary(m);
 }

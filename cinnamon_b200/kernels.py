@@ -22,6 +22,7 @@ Differences a caller can observe, all deliberate:
 from __future__ import annotations
 
 import ctypes
+import math
 import os
 import weakref
 
@@ -845,7 +846,7 @@ _REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}
 def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, target: torch.Tensor, ignore_index: int = -100,
                          reduction: str = "mean") -> torch.Tensor:
     """``F.cross_entropy(F.linear(x, weight).float(), target, ...)`` of an output projection (the reference's ``lm_head`` and
-    loss, src/train.py:345-356) without the logits in memory: forward and both gradients are made from ``x`` and ``weight``
+    loss, src/train.py:338-376) without the logits in memory: forward and both gradients are made from ``x`` and ``weight``
     tile by tile, so that beside inputs and gradients a call holds a piece of the vocabulary at a time (512 MiB at most, or 256
     words for more than a million tokens).
 
@@ -857,6 +858,60 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, target: torch.Te
     are summed in fp32, and the logits' gradient is rounded to the operands' type before the two products that follow."""
     assert reduction in _REDUCTIONS, "reduction must be 'none', 'mean' or 'sum'"
     return _host.linear_cross_entropy(x, weight, target, int(ignore_index), _REDUCTIONS[reduction])
+
+
+def rotary_frequencies(dim: int, base: float = 10000.0, scaling: str = "none", factor: float = 1.0, original_len: int = None,
+                       beta_fast: float = 32.0, beta_slow: float = 1.0, mscale: float = 1.0, device=None):
+    """``(inv_freq, magnitude)`` for ``rotary``: the frequencies of ``dim / 2`` pairs in radians a position (float64), and the factor on
+    what is rotated (reference src/attention.py:35-73).  ``scaling`` for contexts ``factor`` times as long as those of training:
+
+      "none"    base ** (-2 i / dim)
+      "linear"  all frequencies over ``factor``
+      "ntk"     the base times factor ** (dim / (dim - 2)): the fastest pair keeps its frequency, the slowest is divided by ``factor``
+      "yarn"    pairs that turn more than ``beta_fast`` times within ``original_len`` positions keep theirs, those that turn less than
+                ``beta_slow`` times are divided by ``factor``, a ramp in between; magnitude 0.1 mscale ln(factor) + 1"""
+    assert dim >= 2 and dim % 2 == 0, "dim must be even"
+    assert scaling in ("none", "linear", "ntk", "yarn"), "scaling must be 'none', 'linear', 'ntk' or 'yarn'"
+    assert base > 1 and factor >= 1, "base must be over 1 and factor at least 1"
+    magnitude = 1.0
+    if scaling == "ntk" and dim > 2:
+        base = base * factor ** (dim / (dim - 2))
+    i = torch.arange(dim // 2, dtype=torch.float64)
+    freq = base ** (-2.0 * i / dim)
+    if scaling == "linear":
+        freq = freq / factor
+    elif scaling == "yarn":
+        assert original_len is not None and original_len > 0, "scaling='yarn' needs original_len"
+
+        def pair_of(turns):                         # the pair (not whole) that turns so often within original_len positions
+            return dim * math.log(original_len / (2 * math.pi * turns)) / (2 * math.log(base))
+        low, high = max(math.floor(pair_of(beta_fast)), 0), min(math.ceil(pair_of(beta_slow)), dim - 1)
+        ramp = ((i - low) / max(high - low, 1e-3)).clamp(0, 1)
+        freq = freq / factor * ramp + freq * (1 - ramp)
+        magnitude = 0.1 * mscale * math.log(factor) + 1.0
+    return freq.to(device) if device is not None else freq, magnitude
+
+
+def rotary(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor, interleaved: bool = False, start: int = 0,
+           magnitude: float = 1.0):
+    """Rotary positions of queries and keys as ``sparse_attention`` takes them (reference src/attention.py:35-73): ``(q', k')``, of the inputs'
+    type and layout, differentiable in both.
+
+    ``q`` (batch, heads, L, d) and ``k`` (batch, any number of heads, L, any d), or None; any strides, so that a transposed view of (batch,
+    L, heads, d) is read in place.  The ``2 * inv_freq.numel()`` elements from ``start`` on (negative: from a head's end, for
+    each of the two) are rotated, the others copied: pair i is (a, b) = elements (2 i, 2 i + 1) if ``interleaved``, else (i, i +
+    inv_freq.numel()), and becomes ``magnitude`` (a cos t - b sin t, b cos t + a sin t) with t = position ``* inv_freq[i]``.
+    ``positions`` (L,) or (batch, L), int64 or int32, any values; ``inv_freq`` as from ``rotary_frequencies``.  The angles of far positions
+    are exact; products are fp32, rounded once."""
+    return _host.rotary(q, k, positions, inv_freq, bool(interleaved), int(start), float(magnitude), False)
+
+
+def rotary_(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor, interleaved: bool = False, start: int = 0,
+            magnitude: float = 1.0):
+    """``rotary`` in place, without gradients: reads and writes the rotated elements only, and returns ``(q, k)``.  The two must not
+    overlap, in themselves or with each other."""
+    _host.rotary_(q, k, positions, inv_freq, bool(interleaved), int(start), float(magnitude))
+    return q, k
 
 
 def gather_quantized_rows(x_fp8: torch.Tensor, x_scale: torch.Tensor, idx: torch.Tensor):

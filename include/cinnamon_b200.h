@@ -541,7 +541,7 @@ int cinn_moe_route_static(const float* logits, const float* bias, int64_t n_toke
                           int64_t* sorted_experts, int64_t* counts, int64_t* pair_pos, float* pair_gate, void* stream);
 
 /* Output projection and softmax cross entropy without the logits in memory (the reference: lm_head and
- * F.cross_entropy, src/train.py:345-356).
+ * F.cross_entropy, src/train.py:338-376).
  *   z = x W^T, loss_t = log sum_v e^z_tv - z_t,target(t);  dx = dz W, dW = dz^T x with
  *   dz_tv = grad_t (softmax(z_t)_v - [v = target(t)])
  * x: (T, d) and w: (V, d) of one 16-bit type, rows contiguous, pitches ldx and ldw; d and the pitches multiples of 8, bases
@@ -559,6 +559,18 @@ int cinn_linear_ce_forward(const void* x, int64_t ldx, const void* w, int64_t ld
 int cinn_linear_ce_backward(const void* x, int64_t ldx, const void* w, int64_t ldw, int dtype, const float* grad, int64_t T,
                             int64_t V, int64_t d, int reduction, const void* state, void* dx, void* dw, void* workspace,
                             int64_t workspace_bytes, void* stream);
+
+/* Rotary positions of queries and keys (the reference: RoPE, src/attention.py:35-73), one launch for both.
+ *   pair i of a head: (a, b) -> magnitude (a cos t - b sin t, b cos t + a sin t), t = position * inv_freq[i]; inverse: -t
+ * Index 0 of the HOST arrays is q, index 1 k (in[1] NULL: q alone).  Each is (B, heads, L, d) with the elements of a head
+ * contiguous; in_strides and out_strides: HOST, {batch, head, position} of q, then of k, in elements.  The 2 * n_pairs elements from
+ * start[] on are rotated: neighbours are a pair (interleaved != 0), or elements n_pairs apart.  The others are copied; where out
+ * is in for q and k alike, they are left alone.  positions: int64 with strides (0 for what does not vary); inv_freq:
+ * fp64, radians a position.  The angle is exact for any position up to the rounding of inv_freq. */
+int cinn_rotary(const void* const* in, void* const* out, const int64_t* in_strides, const int64_t* out_strides, const int64_t* heads,
+                const int64_t* d, const int64_t* start, int dtype, int64_t B, int64_t L, const int64_t* positions, int64_t pos_stride_b,
+                int64_t pos_stride_l, const double* inv_freq, int64_t n_pairs, int interleaved, int inverse, float magnitude,
+                void* stream);
 
 /* Caps the number of SMs the persistent GEMM kernels (cinn_fp8_gemm, cinn_fp8_grouped_gemm*) occupy from now
  * on, process-wide; 0 = all of them (the default).  Returns the previous cap.  For callers that run other
