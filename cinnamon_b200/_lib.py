@@ -104,6 +104,8 @@ SIGNATURES = {
     "cinn_linear_ce_forward": [_vp, _i64, _vp, _i64, _i32, _vp, _i64, _i64, _i64, _i64, _i32, _vp, _vp, _vp, _i64, _vp],
     "cinn_linear_ce_backward": [_vp, _i64, _vp, _i64, _i32, _vp, _i64, _i64, _i64, _i32, _vp, _vp, _vp, _vp, _i64, _vp],
     "cinn_rotary": [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i32, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i32, _i32, ctypes.c_float, _vp],
+    "cinn_moe_route_form": [_vp, _i32, _vp, _i64, _i32, _i32, _i32, _i32, _i32, _i32, ctypes.c_float] + [_vp] * 12,
+    "cinn_moe_route_form_backward": [_vp, _i32] + [_vp] * 6 + [_i64, _i32, _i32, _i32, _i32, ctypes.c_float, _vp, _vp],
     "cinn_launch_count": [],
     "cinn_device_status": [ctypes.POINTER(ctypes.c_int), _i32],
     "cinn_fp8_grouped_gemm": [_vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _vp, _i32, _vp],

@@ -139,6 +139,12 @@ int gates_backward(const void* logits, int dtype, const int64_t* sorted_experts,
 int rotary(const void* const* in, void* const* out, const int64_t* in_strides, const int64_t* out_strides, const int64_t* heads, const int64_t* d,
            const int64_t* start, int dtype, int64_t B, int64_t L, const int64_t* positions, int64_t pos_b, int64_t pos_l, const double* freq, int64_t pairs,
            int interleaved, int inverse, float magnitude, cudaStream_t st);
+int moe_route_form(const void* logits, int logits_dtype, const float* bias, int64_t T, int E, int top_k, int scores, int n_groups, int top_groups,
+                   int renormalise, float scale, int* workspace, int* top_experts, float* top_gates, int64_t* token_indices, float* sorted_scores,
+                   int64_t* sorted_experts, int64_t* counts, int64_t* starts, int64_t* ends, int64_t* pair_pos, float* pair_gate, cudaStream_t st);
+int moe_route_form_backward(const void* logits, int logits_dtype, const int* top_experts, const int64_t* sorted_experts, const int64_t* pair_pos,
+                            const float* d_top, const float* d_pair, const float* d_sorted, int64_t T, int E, int top_k, int scores, int renormalise, float scale,
+                            void* d_logits, cudaStream_t st);
 int64_t linear_ce_state_bytes(int64_t T);
 int64_t linear_ce_workspace_bytes(int64_t T, int64_t V, int64_t d, int pass);
 int linear_ce_forward(const void* x, int64_t ldx, const void* w, int64_t ldw, int dtype, const int64_t* target, int64_t ignore, int64_t T, int64_t V,
@@ -386,6 +392,21 @@ int cinn_rotary(const void* const* in, void* const* out, const int64_t* in_strid
                 int64_t pos_stride_l, const double* inv_freq, int64_t n_pairs, int interleaved, int inverse, float magnitude, void* stream) {
     return cinn::rotary(in, out, in_strides, out_strides, heads, d, start, dtype, B, L, positions, pos_stride_b, pos_stride_l, inv_freq, n_pairs,
                         interleaved, inverse, magnitude, (cudaStream_t)stream);
+}
+
+int cinn_moe_route_form(const void* logits, int logits_dtype, const float* bias, int64_t n_tokens, int n_experts, int top_k, int scores,
+                        int n_groups, int top_groups, int renormalise, float scale, int* workspace, int* top_experts, float* top_gates,
+                        int64_t* token_indices, float* sorted_scores, int64_t* sorted_experts, int64_t* counts, int64_t* starts, int64_t* ends,
+                        int64_t* pair_pos, float* pair_gate, void* stream) {
+    return cinn::moe_route_form(logits, logits_dtype, bias, n_tokens, n_experts, top_k, scores, n_groups, top_groups, renormalise, scale, workspace,
+                                top_experts, top_gates, token_indices, sorted_scores, sorted_experts, counts, starts, ends, pair_pos, pair_gate,
+                                (cudaStream_t)stream);
+}
+int cinn_moe_route_form_backward(const void* logits, int logits_dtype, const int* top_experts, const int64_t* sorted_experts, const int64_t* pair_pos,
+                                 const float* d_top_gates, const float* d_pair_gate, const float* d_sorted_scores, int64_t n_tokens, int n_experts,
+                                 int top_k, int scores, int renormalise, float scale, void* d_logits, void* stream) {
+    return cinn::moe_route_form_backward(logits, logits_dtype, top_experts, sorted_experts, pair_pos, d_top_gates, d_pair_gate, d_sorted_scores, n_tokens, n_experts,
+                                         top_k, scores, renormalise, scale, d_logits, (cudaStream_t)stream);
 }
 
 int cinn_scatter_rows(const void* in, const int64_t* idx, void* out, int64_t n_rows, int64_t n_dst, int64_t row_bytes,

@@ -24,7 +24,7 @@ using at::Tensor;
     X(cinn_last_error) X(cinn_quant_rowwise) X(cinn_quant_rowwise_dual) X(cinn_quant_rowwise_with_block)             \
     X(cinn_quant_rowwise_with_block_t) X(cinn_quant_rowwise_dual_padded) X(cinn_quant_rowwise_with_block_t_padded) X(cinn_quant_blockwise) X(cinn_quant_block_beside) X(cinn_quant_linear) X(cinn_transpose_bytes)     \
     X(cinn_requant_row_to_block) X(cinn_fp8_gemm_ws) X(cinn_fp8_gemm_pitched) X(cinn_fp8_gemm_workspace_bytes) \
-    X(cinn_lightning_indexer) X(cinn_linear_ce_state_bytes) X(cinn_linear_ce_workspace_bytes) X(cinn_linear_ce_forward) X(cinn_linear_ce_backward) X(cinn_rotary) \
+    X(cinn_lightning_indexer) X(cinn_linear_ce_state_bytes) X(cinn_linear_ce_workspace_bytes) X(cinn_linear_ce_forward) X(cinn_linear_ce_backward) X(cinn_rotary) X(cinn_moe_route_form) X(cinn_moe_route_form_backward) \
     X(cinn_sparse_attn_workspace_bytes) X(cinn_sparse_attn_fwd_ws) X(cinn_sparse_attn_bwd) X(cinn_sparse_attn_bwd_ws)                  \
     X(cinn_fp8_linear_few_takes) X(cinn_fp8_linear_few)                                                                   \
     X(cinn_moe_route_workspace_ints) X(cinn_moe_route_ranges) X(cinn_spread_rows) X(cinn_fp8_grouped_gemm)                \
@@ -138,6 +138,17 @@ std::tuple<std::vector<Tensor>, Tensor> linear_backward_quantised(const Quantise
 Quantised rowwise(const Tensor& x, bool round_scale, int div);                 // moe.cpp
 Quantised swiglu_quantised(const Tensor& h12, int div);
 Tensor grouped(const Quantised& x, const Quantised& w, const Tensor& starts, const Tensor& ends, at::ScalarType type = at::kBFloat16);
+struct RouteForm {                              // the router's scores and gates; `reference`: the form and arithmetic of cinn_moe_route
+    int64_t scores = 0, n_groups = 1, top_groups = 1;
+    bool renormalise = true;
+    double scale = 1.0;
+    bool reference = true;
+};
+// the same from Python: (scores, n_groups, top_groups, renormalise, scale, reference)
+using RouteOptions = std::tuple<int64_t, int64_t, int64_t, bool, double, bool>;
+inline RouteForm route_form(const RouteOptions& o) {
+    return {std::get<0>(o), std::get<1>(o), std::get<2>(o), std::get<3>(o), std::get<4>(o), std::get<5>(o)};
+}
 struct Routes {                                 // moe_route's outputs, in three tensors
     Tensor longs, floats, top;                  // token_indices | sorted_experts | pair_pos | counts | starts | ends; scores | pair_gate
     int64_t pairs = 0, E = 0;
@@ -150,7 +161,7 @@ struct Routes {                                 // moe_route's outputs, in three
     Tensor ends() const { return longs.narrow(0, 3 * pairs + 2 * E, E); }
     float* gates() const { return static_cast<float*>(floats.data_ptr()) + pairs; }
 };
-Routes route(const Tensor& logits, const Tensor& bias, int64_t top_k);
+Routes route(const Tensor& logits, const Tensor& bias, int64_t top_k, const RouteForm& form = RouteForm(), Tensor* top_gates = nullptr);
 // refuses operands on other devices or of other widths, before anything is launched
 void check_layer(const Tensor& x, const Tensor& router, const Tensor& bias, const Quantised& w12, const Quantised& w3);
 Quantised spread(const Quantised& x, const Routes& r, int64_t top_k);

@@ -40,8 +40,8 @@ void check_layer(const Tensor& x, const Tensor& router, const Tensor& bias, cons
                 w3.q.size(1) == d && w12.q.size(1) == 2 * w3.q.size(2), "MoE: the widths of input, router and experts do not fit together");
 }
 
-Routes route(const Tensor& logits_in, const Tensor& bias, int64_t top_k) {
-    const Tensor logits = readable(logits_in).contiguous(), b = bias.to(at::kFloat).contiguous();
+Routes route(const Tensor& logits_in, const Tensor& bias, int64_t top_k, const RouteForm& form, Tensor* gates_by_slot) {
+    const Tensor logits = readable(logits_in).contiguous(), b = bias.defined() ? bias.to(at::kFloat).contiguous() : bias;
     const int64_t T = logits.size(0), E = logits.size(1);
     const at::Device dev = logits.device();
     Routes r;
@@ -52,10 +52,18 @@ Routes route(const Tensor& logits_in, const Tensor& bias, int64_t top_k) {
     r.top = empty({r.pairs}, at::kInt, dev);
     Tensor ws = empty({std::max<int64_t>(1, api.cinn_moe_route_workspace_ints(T, (int)E))}, at::kInt, dev);
     Tensor top_gates = empty({r.pairs}, at::kFloat, dev);
-    check(api.cinn_moe_route_ranges(logits.data_ptr(), tag_of(logits.scalar_type()), f32(b), T, (int)E, (int)top_k, ws.data_ptr<int>(),
-                                    r.top.data_ptr<int>(), f32(top_gates), r.token_indices(), f32(r.floats), r.sorted_experts(),
-                                    r.part(3 * r.pairs), r.part(3 * r.pairs + E), r.part(3 * r.pairs + 2 * E), r.pos(), r.gates(),
-                                    stream()), "cinn_moe_route");
+    if (gates_by_slot) *gates_by_slot = top_gates;
+    if (form.reference)
+        check(api.cinn_moe_route_ranges(logits.data_ptr(), tag_of(logits.scalar_type()), f32(b), T, (int)E, (int)top_k, ws.data_ptr<int>(),
+                                        r.top.data_ptr<int>(), f32(top_gates), r.token_indices(), f32(r.floats), r.sorted_experts(),
+                                        r.part(3 * r.pairs), r.part(3 * r.pairs + E), r.part(3 * r.pairs + 2 * E), r.pos(), r.gates(),
+                                        stream()), "cinn_moe_route");
+    else
+        check(api.cinn_moe_route_form(logits.data_ptr(), tag_of(logits.scalar_type()), b.defined() ? f32(b) : nullptr, T, (int)E, (int)top_k,
+                                      (int)form.scores, (int)form.n_groups, (int)form.top_groups, form.renormalise, (float)form.scale, ws.data_ptr<int>(),
+                                      r.top.data_ptr<int>(), f32(top_gates), r.token_indices(), f32(r.floats), r.sorted_experts(),
+                                      r.part(3 * r.pairs), r.part(3 * r.pairs + E), r.part(3 * r.pairs + 2 * E), r.pos(), r.gates(),
+                                      stream()), "cinn_moe_route");
     return r;
 }
 
@@ -83,7 +91,7 @@ Tensor gemm_whole(const Tensor& a, const Tensor& sa, const Tensor& b, const Tens
 // x (T, d), contiguous; router (E, d) in the type the logits are computed in; the weights as FP8Experts and FP8SwiGLU hold
 // them.  Returns (T, d) fp32.
 Tensor forward(const Tensor& x, const Tensor& router, const Tensor& bias, int64_t top_k, const Quantised& w12, const Quantised& w3,
-               const Quantised& sw12, const Quantised& sw3, bool shared_round, int div) {
+               const Quantised& sw12, const Quantised& sw3, bool shared_round, int div, const RouteForm& form) {
     check_layer(x, router, bias, w12, w3);
     require(!sw12.q.defined() || (sw12.q.device() == x.device() && sw12.q.size(1) == x.size(1) && sw3.q.size(0) == x.size(1) &&
                                   sw12.q.size(0) == 2 * sw3.q.size(1)), "MoE: the shared expert does not fit the input");
@@ -100,7 +108,7 @@ Tensor forward(const Tensor& x, const Tensor& router, const Tensor& bias, int64_
         shared = gemm_whole(h.q, h.s, sw3.q, sw3.s, T, d, I2 / 2);
     }
     Tensor logits = at::mm(x, router.to(x.scalar_type()).t());
-    const Routes r = route(logits, bias, top_k);
+    const Routes r = route(logits, bias, top_k, form);
     const Tensor starts = r.starts(), ends = r.ends();
     const int64_t pairs = r.pairs, *pos = r.pos();
     Quantised rows = spread(xq, r, top_k);
@@ -121,14 +129,99 @@ Tensor forward(const Tensor& x, const Tensor& router, const Tensor& bias, int64_
 
 }  // namespace
 
+namespace {
+
+struct RouteCall {
+    Tensor bias;
+    int64_t top_k;
+    RouteForm form;
+    Routes out;
+};
+
+// gates by slot, in the order of pair_pos and by sorted pair, from the logits
+struct RouteNode : public torch::autograd::Function<RouteNode> {
+    static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const Tensor& logits_in, RouteCall* c) {
+        c10::cuda::CUDAGuard guard(logits_in.device());
+        at::AutoDispatchBelowAutograd below;
+        const Tensor logits = readable(logits_in).contiguous();
+        Tensor top;
+        c->out = route(logits, c->bias, c->top_k, c->form, &top);
+        const Routes& r = c->out;
+        ctx->save_for_backward({logits, r.top, r.longs});
+        ctx->saved_data["n"] = std::vector<int64_t>{c->top_k, c->form.scores, c->form.renormalise, (int64_t)logits_in.scalar_type()};
+        ctx->saved_data["scale"] = c->form.scale;
+        ctx->set_materialize_grads(false);
+        const int64_t T = logits.size(0);
+        return {top.view({T, c->top_k}), r.floats.narrow(0, r.pairs, r.pairs).view({T, c->top_k}), r.floats.narrow(0, 0, r.pairs)};
+    }
+    static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
+        const auto s = ctx->get_saved_variables();
+        const auto n = ctx->saved_data["n"].toIntVector();
+        Tensor d;
+        as_python_error([&] {
+            require(!at::GradMode::is_enabled(), "moe_route has no second derivative (create_graph=True)");
+            const Tensor& logits = s[0];
+            c10::cuda::CUDAGuard guard(logits.device());
+            const int64_t T = logits.size(0), E = logits.size(1);
+            Routes r;
+            r.longs = s[2]; r.pairs = T * n[0]; r.E = E;
+            Tensor g[3];
+            for (int i = 0; i < 3; ++i)
+                if (grads[i].defined()) g[i] = grads[i].to(at::kFloat).contiguous();
+            auto at = [&](int i) { return g[i].defined() ? f32(g[i]) : nullptr; };
+            d = empty({T, E}, logits.scalar_type(), logits.device());
+            check(api.cinn_moe_route_form_backward(logits.data_ptr(), tag_of(logits.scalar_type()), s[1].data_ptr<int>(), r.sorted_experts(), r.pos(), at(0), at(1),
+                                                   at(2), T, (int)E, (int)n[0], (int)n[1], (int)n[2], (float)ctx->saved_data["scale"].toDouble(), d.data_ptr(),
+                                                   stream()), "cinn_moe_route backward");
+            d = d.to((at::ScalarType)n[3]);
+        });
+        return {d, Tensor()};
+    }
+};
+
+}  // namespace
+
 void bind_moe(pybind11::module_& m) {
     using OptT = c10::optional<Tensor>;
+    m.def("moe_route", [](const Tensor& logits, const OptT& bias, int64_t top_k, const RouteOptions& form) {
+        require(logits.is_cuda() && (!bias.has_value() || bias->is_cuda()), "Inputs must be on CUDA");
+        require(logits.dim() == 2, "logits must be (tokens, experts)");
+        require(!bias.has_value() || (bias->device() == logits.device() && bias->dim() == 1 && bias->size(0) == logits.size(1)),
+                "moe_route: bias is one number for every expert, on the logits' device");
+        require(top_k >= 1 && top_k <= 32, "moe_route: 1 to 32 experts of a token");
+        c10::cuda::CUDAGuard guard(logits.device());
+        RouteCall c{bias.has_value() ? bias->detach() : Tensor(), top_k, route_form(form), {}};
+        const int64_t T = logits.size(0), E = logits.size(1), pairs = T * top_k;
+        Tensor top, pair, sorted;
+        if (takes_node(logits)) {
+            const auto v = RouteNode::apply(logits, &c);
+            top = v[0]; pair = v[1]; sorted = v[2];
+        } else {
+            c.out = route(logits, c.bias, top_k, c.form, &top);
+            top = top.view({T, top_k});
+            pair = c.out.floats.narrow(0, pairs, pairs).view({T, top_k});
+            sorted = c.out.floats.narrow(0, 0, pairs);
+        }
+        const Routes& r = c.out;
+        pybind11::dict out;
+        out["top_experts"] = r.top.view({T, top_k});
+        out["top_gates"] = top;
+        out["token_indices"] = r.longs.narrow(0, 0, pairs);
+        out["sorted_scores"] = sorted;
+        out["sorted_experts"] = r.longs.narrow(0, pairs, pairs);
+        out["counts"] = r.counts();
+        out["starts"] = r.starts();
+        out["ends"] = r.ends();
+        out["pair_pos"] = r.longs.narrow(0, 2 * pairs, pairs).view({T, top_k});
+        out["pair_gate"] = pair;
+        return out;
+    });
     m.def("moe_forward", [](const Tensor& x, const Tensor& router, const Tensor& bias, int64_t top_k, const Tensor& w12_q, const Tensor& w12_s,
                             const Tensor& w3_q, const Tensor& w3_s, const OptT& sw12_q, const OptT& sw12_s, const OptT& sw3_q,
-                            const OptT& sw3_s, bool shared_round, int div) {
+                            const OptT& sw3_s, bool shared_round, int div, const RouteOptions& form) {
         auto get = [](const OptT& t) { return t.has_value() ? *t : Tensor(); };
         return forward(x, router, bias, top_k, {w12_q, w12_s}, {w3_q, w3_s}, {get(sw12_q), get(sw12_s)}, {get(sw3_q), get(sw3_s)},
-                       shared_round, div);
+                       shared_round, div, route_form(form));
     });
 }
 

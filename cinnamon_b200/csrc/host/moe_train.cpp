@@ -154,6 +154,7 @@ struct BlockOptions {
     double alpha;                              // balance loss, 0 = none
     at::ScalarType router_type;                // what the router multiplies in (autocast's type, or x's)
     int div;
+    RouteForm form;
     Tensor counts;                             // out: rows per expert
 };
 
@@ -211,7 +212,7 @@ struct BlockNode : public torch::autograd::Function<BlockNode> {
         const int64_t T = x.size(0), d = x.size(1), E = router.size(0), k = o->top_k, seq = T / o->batch;
         const Tensor xr = x.to(o->router_type), wr = router.to(o->router_type);
         const Tensor logits = at::mm(xr, wr.t());
-        const Routes r = route(logits, o->bias, k);
+        const Routes r = route(logits, o->bias, k, o->form);
         const Tensor starts = r.starts(), ends = r.ends();
         const Quantised rows = spread(rowwise(x, false, o->div), r, k);
         const Tensor h12 = grouped(rows, o->w12, starts, ends);
@@ -245,8 +246,12 @@ struct BlockNode : public torch::autograd::Function<BlockNode> {
                                             (int)k, (float)o->alpha, ws.data_ptr(), f32(share), f32(loss), stream()), "cinn_moe_balance_loss");
         }
         o->counts = r.counts();
+        if (!o->form.reference) {
+            ctx->saved_data["form"] = std::vector<int64_t>{o->form.scores, o->form.renormalise};
+            ctx->saved_data["scale"] = o->form.scale;
+        }
         ctx->save_for_backward({xr, wr, logits, r.longs, r.floats, rows.q, rows.s, h12, h.q, h.s, out, o->w12.q, o->w12.s, o->w3.q, o->w3.s,
-                                share});
+                                share, o->form.reference ? Tensor() : r.top});
         ctx->saved_data["n"] = std::vector<int64_t>{k, o->batch, o->div, (int64_t)x.scalar_type(), (int64_t)router.scalar_type(),
                                                     (int64_t)w12.scalar_type(), (int64_t)w3.scalar_type(), (int64_t)addend.scalar_type()};
         ctx->saved_data["alpha"] = o->alpha;
@@ -306,7 +311,13 @@ struct BlockNode : public torch::autograd::Function<BlockNode> {
             if ((want_x || want_r) && (loss || d_gates.defined())) {
                 Tensor d_logits = empty({T, E}, logits.scalar_type(), dev);
                 const Tensor dl = loss ? grads[1].to(at::kFloat) : Tensor();
-                check(api.cinn_moe_gates_backward(logits.data_ptr(), tag_of(logits.scalar_type()), r.sorted_experts(), r.pos(),
+                if (s[16].defined()) {                     // (such a router has no balance loss in here)
+                    const auto form = ctx->saved_data["form"].toIntVector();
+                    check(api.cinn_moe_route_form_backward(logits.data_ptr(), tag_of(logits.scalar_type()), s[16].data_ptr<int>(), r.sorted_experts(), r.pos(),
+                                                           nullptr, f32(d_gates), nullptr, T, (int)E, (int)k, (int)form[0], (int)form[1],
+                                                           (float)ctx->saved_data["scale"].toDouble(), d_logits.data_ptr(), stream()),
+                          "cinn_moe_route backward");
+                } else check(api.cinn_moe_gates_backward(logits.data_ptr(), tag_of(logits.scalar_type()), r.sorted_experts(), r.pos(),
                                                   d_gates.defined() ? f32(d_gates) : nullptr, loss ? f32(s[15]) : nullptr,
                                                   loss ? f32(dl) : nullptr, alpha, batch, seq, (int)E, (int)k, d_logits.data_ptr(), stream()),
                       "cinn_moe_gates_backward");
@@ -405,11 +416,12 @@ void bind_moe_train(pybind11::module_& m) {
     // (y, balance loss or None, rows per expert)
     m.def("moe_block", [](const Tensor& x, const Tensor& router, const Tensor& w12, const Tensor& w3, const Tensor& addend,
                           const Tensor& bias, const Tensor& w12_q, const Tensor& w12_s, const Tensor& w3_q, const Tensor& w3_s, int64_t top_k,
-                          int64_t batch, double alpha, bool cast_router, int div) {
+                          int64_t batch, double alpha, bool cast_router, int div, const RouteOptions& form) {
         check_layer(x, router, bias, {w12_q, w12_s}, {w3_q, w3_s});
         require(addend.device() == x.device() && addend.sizes() == x.sizes(), "MoE: the shared experts' output does not fit the input");
         BlockOptions o{bias, {w12_q, w12_s}, {w3_q, w3_s}, top_k, batch, alpha,
-                       cast_router ? at::autocast::get_autocast_dtype(at::kCUDA) : x.scalar_type(), div, Tensor()};
+                       cast_router ? at::autocast::get_autocast_dtype(at::kCUDA) : x.scalar_type(), div, route_form(form), Tensor()};
+        require(o.form.reference || alpha <= 0, "moe_block: the balance loss is that of the reference's router");
         auto r = BlockNode::apply(x, router, w12, w3, addend, &o);
         return std::make_tuple(r[0], r.size() > 1 ? c10::optional<Tensor>(r[1]) : c10::optional<Tensor>(), o.counts);
     });

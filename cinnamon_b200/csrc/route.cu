@@ -43,6 +43,11 @@ template <> __device__ __forceinline__ float logit<float>(float v) { return v; }
 template <> __device__ __forceinline__ float logit<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }
 template <> __device__ __forceinline__ float logit<__half>(__half v) { return __half2float(v); }
 
+template <typename L> __device__ __forceinline__ L from_float(float v);
+template <> __device__ __forceinline__ float from_float<float>(float v) { return v; }
+template <> __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+template <> __device__ __forceinline__ __half from_float<__half>(float v) { return __float2half_rn(v); }
+
 constexpr int ROUTE_MAX_EXPERTS = 1024;
 constexpr int ROUTE_MAX_TOPK = 32;
 
@@ -111,6 +116,253 @@ route_topk_kernel(const L* __restrict__ logits, const float* __restrict__ bias, 
     }
     __syncthreads();
     for (int e = threadIdx.x; e < E; e += 256) hist[(int64_t)blockIdx.x * E + e] = s_hist[e];
+}
+
+// ---------------------------------------------------------------------------
+// The router's other forms: softmax scores, groups of experts, gates as they are or scaled (moe_route_form)
+//
+//   s = sigmoid(logit) or softmax(logits);  chosen by s + bias: first the groups (of equally many neighbours) with the largest sums of
+//   their two best, then the k best experts in them, ties to the lower id;  gate = scale * s / (sum of the k s + 1e-9), or scale * s
+//
+// Which expert is the last to be chosen can hang on the last bit of a score, so the choice is the one that 64-bit arithmetic makes.
+// Hardly any token needs it: a warp chooses with scores that are off by 2^-20 at most and looks at the gaps between those it
+// chose and to the next one; where one is too small to be sure of (and not a tie of the same logit and bias), the token is chosen
+// again in 64 bits.  Gates come from the chosen experts' logits in fp32.
+//
+// A lane holds VPL neighbouring experts and the largest of their keys (floats as ordered integers); a round is one warp-wide maximum,
+// one vote and a look through the winner's keys.
+// ---------------------------------------------------------------------------
+struct RouteForm {
+    int n_groups, top_groups, renormalise;
+    float scale;
+};
+
+constexpr int ROUTE_MAX_GROUPS = 32;
+
+__device__ __forceinline__ uint32_t ordered(float v) {
+    const uint32_t b = __float_as_uint(v);
+    return b & 0x80000000u ? ~b : b | 0x80000000u;
+}
+__device__ __forceinline__ float unordered(uint32_t k) { return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k); }
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+}
+__device__ __forceinline__ double warp_sum(double v) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+}
+
+// The groups of rank < top_groups among the warp's lanes' scores (lane g: group g), as a mask; equal scores: the lower group first
+template <typename F>
+__device__ __forceinline__ unsigned best_groups(F score, int n_groups, int top_groups, int lane) {
+    int rank = 0;
+    for (int g = 0; g < n_groups; ++g) {
+        const F o = __shfl_sync(0xffffffffu, score, g);
+        rank += o > score || (o == score && g < lane);
+    }
+    return __ballot_sync(0xffffffffu, lane < n_groups && rank < top_groups);
+}
+
+// One token in 64 bits; returns lane r's expert (r < top_k).
+template <int VPL, bool SOFTMAX>
+__device__ __noinline__ int route_exact(const float (&x)[VPL], const float* __restrict__ bias, int E, int top_k, int n_groups, int top_groups) {
+    const int lane = threadIdx.x & 31, e0 = lane * VPL;
+    double sel[VPL];
+    if constexpr (SOFTMAX) {
+        float m = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < VPL; ++i)
+            if (e0 + i < E) m = fmaxf(m, x[i]);
+        m = warp_max(m);
+        double sum = 0.0;
+#pragma unroll
+        for (int i = 0; i < VPL; ++i) {
+            sel[i] = e0 + i < E ? exp((double)x[i] - (double)m) : 0.0;
+            sum += sel[i];
+        }
+        sum = warp_sum(sum);
+#pragma unroll
+        for (int i = 0; i < VPL; ++i) sel[i] /= sum;
+    } else {
+#pragma unroll
+        for (int i = 0; i < VPL; ++i) sel[i] = 1.0 / (1.0 + exp(-(double)x[i]));
+    }
+    unsigned open = 0;                                       // experts that can be chosen
+#pragma unroll
+    for (int i = 0; i < VPL; ++i) {
+        if (e0 + i < E) {
+            if (bias) sel[i] += (double)bias[e0 + i];
+            if (sel[i] != sel[i]) sel[i] = -INFINITY;       // a NaN comes last
+            open |= 1u << i;
+        }
+    }
+    if (n_groups > 1) {
+        const int per = E / n_groups;
+        double mine = -INFINITY;
+        for (int g = 0; g < n_groups; ++g) {
+            double a = -INFINITY, b = -INFINITY;             // the group's two best
+#pragma unroll
+            for (int i = 0; i < VPL; ++i)
+                if ((open >> i & 1) && (e0 + i) / per == g) {
+                    if (sel[i] > a) { b = a; a = sel[i]; }
+                    else if (sel[i] > b) b = sel[i];
+                }
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) {
+                const double oa = __shfl_xor_sync(0xffffffffu, a, o), ob = __shfl_xor_sync(0xffffffffu, b, o);
+                b = oa > a ? fmax(a, ob) : fmax(b, oa);
+                a = fmax(a, oa);
+            }
+            if (lane == g) mine = per > 1 ? a + b : a;
+        }
+        if (mine != mine) mine = -INFINITY;                  // (infinities of both signs)
+        const unsigned groups = best_groups(mine, n_groups, top_groups, lane);
+#pragma unroll
+        for (int i = 0; i < VPL; ++i)
+            if (e0 + i < E && !(groups >> ((e0 + i) / per) & 1)) open &= ~(1u << i);
+    }
+    int my_expert = 0;
+    for (int r = 0; r < top_k; ++r) {
+        double best = 0.0;
+        int best_e = 0x7fffffff;
+#pragma unroll
+        for (int i = VPL - 1; i >= 0; --i)
+            if ((open >> i & 1) && (best_e == 0x7fffffff || sel[i] >= best)) { best = sel[i]; best_e = e0 + i; }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) {
+            const double ov = __shfl_xor_sync(0xffffffffu, best, o);
+            const int oe = __shfl_xor_sync(0xffffffffu, best_e, o);
+            if (oe != 0x7fffffff && (best_e == 0x7fffffff || ov > best || (ov == best && oe < best_e))) { best = ov; best_e = oe; }
+        }
+        if (best_e / VPL == lane) open &= ~(1u << (best_e - e0));
+        if (lane == r) my_expert = best_e;
+    }
+    return my_expert;
+}
+
+template <int VPL, typename L, bool SOFTMAX>                 // E <= 32 * VPL
+__global__ void __launch_bounds__(256)
+route_form_kernel(const L* __restrict__ logits, const float* __restrict__ bias, int T, int E, int top_k, const RouteForm form, int tokens_per_cta,
+                  int* __restrict__ top_experts, float* __restrict__ top_gates, int* __restrict__ hist) {
+    pdl_wait();
+    pdl_trigger();
+    __shared__ int s_hist[ROUTE_MAX_EXPERTS];
+    for (int e = threadIdx.x; e < E; e += 256) s_hist[e] = 0;
+    __syncthreads();
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, e0 = lane * VPL;
+    const int t_end = min((int)(blockIdx.x + 1) * tokens_per_cta, T);
+    for (int t = blockIdx.x * tokens_per_cta + warp; t < t_end; t += 8) {
+        const L* row = logits + (int64_t)t * E;
+        float x[VPL];
+#pragma unroll
+        for (int i = 0; i < VPL; ++i) x[i] = e0 + i < E ? logit<L>(row[e0 + i]) : -INFINITY;
+        float m = 0.0f, sum = 1.0f;
+        if constexpr (SOFTMAX) {
+            m = x[0];
+#pragma unroll
+            for (int i = 1; i < VPL; ++i) m = fmaxf(m, x[i]);
+            m = warp_max(m);
+            float part = 0.0f;
+#pragma unroll
+            for (int i = 0; i < VPL; ++i) part += e0 + i < E ? expf(x[i] - m) : 0.0f;
+            sum = warp_sum(part);
+        }
+        const int my_expert = route_exact<VPL, SOFTMAX>(x, bias, E, top_k, form.n_groups, form.top_groups);
+        float score = 0.0f;
+        if (lane < top_k) {
+            const float v = logit<L>(row[my_expert]);
+            score = SOFTMAX ? __fdiv_rn(expf(v - m), sum) : __fdiv_rn(1.0f, 1.0f + expf(-v));
+        }
+        const float total = warp_sum(score) + 1e-9f;
+        if (lane < top_k) {
+            top_experts[(int64_t)t * top_k + lane] = my_expert;
+            top_gates[(int64_t)t * top_k + lane] = (form.renormalise ? __fdiv_rn(score, total) : score) * form.scale;
+            atomicAdd(&s_hist[my_expert], 1);
+        }
+    }
+    __syncthreads();
+    for (int e = threadIdx.x; e < E; e += 256) hist[(int64_t)blockIdx.x * E + e] = s_hist[e];
+}
+
+// d logits of the gates, from their gradients by slot (d_top), in the order of pair_pos (d_pair) and by sorted pair (d_sorted); null: none.  One warp per
+// token; d score of a chosen expert is scale * d gate, or with renormalised gates scale * (d gate - sum_j d gate_j s_j / S) / S, S = sum of
+// the chosen s + 1e-9; then s (1 - s) d, or for a softmax s_e (d_e - sum_j d_j s_j).  Bound by reading and writing the logits.
+template <int VPL, typename L, bool SOFTMAX>
+__global__ void __launch_bounds__(256)
+route_form_backward_kernel(const L* __restrict__ logits, const int* __restrict__ top_experts, const int64_t* __restrict__ sorted_experts,
+                           const int64_t* __restrict__ pair_pos, const float* __restrict__ d_top, const float* __restrict__ d_pair,
+                           const float* __restrict__ d_sorted, const RouteForm form,
+                           L* __restrict__ d_logits, int64_t T, int E, int top_k) {
+    pdl_wait();
+    pdl_trigger();
+    const int lane = threadIdx.x & 31, e0 = lane * VPL;
+    for (int64_t t = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); t < T; t += (int64_t)gridDim.x * 8) {
+        const L* row = logits + t * E;
+        float x[VPL], m = 0.0f, inv = 1.0f;
+        if constexpr (SOFTMAX) {
+            m = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < VPL; ++i) {
+                x[i] = e0 + i < E ? logit<L>(row[e0 + i]) : -INFINITY;
+                m = fmaxf(m, x[i]);
+            }
+            m = warp_max(m);
+            float part = 0.0f;
+#pragma unroll
+            for (int i = 0; i < VPL; ++i) {
+                x[i] = e0 + i < E ? expf(x[i] - m) : 0.0f;
+                part += x[i];
+            }
+            inv = __fdiv_rn(1.0f, warp_sum(part));
+        }
+        int mine = -1;
+        float s = 0.0f, g = 0.0f;
+        if (lane < top_k) {
+            mine = top_experts[t * top_k + lane];
+            const float v = logit<L>(row[mine]);
+            s = SOFTMAX ? expf(v - m) * inv : __fdiv_rn(1.0f, 1.0f + expf(-v));
+            if (d_top) g = d_top[t * top_k + lane];
+        }
+        if (d_pair || d_sorted) {                                              // lane j: the token's j-th pair, its expert and its gradient
+            int e = -2;
+            float h = 0.0f;
+            if (lane < top_k) {
+                const int64_t at = pair_pos[t * top_k + lane];
+                e = (int)sorted_experts[at];
+                if (d_pair) h = d_pair[t * top_k + lane];
+                if (d_sorted) h += d_sorted[at];
+            }
+            for (int j = 0; j < top_k; ++j) {
+                const int ej = __shfl_sync(0xffffffffu, e, j);
+                const float hj = __shfl_sync(0xffffffffu, h, j);
+                if (ej == mine) g += hj;
+            }
+        }
+        g *= form.scale;
+        if (form.renormalise) {
+            const float total = warp_sum(s) + 1e-9f, dot = warp_sum(g * s);
+            g = lane < top_k ? (g - dot / total) / total : 0.0f;
+        }
+        float d = SOFTMAX ? s * g : s * (1.0f - s) * g;                        // of the chosen expert (softmax: before the sum's part)
+        const float common = SOFTMAX ? warp_sum(d) : 0.0f;
+        float out[VPL];
+#pragma unroll
+        for (int i = 0; i < VPL; ++i) out[i] = SOFTMAX ? -(x[i] * inv) * common : 0.0f;
+        if constexpr (SOFTMAX) d = s * (g - common);
+        for (int j = 0; j < top_k; ++j) {
+            const int e = __shfl_sync(0xffffffffu, mine, j) - e0;
+            const float v = __shfl_sync(0xffffffffu, d, j);
+#pragma unroll
+            for (int i = 0; i < VPL; ++i)
+                if (e == i) out[i] = v;
+        }
+#pragma unroll
+        for (int i = 0; i < VPL; ++i)
+            if (e0 + i < E) d_logits[t * E + e0 + i] = from_float<L>(out[i]);
+    }
 }
 
 __global__ void __launch_bounds__(256)
@@ -268,10 +520,46 @@ static void launch_topk(const L* logits, const float* bias, int T, int E, int to
 #undef CINN_TOPK
 }
 
-// logits_dtype: CINN_F32, or a 16-bit type that is widened on load.  starts / ends (E each): null, or every expert's rows.
-int moe_route(const void* logits, int logits_dtype, const float* bias, int64_t T, int E, int top_k, int* workspace, int* top_experts,
+#define CINN_FORM_VPL(CALL) \
+    do { if (E <= 32) { CALL(1); } else if (E <= 64) { CALL(2); } else if (E <= 128) { CALL(4); } else if (E <= 256) { CALL(8); } \
+         else if (E <= 512) { CALL(16); } else { CALL(32); } } while (0)
+
+template <typename L>
+static void launch_form(const L* logits, const float* bias, int T, int E, int top_k, const RouteForm& form, bool softmax, int per, int n_ctas,
+                        int* top_experts, float* top_gates, int* hist, cudaStream_t st) {
+#define CINN_CALL(V) \
+    if (softmax) launch_dependent(route_form_kernel<V, L, true>, dim3(n_ctas), dim3(256), 0, st, logits, bias, T, E, top_k, form, per, top_experts, top_gates, hist); \
+    else launch_dependent(route_form_kernel<V, L, false>, dim3(n_ctas), dim3(256), 0, st, logits, bias, T, E, top_k, form, per, top_experts, top_gates, hist)
+    CINN_FORM_VPL(CINN_CALL);
+#undef CINN_CALL
+}
+
+template <typename L>
+static void launch_form_backward(const L* logits, const int* top, const int64_t* se, const int64_t* pos, const float* d_top, const float* d_pair,
+                                 const float* d_sorted, const RouteForm& form, bool softmax, L* out, int64_t T, int E, int top_k, cudaStream_t st) {
+    const int64_t want = (T + 7) / 8, cap = (int64_t)sm_count() * 16;
+    const unsigned grid = (unsigned)(want < cap ? want : cap);
+#define CINN_CALL(V) \
+    if (softmax) launch_dependent(route_form_backward_kernel<V, L, true>, dim3(grid), dim3(256), 0, st, logits, top, se, pos, d_top, d_pair, d_sorted, form, out, T, E, top_k); \
+    else launch_dependent(route_form_backward_kernel<V, L, false>, dim3(grid), dim3(256), 0, st, logits, top, se, pos, d_top, d_pair, d_sorted, form, out, T, E, top_k)
+    CINN_FORM_VPL(CINN_CALL);
+#undef CINN_CALL
+}
+
+static int check_form(int scores, int n_groups, int top_groups, int E, int top_k) {
+    CINN_CHECK_ARG(scores == 0 || scores == 1, "moe_route: scores %d (0 sigmoid, 1 softmax)", scores);
+    CINN_CHECK_ARG(n_groups >= 1 && n_groups <= ROUTE_MAX_GROUPS && E % n_groups == 0, "moe_route: %d experts in %d groups (1 to %d groups of equally many)",
+                   E, n_groups, ROUTE_MAX_GROUPS);
+    CINN_CHECK_ARG(top_groups >= 1 && top_groups <= n_groups && top_k <= top_groups * (E / n_groups),
+                   "moe_route: %d experts out of %d of %d groups of %d", top_k, top_groups, n_groups, E / n_groups);
+    return CINN_OK;
+}
+
+// logits_dtype: CINN_F32, or a 16-bit type that is widened on load.  starts / ends (E each): null, or every expert's rows.  form: null, or what
+// the scores and gates are (with a bias that may be null then).
+static int moe_route(const void* logits, int logits_dtype, const float* bias, int64_t T, int E, int top_k, int* workspace, int* top_experts,
               float* top_gates, int64_t* token_indices, float* sorted_scores, int64_t* sorted_experts, int64_t* counts,
-              int64_t* starts, int64_t* ends, int64_t* pair_pos, float* pair_gate, cudaStream_t st) {
+              int64_t* starts, int64_t* ends, int64_t* pair_pos, float* pair_gate, cudaStream_t st, const RouteForm* form, bool softmax) {
     CINN_CHECK_ARG(T >= 0 && E >= 1 && E <= ROUTE_MAX_EXPERTS, "moe_route: 1 <= E <= %d experts (got %d)", ROUTE_MAX_EXPERTS, E);
     CINN_CHECK_ARG(top_k >= 1 && top_k <= ROUTE_MAX_TOPK && top_k <= E, "moe_route: 1 <= top_k <= min(E, %d) (got %d)",
                    ROUTE_MAX_TOPK, top_k);
@@ -287,12 +575,16 @@ int moe_route(const void* logits, int logits_dtype, const float* bias, int64_t T
         }
         return CINN_OK;
     }
-    CINN_CHECK_ARG(logits && bias && workspace && top_experts && top_gates && token_indices && sorted_scores &&
+    CINN_CHECK_ARG(logits && (bias || form) && workspace && top_experts && top_gates && token_indices && sorted_scores &&
                    sorted_experts && pair_pos && pair_gate, "moe_route: null pointer");
     const int per = route_tokens_per_cta(T, E), n_ctas = (int)((T + per - 1) / per);
     int* hist = workspace;
     int* totals = n_ctas > ROUTE_FEW_CTAS ? workspace + (int64_t)n_ctas * E : nullptr;
-    if (logits_dtype == CINN_F32) launch_topk((const float*)logits, bias, (int)T, E, top_k, per, n_ctas, top_experts, top_gates, hist, st);
+    if (form) {
+        if (logits_dtype == CINN_F32) launch_form((const float*)logits, bias, (int)T, E, top_k, *form, softmax, per, n_ctas, top_experts, top_gates, hist, st);
+        else if (logits_dtype == CINN_BF16) launch_form((const __nv_bfloat16*)logits, bias, (int)T, E, top_k, *form, softmax, per, n_ctas, top_experts, top_gates, hist, st);
+        else launch_form((const __half*)logits, bias, (int)T, E, top_k, *form, softmax, per, n_ctas, top_experts, top_gates, hist, st);
+    } else if (logits_dtype == CINN_F32) launch_topk((const float*)logits, bias, (int)T, E, top_k, per, n_ctas, top_experts, top_gates, hist, st);
     else if (logits_dtype == CINN_BF16) launch_topk((const __nv_bfloat16*)logits, bias, (int)T, E, top_k, per, n_ctas, top_experts, top_gates, hist, st);
     else launch_topk((const __half*)logits, bias, (int)T, E, top_k, per, n_ctas, top_experts, top_gates, hist, st);
     CINN_CHECK_LAUNCH();
@@ -302,6 +594,40 @@ int moe_route(const void* logits, int logits_dtype, const float* bias, int64_t T
     }
     launch_dependent(route_scatter_kernel, dim3(n_ctas), dim3(256), 0, st, top_experts, top_gates, hist, totals, (int)T, E, top_k, per, token_indices, sorted_scores,
                                                  sorted_experts, counts, starts, ends, pair_pos, pair_gate);
+    CINN_CHECK_LAUNCH();
+    return CINN_OK;
+}
+
+int moe_route(const void* logits, int logits_dtype, const float* bias, int64_t T, int E, int top_k, int* workspace, int* top_experts,
+              float* top_gates, int64_t* token_indices, float* sorted_scores, int64_t* sorted_experts, int64_t* counts,
+              int64_t* starts, int64_t* ends, int64_t* pair_pos, float* pair_gate, cudaStream_t st) {
+    return moe_route(logits, logits_dtype, bias, T, E, top_k, workspace, top_experts, top_gates, token_indices, sorted_scores, sorted_experts, counts,
+                     starts, ends, pair_pos, pair_gate, st, nullptr, false);
+}
+
+int moe_route_form(const void* logits, int logits_dtype, const float* bias, int64_t T, int E, int top_k, int scores, int n_groups, int top_groups,
+                   int renormalise, float scale, int* workspace, int* top_experts, float* top_gates, int64_t* token_indices, float* sorted_scores,
+                   int64_t* sorted_experts, int64_t* counts, int64_t* starts, int64_t* ends, int64_t* pair_pos, float* pair_gate, cudaStream_t st) {
+    CINN_CHECK_ARG(E >= 1, "moe_route: no experts");
+    int rc = check_form(scores, n_groups, top_groups, E, top_k);
+    if (rc) return rc;
+    const RouteForm form{n_groups, top_groups, renormalise != 0, scale};
+    return moe_route(logits, logits_dtype, bias, T, E, top_k, workspace, top_experts, top_gates, token_indices, sorted_scores, sorted_experts, counts,
+                     starts, ends, pair_pos, pair_gate, st, &form, scores == 1);
+}
+
+int moe_route_form_backward(const void* logits, int logits_dtype, const int* top_experts, const int64_t* sorted_experts, const int64_t* pair_pos,
+                            const float* d_top, const float* d_pair, const float* d_sorted, int64_t T, int E, int top_k, int scores, int renormalise, float scale,
+                            void* d_logits, cudaStream_t st) {
+    CINN_CHECK_ARG(T >= 0 && E >= 1 && E <= ROUTE_MAX_EXPERTS && top_k >= 1 && top_k <= ROUTE_MAX_TOPK && top_k <= E && (scores == 0 || scores == 1),
+                   "moe_route backward: bad shape");
+    CINN_CHECK_ARG(logits_dtype == CINN_F32 || logits_dtype == CINN_BF16 || logits_dtype == CINN_F16, "moe_route: unknown dtype tag %d", logits_dtype);
+    if (T == 0) return CINN_OK;
+    CINN_CHECK_ARG(logits && top_experts && d_logits && ((!d_pair && !d_sorted) || (sorted_experts && pair_pos)), "moe_route backward: null pointer");
+    const RouteForm form{1, 1, renormalise != 0, scale};
+    if (logits_dtype == CINN_F32) launch_form_backward((const float*)logits, top_experts, sorted_experts, pair_pos, d_top, d_pair, d_sorted, form, scores == 1, (float*)d_logits, T, E, top_k, st);
+    else if (logits_dtype == CINN_BF16) launch_form_backward((const __nv_bfloat16*)logits, top_experts, sorted_experts, pair_pos, d_top, d_pair, d_sorted, form, scores == 1, (__nv_bfloat16*)d_logits, T, E, top_k, st);
+    else launch_form_backward((const __half*)logits, top_experts, sorted_experts, pair_pos, d_top, d_pair, d_sorted, form, scores == 1, (__half*)d_logits, T, E, top_k, st);
     CINN_CHECK_LAUNCH();
     return CINN_OK;
 }

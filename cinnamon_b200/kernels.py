@@ -1017,12 +1017,34 @@ def p2p_return(rows, seg_start, home_base, peer_home, n_ranks: int, capacity_row
                                       _stream(rows)), "cinn_p2p_return")
 
 
-def moe_route(logits: torch.Tensor, bias: torch.Tensor, top_k: int):
+_SCORES = {"sigmoid": 0, "softmax": 1}
+
+
+def _route_options(scores="sigmoid", n_groups=1, top_groups=1, renormalise=True, scale=1.0, no_bias=False):
+    """A router's form as the native calls take it; the last item: whether it is the reference's."""
+    assert scores in _SCORES, "scores must be 'sigmoid' or 'softmax'"
+    reference = scores == "sigmoid" and n_groups == 1 and top_groups == 1 and bool(renormalise) and scale == 1.0 and not no_bias
+    return _SCORES[scores], int(n_groups), int(top_groups), bool(renormalise), float(scale), reference
+
+
+def moe_route(logits: torch.Tensor, bias: torch.Tensor, top_k: int, scores: str = "sigmoid", n_groups: int = 1, top_groups: int = 1,
+              renormalise: bool = True, scale: float = 1.0):
     """Routing of ``MoE.forward`` (reference src/layers.py:122-148) from the router's logits (evaluated in fp32), on the
     device and without a host synchronisation: sigmoid scores, top-k of score + bias, normalised gates, and the
     (token, expert) pairs in the order of a stable sort by expert.  Returns a dict of tensors:
     ``top_experts`` (T, k) int32, ``top_gates`` (T, k), ``token_indices`` / ``sorted_scores`` /
-    ``sorted_experts`` (T*k), ``counts`` and the row ranges ``starts`` / ``ends`` (E) int64, ``pair_pos`` / ``pair_gate`` (T, k)."""
+    ``sorted_experts`` (T*k), ``counts`` and the row ranges ``starts`` / ``ends`` (E) int64, ``pair_pos`` / ``pair_gate`` (T, k).
+    Where ``logits`` requires a gradient, it reaches them through ``top_gates``, ``pair_gate`` and ``sorted_scores`` (the gates by
+    slot, by rising position, by expert).
+
+    The router's other forms: ``scores`` "softmax" over the experts; ``n_groups`` (1 to 32) groups of equally many neighbouring experts, of which
+    the ``top_groups`` whose two best scores + bias add up to the most are open to a token; gates without ``renormalise``, the scores as
+    they are; gates times ``scale``; ``bias`` None.  Ties go to the lower id, NaN comes last, and
+    no expert is chosen twice.  The form of the reference (all defaults) is computed as the reference computes it, its scores in fp32; in the
+    others the choice is that of 64-bit arithmetic."""
+    form = _route_options(scores, n_groups, top_groups, renormalise, scale, bias is None)
+    if not form[-1] or (torch.is_grad_enabled() and logits.requires_grad):
+        return _host.moe_route(logits, bias, int(top_k), form)
     assert logits.is_cuda and bias.is_cuda, "Inputs must be on CUDA"
     assert logits.ndim == 2, "logits must be (tokens, experts)"
     logits = (logits if logits.dtype in _DTYPE_TAG else logits.float()).contiguous()

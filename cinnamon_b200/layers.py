@@ -78,11 +78,13 @@ class GroupedExperts(nn.Module):
 
 class MoE(nn.Module):
     """Routed + shared experts (src/layers.py:89-179).  ``group``: process group over which the routed experts are
-    sharded (None = all experts on this rank)."""
+    sharded (None = all experts on this rank).  ``router_form``: softmax scores, groups of experts, gates that are scaled or not
+    renormalised, in the place of the reference's router."""
 
     def __init__(self, n_routed, n_shared, top_k, d_model, hidden_dim, expert_scale, gamma, balance_alpha=0.0, group=None,
-                 exchange: str = "nccl"):
+                 exchange: str = "nccl", router_form: _moe.RouterForm = _moe.RouterForm()):
         super().__init__()
+        self.router_form = router_form.check(n_routed, top_k)
         assert exchange in ("nccl", "p2p"), "exchange: 'nccl' (all-to-all collectives) or 'p2p' (peer stores over NVLink)"
         self.exchange = exchange
         self._peer = None                # p2p.PeerBuffers, allocated (collectively) by the first sharded call on GPUs
@@ -141,11 +143,12 @@ class MoE(nn.Module):
         nodes."""
         from . import kernels as K
         ex, r = self.routed_experts, self.router
+        reference = self.router_form == _moe.RouterForm()
         plain = (type(ex) is GroupedExperts and type(r) is nn.Linear and r.bias is None and not K.has_hooks(ex) and not K.has_hooks(r))
         if self.balance_alpha > 0 and shared_out.requires_grad:
             plain = plain and all(type(e) is SwiGLU and not K.has_hooks(e) and K.swiglu_block_ready(x, e.w1, e.w2, e.w3)
                                   for e in self.shared_experts)
-        return (plain and not self.sharded and flat.shape[0] > 0 and not torch.compiler.is_compiling() and K.gemm_events is None
+        return (plain and (reference or self.balance_alpha <= 0) and not self.sharded and flat.shape[0] > 0 and not torch.compiler.is_compiling() and K.gemm_events is None
                 and K._MOE_GROUPED_PRECISION == "fp8" and ex.d_model % 256 == 0 and ex.hidden_dim % 256 == 0
                 and all(w.dtype in (torch.float32, torch.bfloat16) and w.is_contiguous() for w in (ex.w12, ex.w3))
                 and flat.dtype in K._DTYPE_TAG and shared_out.dtype in K._DTYPE_TAG and self.expert_bias.dtype == torch.float32
@@ -158,7 +161,8 @@ class MoE(nn.Module):
         y, balance, counts = K._host.moe_block(flat.contiguous(), self.router.weight, ex.w12, ex.w3,
                                                shared_out.reshape(flat.shape).contiguous(), self.expert_bias, *K.cached_expert_weights(ex.w12),
                                                *K.cached_expert_weights(ex.w3), self.top_k, batch, float(self.balance_alpha),
-                                               torch.is_autocast_enabled("cuda"), K._DIV_MODE)
+                                               torch.is_autocast_enabled("cuda"), K._DIV_MODE,
+                                               K._route_options(**self.router_form.options()))
         if self.training:
             K._host.moe_update_bias(self.expert_bias, counts, flat.shape[0] * self.top_k / self.n_routed, self.gamma)
         return y.view(batch, seq, -1), balance
@@ -170,21 +174,21 @@ class MoE(nn.Module):
         if flat.is_cuda and self._native_ready(x, flat, shared_out):
             return self._forward_native(flat, shared_out, batch, seq)
         logits = self.router(flat)
-        scores = torch.sigmoid(logits.float())
+        form = self.router_form
+        scores = form.all_scores(logits.float())
         if flat.is_cuda:
             from . import kernels as K
-            r = K.moe_route(logits.detach(), self.expert_bias, self.top_k)
+            r = K.moe_route(logits.detach(), self.expert_bias, self.top_k, **form.options())
             routing = _moe.Routing(token_indices=r["token_indices"], sorted_scores=r["sorted_scores"],
                                    sorted_experts=r["sorted_experts"], counts=r["counts"], pair_pos=r["pair_pos"],
                                    pair_gate=r["pair_gate"])
             top_idx = r["top_experts"].long()
         else:
-            routing = _moe.route_torch(logits.detach().float(), self.expert_bias, self.top_k, self.n_routed)
-            top_idx = (scores.detach() + self.expert_bias).topk(self.top_k, dim=-1).indices
+            routing = _moe.route_torch(logits.detach().float(), self.expert_bias, self.top_k, self.n_routed, form)
+            top_idx = form.choose(scores.detach(), self.expert_bias, self.top_k)
         # the gates once more, differentiably, in the order of routing.pair_pos (a token's pairs by ascending expert)
         chosen = top_idx.sort(dim=-1).values
-        picked = scores.gather(-1, chosen)
-        gates = picked / (picked.sum(dim=-1, keepdim=True) + 1e-9)
+        gates = form.gates(scores.gather(-1, chosen))
         experts = lambda rows, starts, ends: self.routed_experts(rows, starts, ends)          # noqa: E731
         peer = None
         if self.sharded and self.exchange == "p2p" and flat.is_cuda:

@@ -39,6 +39,45 @@ class Routing:
     pair_gate: torch.Tensor = None  # (T, k) the gates in the same order
 
 
+@dataclass(frozen=True)
+class RouterForm:
+    """What a router makes of its logits (``kernels.moe_route``); the defaults are the reference's form."""
+    scores: str = "sigmoid"        # or "softmax"
+    n_groups: int = 1              # groups of equally many neighbouring experts, of which
+    top_groups: int = 1            # so many are open to a token
+    renormalise: bool = True       # gates that add up to ``scale``
+    scale: float = 1.0
+
+    def check(self, n_experts: int, top_k: int) -> "RouterForm":
+        assert self.scores in ("sigmoid", "softmax"), "scores must be 'sigmoid' or 'softmax'"
+        assert 1 <= self.n_groups <= 32 and n_experts % self.n_groups == 0, "1 to 32 groups of equally many experts"
+        assert 1 <= self.top_groups <= self.n_groups and top_k <= self.top_groups * (n_experts // self.n_groups), \
+            "the open groups must hold top_k experts"
+        return self
+
+    def options(self) -> dict:
+        return dict(scores=self.scores, n_groups=self.n_groups, top_groups=self.top_groups, renormalise=self.renormalise, scale=self.scale)
+
+    def all_scores(self, logits: torch.Tensor) -> torch.Tensor:
+        return torch.sigmoid(logits) if self.scores == "sigmoid" else torch.softmax(logits, dim=-1)
+
+    def choose(self, scores: torch.Tensor, bias: torch.Tensor, top_k: int) -> torch.Tensor:
+        """The experts of every token, in torch (host logic and CPU tensors)."""
+        by = scores + bias
+        if self.n_groups > 1:
+            groups = by.unflatten(-1, (self.n_groups, -1))
+            best = groups.topk(min(2, groups.shape[-1]), dim=-1).values.sum(-1).topk(self.top_groups, dim=-1).indices
+            closed = torch.ones_like(groups[..., 0], dtype=torch.bool).scatter_(-1, best, False)
+            by = by.masked_fill(closed.repeat_interleave(groups.shape[-1], dim=-1), float("-inf"))
+        return by.topk(top_k, dim=-1).indices
+
+    def gates(self, picked: torch.Tensor) -> torch.Tensor:
+        """Gates of the chosen experts' scores."""
+        if self.renormalise:
+            picked = picked / (picked.sum(dim=-1, keepdim=True) + 1e-9)
+        return picked if self.scale == 1.0 else picked * self.scale
+
+
 def router_logits(x: torch.Tensor, router_weight: torch.Tensor) -> torch.Tensor:
     """The reference's router is an ``nn.Linear`` under autocast (src/layers.py:122): a 16-bit GEMM for 16-bit
     activations, scores in fp32 afterwards."""
@@ -49,28 +88,27 @@ def router_logits(x: torch.Tensor, router_weight: torch.Tensor) -> torch.Tensor:
     return torch.nn.functional.linear(x.float(), router_weight.float())
 
 
-def route(x: torch.Tensor, router_weight: torch.Tensor, expert_bias: torch.Tensor, top_k: int) -> Routing:
+def route(x: torch.Tensor, router_weight: torch.Tensor, expert_bias: torch.Tensor, top_k: int, form: RouterForm = RouterForm()) -> Routing:
     """Router of ``MoE.forward`` (src/layers.py:122-148): sigmoid scores, top-k on
-    scores + bias, gates normalised over the selected experts, pairs sorted by expert.
+    scores + bias, gates normalised over the selected experts, pairs sorted by expert (or another ``form``).
     On a GPU everything after the router GEMM is two or three kernel launches (``kernels.moe_route``) with no host
     synchronisation; on the CPU (host-logic tests) it is the reference's chain of torch calls."""
     n_experts = router_weight.shape[0]
     logits = router_logits(x, router_weight)
     if logits.is_cuda:
         from . import kernels as K
-        r = K.moe_route(logits, expert_bias, top_k)
+        r = K.moe_route(logits.detach(), expert_bias, top_k, **form.options())
         return Routing(token_indices=r["token_indices"], sorted_scores=r["sorted_scores"],
                        sorted_experts=r["sorted_experts"], counts=r["counts"], pair_pos=r["pair_pos"],
                        pair_gate=r["pair_gate"])
-    return route_torch(logits, expert_bias, top_k, n_experts)
+    return route_torch(logits, expert_bias, top_k, n_experts, form)
 
 
-def route_torch(logits: torch.Tensor, expert_bias: torch.Tensor, top_k: int, n_experts: int) -> Routing:
+def route_torch(logits: torch.Tensor, expert_bias: torch.Tensor, top_k: int, n_experts: int, form: RouterForm = RouterForm()) -> Routing:
     """The routing arithmetic as the reference writes it (src/layers.py:122-148), in torch."""
-    scores = torch.sigmoid(logits)
-    _, top_idx = (scores + expert_bias).topk(top_k, dim=-1)
-    top_scores = scores.gather(-1, top_idx)
-    top_scores = top_scores / (top_scores.sum(dim=-1, keepdim=True) + 1e-9)
+    scores = form.all_scores(logits)
+    top_idx = form.choose(scores, expert_bias, top_k)
+    top_scores = form.gates(scores.gather(-1, top_idx))
     expanded = top_idx.reshape(-1)
     sorted_experts, order = expanded.sort(stable=True)
     # where each (token, slot) pair sits in the sorted order, per token in ascending position
@@ -679,8 +717,9 @@ class ExpertParallelMoE(torch.nn.Module):
     def __init__(self, router_weight: torch.Tensor, expert_bias: torch.Tensor, w12_local: torch.Tensor,
                  w3_local: torch.Tensor, top_k: int, group=None, shared: Optional[FP8SwiGLU] = None, n_chunks: int = 1,
                  exchange: str = "nccl", max_tokens_per_rank: Optional[int] = None, check_status_every: int = 0,
-                 up_splits: int = 1, dispatch_sms: int = 0):
-        """``max_tokens_per_rank`` (peer-store exchanges): the largest number of tokens any rank will ever bring to a
+                 up_splits: int = 1, dispatch_sms: int = 0, router_form: RouterForm = RouterForm()):
+        """``router_form``: scores, groups and gates of the router, where they are not the reference's.
+        ``max_tokens_per_rank`` (peer-store exchanges): the largest number of tokens any rank will ever bring to a
         call; it sizes the receive buffers, whose allocation is a collective, so it must be the same on every rank.
         When omitted the first call agrees on it (one all-reduce of the ranks' token counts, on the first call
         only); a later call with more tokens raises instead of re-allocating (a rank re-allocating on its own would
@@ -692,6 +731,7 @@ class ExpertParallelMoE(torch.nn.Module):
         ``dispatch_sms`` ("p2p-fused" with a shared expert; 0 = off): the peer stores of the dispatch come from that
         many SMs and the shared expert's GEMMs run beside them on the other SMs, instead of after the dispatch."""
         super().__init__()
+        self.router_form = router_form.check(router_weight.shape[0], top_k)
         self.up_splits = int(up_splits)
         self.dispatch_sms = int(dispatch_sms)
         self.max_tokens_per_rank = max_tokens_per_rank
@@ -734,7 +774,8 @@ class ExpertParallelMoE(torch.nn.Module):
             e, sh = self.experts, self.shared
             shared = (None,) * 4 if sh is None else (sh.w12_q, sh.w12_s, sh.w3_q, sh.w3_s)
             y = self.K._host.moe_forward(flat.contiguous(), router, self.expert_bias, self.top_k, e.w12_q, e.w12_s, e.w3_q, e.w3_s,
-                                         *shared, sh is not None and sh.round_scale, self.K._DIV_MODE)
+                                         *shared, sh is not None and sh.round_scale, self.K._DIV_MODE,
+                                         self.K._route_options(**self.router_form.options()))
             return y.reshape(x.shape)
         world = dist.get_world_size(self.group) if dist.is_initialized() else 1
         sh, join = None, None
@@ -771,7 +812,7 @@ class ExpertParallelMoE(torch.nn.Module):
             _mark(self.trace, "shared expert (on the main stream: one rank)")
         if world > 1 and self.exchange in ("p2p", "p2p-fused") and flat.is_cuda:
             from . import p2p
-            r = route(flat, router, self.expert_bias, self.top_k)
+            r = route(flat, router, self.expert_bias, self.top_k, self.router_form)
             _mark(self.trace, "router GEMM + routing")
             T, d = flat.shape
             if self._peer_buffers is None:
@@ -807,13 +848,13 @@ class ExpertParallelMoE(torch.nn.Module):
                     raise RuntimeError(f"expert-parallel exchange: device status {status >> 8}/{status & 255} (a bounded wait "
                                        "ran out or a row fell outside a buffer); the outputs since the last check are invalid")
         elif world > 1 and self.n_chunks > 1 and flat.shape[0] >= self.n_chunks:
-            routings = [route(c, router, self.expert_bias, self.top_k) for c in torch.tensor_split(flat, self.n_chunks)]
+            routings = [route(c, router, self.expert_bias, self.top_k, self.router_form) for c in torch.tensor_split(flat, self.n_chunks)]
             if launch_shared is not None:
                 sh = launch_shared()
             y = moe_forward_pipelined(flat, routings, self.experts, self.K.quantize_fp8_rowwise, self.group, addend=sh,
                                       before_combine=join)
         else:
-            r = route(flat, router, self.expert_bias, self.top_k)
+            r = route(flat, router, self.expert_bias, self.top_k, self.router_form)
             _mark(self.trace, "router GEMM + routing")
             if launch_shared is not None:
                 sh = launch_shared()
