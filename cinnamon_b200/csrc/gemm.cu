@@ -1157,11 +1157,12 @@ int read_indexer_status(int* out, int reset);
 int read_attn_status(int* out, int reset);
 int read_linear_few_status(int* out, int reset);
 int read_loss_status(int* out, int reset);
+int read_rotary_status(int* out, int reset);
 
 // One word for the caller: the GEMM's code if it has one, else the quantisers', the exchange kernels', the indexer's,
-// the attention's, the few-row linear's, the cross entropy's.
+// the attention's, the few-row linear's, the cross entropy's, the rotary positions'.
 int read_device_status(int* out, int reset) {
-    int v = 0, q = 0, m = 0, x = 0, a = 0, f = 0, l = 0;
+    int v = 0, q = 0, m = 0, x = 0, a = 0, f = 0, l = 0, r = 0;
     CINN_CHECK_CUDA(cudaMemcpyFromSymbol(&v, g_device_status, sizeof(int)));
     if (reset && v != 0) {
         int z = 0;
@@ -1179,7 +1180,9 @@ int read_device_status(int* out, int reset) {
     if (rc) return rc;
     rc = read_loss_status(&l, reset);
     if (rc) return rc;
-    *out = v != 0 ? v : (q != 0 ? q : (m != 0 ? m : (x != 0 ? x : (a != 0 ? a : (f != 0 ? f : l)))));
+    rc = read_rotary_status(&r, reset);
+    if (rc) return rc;
+    *out = v != 0 ? v : (q != 0 ? q : (m != 0 ? m : (x != 0 ? x : (a != 0 ? a : (f != 0 ? f : (l != 0 ? l : r))))));
     return CINN_OK;
 }
 

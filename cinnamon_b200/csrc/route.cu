@@ -167,9 +167,12 @@ __device__ __forceinline__ unsigned best_groups(F score, int n_groups, int top_g
 }
 
 // One token in 64 bits; returns lane r's expert (r < top_k).
-template <int VPL, bool SOFTMAX>
-__device__ __noinline__ int route_exact(const float (&x)[VPL], const float* __restrict__ bias, int E, int top_k, int n_groups, int top_groups) {
+template <int VPL, typename L, bool SOFTMAX>
+__device__ __noinline__ int route_exact(const L* __restrict__ row, const float* __restrict__ bias, int E, int top_k, int n_groups, int top_groups) {
     const int lane = threadIdx.x & 31, e0 = lane * VPL;
+    float x[VPL];
+#pragma unroll
+    for (int i = 0; i < VPL; ++i) x[i] = e0 + i < E ? logit<L>(row[e0 + i]) : -INFINITY;
     double sel[VPL];
     if constexpr (SOFTMAX) {
         float m = -INFINITY;
@@ -243,9 +246,47 @@ __device__ __noinline__ int route_exact(const float (&x)[VPL], const float* __re
     return my_expert;
 }
 
+__device__ __forceinline__ float exp2_approx(float x) {          // relative error 2^-22
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+__device__ __forceinline__ float rcp_approx(float x) {           // relative error 2^-23
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+
+// a lane's VPL neighbouring logits; vec: rows of whole, aligned pieces
+template <int VPL, typename L>
+__device__ __forceinline__ void load_logits(const L* __restrict__ row, int e0, int E, bool vec, float (&x)[VPL]) {
+    constexpr int BYTES = VPL * (int)sizeof(L) < 16 ? VPL * (int)sizeof(L) : 16, PER = BYTES / (int)sizeof(L);
+    struct alignas(BYTES) Piece { L v[PER]; };
+    if (vec) {
+#pragma unroll
+        for (int i = 0; i < VPL; i += PER) {
+            if (e0 < E) {
+                const Piece q = *reinterpret_cast<const Piece*>(row + e0 + i);
+#pragma unroll
+                for (int j = 0; j < PER; ++j) x[i + j] = logit<L>(q.v[j]);
+            } else {
+#pragma unroll
+                for (int j = 0; j < PER; ++j) x[i + j] = -INFINITY;
+            }
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < VPL; ++i) x[i] = e0 + i < E ? logit<L>(row[e0 + i]) : -INFINITY;
+    }
+}
+
+// Errors of the quick scores.  Sigmoid: the exponent's rounding is |x| 2^-24 of e^-x, its part in the score s (1 - s) |x| 2^-24 < 2^-26, and
+// ex2, the sum and rcp add less than 2^-22: two scores are sure to be in order when they are 2^-20 apart (and 2^-22 of themselves, for
+// the bias's sum).  Softmax: p |x - max| 2^-24 is below 2^-25 of the largest p, ex2, the sum and the quotient are 2^-21 of p: 2^-19 of
+// the largest p.  A group's sum of two: twice as much.
 template <int VPL, typename L, bool SOFTMAX>                 // E <= 32 * VPL
 __global__ void __launch_bounds__(256)
-route_form_kernel(const L* __restrict__ logits, const float* __restrict__ bias, int T, int E, int top_k, const RouteForm form, int tokens_per_cta,
+route_form_kernel(const L* __restrict__ logits, const float* __restrict__ bias, int T, int E, int top_k, const RouteForm form, int tokens_per_cta, int vec,
                   int* __restrict__ top_experts, float* __restrict__ top_gates, int* __restrict__ hist) {
     pdl_wait();
     pdl_trigger();
@@ -254,28 +295,140 @@ route_form_kernel(const L* __restrict__ logits, const float* __restrict__ bias, 
     __syncthreads();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, e0 = lane * VPL;
     const int t_end = min((int)(blockIdx.x + 1) * tokens_per_cta, T);
+    const int per = E / form.n_groups, lanes_per = per / VPL;                  // a group's experts; its lanes, where they are whole
+    const bool whole = form.n_groups > 1 && per % VPL == 0 && (lanes_per & (lanes_per - 1)) == 0;
+    float b[VPL];
+#pragma unroll
+    for (int i = 0; i < VPL; ++i) b[i] = bias && e0 + i < E ? bias[e0 + i] : 0.0f;
     for (int t = blockIdx.x * tokens_per_cta + warp; t < t_end; t += 8) {
         const L* row = logits + (int64_t)t * E;
-        float x[VPL];
+        float m = 0.0f, sum = 1.0f, near;
+        uint32_t key[VPL];                                                     // score + bias, ordered; 0: not to be chosen
+        bool unsure = false;
+        {
+            float x[VPL];
+            load_logits<VPL, L>(row, e0, E, vec, x);
+            if constexpr (SOFTMAX) {
+                m = x[0];
 #pragma unroll
-        for (int i = 0; i < VPL; ++i) x[i] = e0 + i < E ? logit<L>(row[e0 + i]) : -INFINITY;
-        float m = 0.0f, sum = 1.0f;
-        if constexpr (SOFTMAX) {
-            m = x[0];
+                for (int i = 1; i < VPL; ++i) m = fmaxf(m, x[i]);
+                m = warp_max(m);
+                float part = 0.0f;
 #pragma unroll
-            for (int i = 1; i < VPL; ++i) m = fmaxf(m, x[i]);
-            m = warp_max(m);
-            float part = 0.0f;
+                for (int i = 0; i < VPL; ++i) {
+                    x[i] = exp2_approx((x[i] - m) * 1.4426950408889634f);
+                    part += x[i];
+                }
+                sum = warp_sum(part);
+                const float inv = rcp_approx(sum);
+                near = inv * 0x1p-19f;
 #pragma unroll
-            for (int i = 0; i < VPL; ++i) part += e0 + i < E ? expf(x[i] - m) : 0.0f;
-            sum = warp_sum(part);
+                for (int i = 0; i < VPL; ++i) x[i] = fmaf(x[i], inv, b[i]);
+            } else {
+                near = 0x1p-20f;
+#pragma unroll
+                for (int i = 0; i < VPL; ++i) x[i] = rcp_approx(1.0f + exp2_approx(x[i] * -1.4426950408889634f)) + b[i];
+            }
+#pragma unroll
+            for (int i = 0; i < VPL; ++i) {
+                unsure |= x[i] != x[i];
+                key[i] = e0 + i < E ? ordered(x[i]) : 0u;
+            }
         }
-        const int my_expert = route_exact<VPL, SOFTMAX>(x, bias, E, top_k, form.n_groups, form.top_groups);
+        unsure = __any_sync(0xffffffffu, unsure);
+        if (form.n_groups > 1 && !unsure) {
+            float mine = -INFINITY;                                            // lane g: group g's score
+            if (whole) {
+                uint32_t a = key[0], c = 0;                                    // the lane's two best, then the group's
+#pragma unroll
+                for (int i = 1; i < VPL; ++i) { c = max(c, min(a, key[i])); a = max(a, key[i]); }
+                for (int o = 1; o < lanes_per; o <<= 1) {
+                    const uint32_t oa = __shfl_xor_sync(0xffffffffu, a, o), oc = __shfl_xor_sync(0xffffffffu, c, o);
+                    c = max(min(a, oa), max(c, oc));
+                    a = max(a, oa);
+                }
+                const float score = per > 1 ? unordered(a) + unordered(c) : unordered(a);
+                const float of_group = __shfl_sync(0xffffffffu, score, (lane * lanes_per) & 31);
+                if (lane < form.n_groups) mine = of_group;
+            } else {
+                for (int g = 0; g < form.n_groups; ++g) {
+                    uint32_t a = 0, c = 0;
+#pragma unroll
+                    for (int i = 0; i < VPL; ++i) {
+                        const uint32_t k = e0 + i >= g * per && e0 + i < (g + 1) * per ? key[i] : 0u;
+                        c = max(c, min(a, k));
+                        a = max(a, k);
+                    }
+                    const uint32_t top = __reduce_max_sync(0xffffffffu, a);
+                    const int owner = __ffs(__ballot_sync(0xffffffffu, a == top)) - 1;
+                    const uint32_t next = __reduce_max_sync(0xffffffffu, lane == owner ? c : a);
+                    if (lane == g) mine = per > 1 ? unordered(top) + unordered(next) : unordered(top);
+                }
+            }
+            unsure = __any_sync(0xffffffffu, mine != mine);
+            const unsigned groups = best_groups(mine, form.n_groups, form.top_groups, lane);
+            const bool in = groups >> lane & 1;
+            const float worst = unordered(__reduce_min_sync(0xffffffffu, in ? ordered(mine) : 0xffffffffu));
+            const float next = unordered(__reduce_max_sync(0xffffffffu, in || lane >= form.n_groups ? ordered(-INFINITY) : ordered(mine)));
+            if (form.top_groups < form.n_groups && !(worst - next > 2.0f * near + fabsf(worst) * 0x1p-21f)) unsure = true;
+#pragma unroll
+            for (int i = 0; i < VPL; ++i)
+                if (e0 + i < E && !(groups >> ((unsigned)(e0 + i) / (unsigned)per) & 1)) key[i] = 0u;
+        }
+        int my_expert = 0;
+        float my_logit = 0.0f;
+        if (!unsure) {
+            uint32_t best = 0, my_key = 0;
+            int at = 0;
+            auto look = [&]() {
+                best = 0;
+#pragma unroll
+                for (int i = 0; i < VPL; ++i)
+                    if (key[i] > best) { best = key[i]; at = i; }
+            };
+            auto take = [&](uint32_t& top) {                                   // the best expert left, out of the list; -1: there is none
+                top = __reduce_max_sync(0xffffffffu, best);
+                const int w = __ffs(__ballot_sync(0xffffffffu, best == top)) - 1;
+                const int e = w * VPL + __shfl_sync(0xffffffffu, at, w);
+                if (lane == w) {
+#pragma unroll
+                    for (int i = 0; i < VPL; ++i)
+                        if (i == at) key[i] = 0u;
+                    look();
+                }
+                return top ? e : -1;
+            };
+            look();
+            for (int r = 0; r < top_k; ++r) {
+                uint32_t top;
+                const int e = take(top);
+                if (lane == r) { my_expert = e; my_key = top; }
+            }
+            float my_bias = 0.0f;
+            if (lane < top_k) {
+                my_logit = logit<L>(row[my_expert]);
+                my_bias = bias ? bias[my_expert] : 0.0f;
+            }
+            // sure of the order: every gap is wide, or the two are equal in logit and bias (the lower expert came first)
+            const float v = unordered(my_key), v_next = __shfl_down_sync(0xffffffffu, v, 1);
+            const float l_next = __shfl_down_sync(0xffffffffu, my_logit, 1), b_next = __shfl_down_sync(0xffffffffu, my_bias, 1);
+            bool gap = v - v_next > near + fabsf(v) * 0x1p-22f || (my_logit == l_next && my_bias == b_next);
+            unsure = !__all_sync(0xffffffffu, lane >= top_k - 1 || gap);
+            const float v_last = __shfl_sync(0xffffffffu, v, top_k - 1), l_last = __shfl_sync(0xffffffffu, my_logit, top_k - 1);
+            const float b_last = __shfl_sync(0xffffffffu, my_bias, top_k - 1);
+            while (!unsure) {                                                  // those behind the last one, while they equal it
+                uint32_t top;
+                const int e = take(top);
+                if (e < 0 || v_last - unordered(top) > near + fabsf(v_last) * 0x1p-22f) break;
+                unsure = !(logit<L>(row[e]) == l_last && (!bias || bias[e] == b_last));
+            }
+        }
+        if (unsure) {
+            my_expert = route_exact<VPL, L, SOFTMAX>(row, bias, E, top_k, form.n_groups, form.top_groups);
+            if (lane < top_k) my_logit = logit<L>(row[my_expert]);
+        }
         float score = 0.0f;
-        if (lane < top_k) {
-            const float v = logit<L>(row[my_expert]);
-            score = SOFTMAX ? __fdiv_rn(expf(v - m), sum) : __fdiv_rn(1.0f, 1.0f + expf(-v));
-        }
+        if (lane < top_k) score = SOFTMAX ? __fdiv_rn(expf(my_logit - m), sum) : __fdiv_rn(1.0f, 1.0f + expf(-my_logit));
         const float total = warp_sum(score) + 1e-9f;
         if (lane < top_k) {
             top_experts[(int64_t)t * top_k + lane] = my_expert;
@@ -527,9 +680,11 @@ static void launch_topk(const L* logits, const float* bias, int T, int E, int to
 template <typename L>
 static void launch_form(const L* logits, const float* bias, int T, int E, int top_k, const RouteForm& form, bool softmax, int per, int n_ctas,
                         int* top_experts, float* top_gates, int* hist, cudaStream_t st) {
+    const bool aligned = (reinterpret_cast<uintptr_t>(logits) & 15) == 0;
 #define CINN_CALL(V) \
-    if (softmax) launch_dependent(route_form_kernel<V, L, true>, dim3(n_ctas), dim3(256), 0, st, logits, bias, T, E, top_k, form, per, top_experts, top_gates, hist); \
-    else launch_dependent(route_form_kernel<V, L, false>, dim3(n_ctas), dim3(256), 0, st, logits, bias, T, E, top_k, form, per, top_experts, top_gates, hist)
+    const int vec = aligned && E % V == 0; \
+    if (softmax) launch_dependent(route_form_kernel<V, L, true>, dim3(n_ctas), dim3(256), 0, st, logits, bias, T, E, top_k, form, per, vec, top_experts, top_gates, hist); \
+    else launch_dependent(route_form_kernel<V, L, false>, dim3(n_ctas), dim3(256), 0, st, logits, bias, T, E, top_k, form, per, vec, top_experts, top_gates, hist)
     CINN_FORM_VPL(CINN_CALL);
 #undef CINN_CALL
 }
