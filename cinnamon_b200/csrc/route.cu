@@ -125,12 +125,10 @@ route_topk_kernel(const L* __restrict__ logits, const float* __restrict__ bias, 
 //   their two best, then the k best experts in them, ties to the lower id;  gate = scale * s / (sum of the k s + 1e-9), or scale * s
 //
 // Which expert is the last to be chosen can hang on the last bit of a score, so the choice is the one that 64-bit arithmetic makes.
-// Hardly any token needs it: a warp chooses with scores that are off by 2^-20 at most and looks at the gaps between those it
-// chose and to the next one; where one is too small to be sure of (and not a tie of the same logit and bias), the token is chosen
-// again in 64 bits.  Gates come from the chosen experts' logits in fp32.
-//
-// A lane holds VPL neighbouring experts and the largest of their keys (floats as ordered integers); a round is one warp-wide maximum,
-// one vote and a look through the winner's keys.
+// Hardly any token needs it: a warp chooses with quick scores and looks at the gaps between those it chose and to the next ones; where one
+// is too small to be sure of (and not a tie of the same logit and bias), those that can be meant are ranked in 64 bits, a lane
+// each.  Where it is a group that is in doubt, a softmax with a bias, or a NaN, the whole token is (route_exact).  Gates come
+// from the chosen experts' logits in fp32.
 // ---------------------------------------------------------------------------
 struct RouteForm {
     int n_groups, top_groups, renormalise;
@@ -166,84 +164,103 @@ __device__ __forceinline__ unsigned best_groups(F score, int n_groups, int top_g
     return __ballot_sync(0xffffffffu, lane < n_groups && rank < top_groups);
 }
 
-// One token in 64 bits; returns lane r's expert (r < top_k).
+__device__ __forceinline__ uint64_t ordered(double v) {
+    const uint64_t b = (uint64_t)__double_as_longlong(v);
+    return b >> 63 ? ~b : b | 0x8000000000000000ull;
+}
+__device__ __forceinline__ double unordered(uint64_t k) { return __longlong_as_double((long long)(k >> 63 ? k & 0x7fffffffffffffffull : ~k)); }
+__device__ __forceinline__ uint64_t reduce_max(uint64_t k) {
+    const uint32_t hi = __reduce_max_sync(0xffffffffu, (uint32_t)(k >> 32));
+    return (uint64_t)hi << 32 | __reduce_max_sync(0xffffffffu, (uint32_t)(k >> 32) == hi ? (uint32_t)k : 0u);
+}
+
+// One token in 64 bits, all of it; returns lane r's expert (r < top_k).
 template <int VPL, typename L, bool SOFTMAX>
 __device__ __noinline__ int route_exact(const L* __restrict__ row, const float* __restrict__ bias, int E, int top_k, int n_groups, int top_groups) {
     const int lane = threadIdx.x & 31, e0 = lane * VPL;
-    float x[VPL];
+    uint64_t key[VPL];                                       // score + bias, ordered; 0: not to be chosen
+    {
+        float x[VPL];
+        double sel[VPL], m = 0.0, sum = 1.0;
 #pragma unroll
-    for (int i = 0; i < VPL; ++i) x[i] = e0 + i < E ? logit<L>(row[e0 + i]) : -INFINITY;
-    double sel[VPL];
-    if constexpr (SOFTMAX) {
-        float m = -INFINITY;
+        for (int i = 0; i < VPL; ++i) x[i] = e0 + i < E ? logit<L>(row[e0 + i]) : -INFINITY;
+        if constexpr (SOFTMAX) {
+            float top = x[0];
 #pragma unroll
-        for (int i = 0; i < VPL; ++i)
-            if (e0 + i < E) m = fmaxf(m, x[i]);
-        m = warp_max(m);
-        double sum = 0.0;
+            for (int i = 1; i < VPL; ++i) top = fmaxf(top, x[i]);
+            m = (double)warp_max(top);
+            sum = 0.0;
+        }
 #pragma unroll
         for (int i = 0; i < VPL; ++i) {
-            sel[i] = e0 + i < E ? exp((double)x[i] - (double)m) : 0.0;
-            sum += sel[i];
+            sel[i] = exp(SOFTMAX ? (double)x[i] - m : -(double)x[i]);
+            if (SOFTMAX && e0 + i < E) sum += sel[i];
         }
-        sum = warp_sum(sum);
+        if constexpr (SOFTMAX) sum = warp_sum(sum);
 #pragma unroll
-        for (int i = 0; i < VPL; ++i) sel[i] /= sum;
-    } else {
-#pragma unroll
-        for (int i = 0; i < VPL; ++i) sel[i] = 1.0 / (1.0 + exp(-(double)x[i]));
-    }
-    unsigned open = 0;                                       // experts that can be chosen
-#pragma unroll
-    for (int i = 0; i < VPL; ++i) {
-        if (e0 + i < E) {
-            if (bias) sel[i] += (double)bias[e0 + i];
-            if (sel[i] != sel[i]) sel[i] = -INFINITY;       // a NaN comes last
-            open |= 1u << i;
+        for (int i = 0; i < VPL; ++i) {
+            sel[i] = SOFTMAX ? sel[i] / sum : 1.0 / (1.0 + sel[i]);
+            if (bias && e0 + i < E) sel[i] += (double)bias[e0 + i];
+            key[i] = e0 + i < E ? ordered(sel[i] == sel[i] ? sel[i] : (double)-INFINITY) : 0ull;        // a NaN comes last
         }
     }
     if (n_groups > 1) {
         const int per = E / n_groups;
         double mine = -INFINITY;
         for (int g = 0; g < n_groups; ++g) {
-            double a = -INFINITY, b = -INFINITY;             // the group's two best
+            uint64_t a = 0, c = 0;                           // the group's two best
 #pragma unroll
-            for (int i = 0; i < VPL; ++i)
-                if ((open >> i & 1) && (e0 + i) / per == g) {
-                    if (sel[i] > a) { b = a; a = sel[i]; }
-                    else if (sel[i] > b) b = sel[i];
-                }
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1) {
-                const double oa = __shfl_xor_sync(0xffffffffu, a, o), ob = __shfl_xor_sync(0xffffffffu, b, o);
-                b = oa > a ? fmax(a, ob) : fmax(b, oa);
-                a = fmax(a, oa);
+            for (int i = 0; i < VPL; ++i) {
+                const uint64_t k = e0 + i >= g * per && e0 + i < (g + 1) * per ? key[i] : 0ull;
+                c = max(c, min(a, k));
+                a = max(a, k);
             }
-            if (lane == g) mine = per > 1 ? a + b : a;
+            const uint64_t top = reduce_max(a);
+            const int owner = __ffs(__ballot_sync(0xffffffffu, a == top)) - 1;
+            const uint64_t next = reduce_max(lane == owner ? c : a);
+            if (lane == g) mine = per > 1 ? unordered(top) + unordered(next) : unordered(top);
         }
         if (mine != mine) mine = -INFINITY;                  // (infinities of both signs)
         const unsigned groups = best_groups(mine, n_groups, top_groups, lane);
 #pragma unroll
         for (int i = 0; i < VPL; ++i)
-            if (e0 + i < E && !(groups >> ((e0 + i) / per) & 1)) open &= ~(1u << i);
+            if (e0 + i < E && !(groups >> ((unsigned)(e0 + i) / (unsigned)per) & 1)) key[i] = 0ull;
     }
     int my_expert = 0;
     for (int r = 0; r < top_k; ++r) {
-        double best = 0.0;
-        int best_e = 0x7fffffff;
+        uint64_t best = 0;
+        int at = 0;
 #pragma unroll
-        for (int i = VPL - 1; i >= 0; --i)
-            if ((open >> i & 1) && (best_e == 0x7fffffff || sel[i] >= best)) { best = sel[i]; best_e = e0 + i; }
+        for (int i = 0; i < VPL; ++i)
+            if (key[i] > best) { best = key[i]; at = i; }
+        const uint64_t top = reduce_max(best);
+        const int w = __ffs(__ballot_sync(0xffffffffu, best == top)) - 1, e = w * VPL + __shfl_sync(0xffffffffu, at, w);
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) {
-            const double ov = __shfl_xor_sync(0xffffffffu, best, o);
-            const int oe = __shfl_xor_sync(0xffffffffu, best_e, o);
-            if (oe != 0x7fffffff && (best_e == 0x7fffffff || ov > best || (ov == best && oe < best_e))) { best = ov; best_e = oe; }
-        }
-        if (best_e / VPL == lane) open &= ~(1u << (best_e - e0));
-        if (lane == r) my_expert = best_e;
+        for (int i = 0; i < VPL; ++i)
+            if (lane == w && i == at) key[i] = 0ull;
+        if (lane == r) my_expert = e;
     }
     return my_expert;
+}
+
+// The same for a list that is known to hold the best: lane r < n has an expert, its logit and bias; afterwards lane r has the expert of
+// rank r.  Scores of a softmax without a bias are compared before their common quotient.
+template <bool SOFTMAX>
+__device__ __noinline__ int rank_exact(int expert, float x, float bias, float m, int n) {
+    const int lane = threadIdx.x & 31;
+    const double e = exp(SOFTMAX ? (double)x - (double)m : -(double)x), mine = SOFTMAX ? e : 1.0 / (1.0 + e) + (double)bias;
+    int rank = 0;
+    for (int j = 0; j < n; ++j) {
+        const double o = __shfl_sync(0xffffffffu, mine, j);
+        const int oe = __shfl_sync(0xffffffffu, expert, j);
+        rank += o > mine || (o == mine && oe < expert);
+    }
+    int out = 0;
+    for (int j = 0; j < n; ++j) {
+        const int r = __shfl_sync(0xffffffffu, rank, j), oe = __shfl_sync(0xffffffffu, expert, j);
+        if (r == lane) out = oe;
+    }
+    return out;
 }
 
 __device__ __forceinline__ float exp2_approx(float x) {          // relative error 2^-22
@@ -280,12 +297,35 @@ __device__ __forceinline__ void load_logits(const L* __restrict__ row, int e0, i
     }
 }
 
+// VPL keys in falling order (odd-even merges)
+template <int VPL>
+__device__ __forceinline__ void sort_keys(uint32_t (&k)[VPL]) {
+#pragma unroll
+    for (int p = 1; p < VPL; p *= 2)
+#pragma unroll
+        for (int q = p; q >= 1; q /= 2)
+#pragma unroll
+            for (int j = q % p; j + q < VPL; j += 2 * q)
+#pragma unroll
+                for (int i = 0; i < q; ++i)
+                    if (j + i + q < VPL && (j + i) / (2 * p) == (j + i + q) / (2 * p)) {
+                        const uint32_t hi = max(k[j + i], k[j + i + q]), lo = min(k[j + i], k[j + i + q]);
+                        k[j + i] = hi;
+                        k[j + i + q] = lo;
+                    }
+}
+
+// A lane holds VPL neighbouring experts as keys: score + bias as an ordered integer whose last bits are the expert's number in the lane (the
+// lower one larger), sorted.  A round is the largest key without those bits among the warp's, and the lowest expert that has it: two
+// warp-wide reductions and a shift of the winner's keys.  (Unsorted, with a vote and a look through the winner's keys: 1280
+// instructions a token for 8 of 256 experts, 83 us for 32768 tokens.)
+//
 // Errors of the quick scores.  Sigmoid: the exponent's rounding is |x| 2^-24 of e^-x, its part in the score s (1 - s) |x| 2^-24 < 2^-26, and
 // ex2, the sum and rcp add less than 2^-22: two scores are sure to be in order when they are 2^-20 apart (and 2^-22 of themselves, for
-// the bias's sum).  Softmax: p |x - max| 2^-24 is below 2^-25 of the largest p, ex2, the sum and the quotient are 2^-21 of p: 2^-19 of
-// the largest p.  A group's sum of two: twice as much.
+// the bias's sum, and what the key's last bits hide).  Softmax: p |x - max| 2^-24 is below 2^-25 of the largest p, ex2, the sum and the
+// quotient are 2^-21 of p: 2^-19 of the largest p.  A group's sum of two: twice as much.
 template <int VPL, typename L, bool SOFTMAX>                 // E <= 32 * VPL
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(256, VPL <= 8 ? 5 : 2)
 route_form_kernel(const L* __restrict__ logits, const float* __restrict__ bias, int T, int E, int top_k, const RouteForm form, int tokens_per_cta, int vec,
                   int* __restrict__ top_experts, float* __restrict__ top_gates, int* __restrict__ hist) {
     pdl_wait();
@@ -293,17 +333,26 @@ route_form_kernel(const L* __restrict__ logits, const float* __restrict__ bias, 
     __shared__ int s_hist[ROUTE_MAX_EXPERTS];
     for (int e = threadIdx.x; e < E; e += 256) s_hist[e] = 0;
     __syncthreads();
+    constexpr int BITS = VPL == 1 ? 0 : VPL == 2 ? 1 : VPL == 4 ? 2 : VPL == 8 ? 3 : VPL == 16 ? 4 : 5;
+    constexpr uint32_t INDEX = VPL - 1;
+    constexpr float HIDDEN = (float)(2 * VPL + 2) * 0x1p-23f;                  // of a score + bias: its rounding and what the last bits hide
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, e0 = lane * VPL;
     const int t_end = min((int)(blockIdx.x + 1) * tokens_per_cta, T);
     const int per = E / form.n_groups, lanes_per = per / VPL;                  // a group's experts; its lanes, where they are whole
-    const bool whole = form.n_groups > 1 && per % VPL == 0 && (lanes_per & (lanes_per - 1)) == 0;
+    const bool whole = per % VPL == 0 && (lanes_per & (lanes_per - 1)) == 0;
     float b[VPL];
 #pragma unroll
     for (int i = 0; i < VPL; ++i) b[i] = bias && e0 + i < E ? bias[e0 + i] : 0.0f;
+    float bias_most = 0.0f;                                                    // what can cancel in a group's sum: not the biases that ban experts
+    if (form.n_groups > 1) {
+#pragma unroll
+        for (int i = 0; i < VPL; ++i) bias_most = fmaxf(bias_most, b[i] > -1e30f ? fabsf(b[i]) : 0.0f);
+        bias_most = warp_max(bias_most);
+    }
     for (int t = blockIdx.x * tokens_per_cta + warp; t < t_end; t += 8) {
         const L* row = logits + (int64_t)t * E;
         float m = 0.0f, sum = 1.0f, near;
-        uint32_t key[VPL];                                                     // score + bias, ordered; 0: not to be chosen
+        uint32_t key[VPL];                                                     // 0: not to be chosen
         bool unsure = false;
         {
             float x[VPL];
@@ -332,16 +381,15 @@ route_form_kernel(const L* __restrict__ logits, const float* __restrict__ bias, 
 #pragma unroll
             for (int i = 0; i < VPL; ++i) {
                 unsure |= x[i] != x[i];
-                key[i] = e0 + i < E ? ordered(x[i]) : 0u;
+                key[i] = e0 + i < E ? (ordered(x[i]) & ~INDEX) | (INDEX - i) : 0u;
             }
         }
         unsure = __any_sync(0xffffffffu, unsure);
+        if (whole) sort_keys<VPL>(key);
         if (form.n_groups > 1 && !unsure) {
             float mine = -INFINITY;                                            // lane g: group g's score
             if (whole) {
-                uint32_t a = key[0], c = 0;                                    // the lane's two best, then the group's
-#pragma unroll
-                for (int i = 1; i < VPL; ++i) { c = max(c, min(a, key[i])); a = max(a, key[i]); }
+                uint32_t a = key[0] & ~INDEX, c = VPL > 1 ? key[VPL > 1] & ~INDEX : 0u;        // the lane's two best, then the group's
                 for (int o = 1; o < lanes_per; o <<= 1) {
                     const uint32_t oa = __shfl_xor_sync(0xffffffffu, a, o), oc = __shfl_xor_sync(0xffffffffu, c, o);
                     c = max(min(a, oa), max(c, oc));
@@ -362,7 +410,7 @@ route_form_kernel(const L* __restrict__ logits, const float* __restrict__ bias, 
                     const uint32_t top = __reduce_max_sync(0xffffffffu, a);
                     const int owner = __ffs(__ballot_sync(0xffffffffu, a == top)) - 1;
                     const uint32_t next = __reduce_max_sync(0xffffffffu, lane == owner ? c : a);
-                    if (lane == g) mine = per > 1 ? unordered(top) + unordered(next) : unordered(top);
+                    if (lane == g) mine = per > 1 ? unordered(top & ~INDEX) + unordered(next & ~INDEX) : unordered(top & ~INDEX);
                 }
             }
             unsure = __any_sync(0xffffffffu, mine != mine);
@@ -370,57 +418,66 @@ route_form_kernel(const L* __restrict__ logits, const float* __restrict__ bias, 
             const bool in = groups >> lane & 1;
             const float worst = unordered(__reduce_min_sync(0xffffffffu, in ? ordered(mine) : 0xffffffffu));
             const float next = unordered(__reduce_max_sync(0xffffffffu, in || lane >= form.n_groups ? ordered(-INFINITY) : ordered(mine)));
-            if (form.top_groups < form.n_groups && !(worst - next > 2.0f * near + fabsf(worst) * 0x1p-21f)) unsure = true;
+            // (a sum's two scores + biases may cancel: what is hidden of them goes by the largest bias)
+            const float hidden = (4.0f + 4.0f * bias_most + 2.0f * fabsf(worst) + (next > -INFINITY ? 2.0f * fabsf(next) : 0.0f)) * HIDDEN;
+            if (form.top_groups < form.n_groups && !(worst - next > 2.0f * near + hidden)) unsure = true;
+            if (whole) {
+                const bool open = groups >> ((unsigned)lane / (unsigned)lanes_per & 31u) & 1;
 #pragma unroll
-            for (int i = 0; i < VPL; ++i)
-                if (e0 + i < E && !(groups >> ((unsigned)(e0 + i) / (unsigned)per) & 1)) key[i] = 0u;
+                for (int i = 0; i < VPL; ++i) key[i] = open ? key[i] : 0u;
+            } else {
+#pragma unroll
+                for (int i = 0; i < VPL; ++i)
+                    if (e0 + i < E && !(groups >> ((unsigned)(e0 + i) / (unsigned)per) & 1)) key[i] = 0u;
+            }
         }
+        if (!whole) sort_keys<VPL>(key);
         int my_expert = 0;
         float my_logit = 0.0f;
         if (!unsure) {
-            uint32_t best = 0, my_key = 0;
-            int at = 0;
-            auto look = [&]() {
-                best = 0;
+            uint32_t my_key = 0;
+            auto take = [&](uint32_t& top) {                                   // the best expert left, out of the list; top 0: there is none
+                const uint32_t head = key[0] & ~INDEX;
+                top = __reduce_max_sync(0xffffffffu, head);
+                const int e = (int)__reduce_min_sync(0xffffffffu, head == top ? (unsigned)(e0 + (int)(INDEX - (key[0] & INDEX))) : 0xffffffffu);
+                const bool won = e >> BITS == lane;
 #pragma unroll
-                for (int i = 0; i < VPL; ++i)
-                    if (key[i] > best) { best = key[i]; at = i; }
+                for (int i = 0; i + 1 < VPL; ++i) key[i] = won ? key[i + 1] : key[i];
+                key[VPL - 1] = won ? 0u : key[VPL - 1];
+                return e;
             };
-            auto take = [&](uint32_t& top) {                                   // the best expert left, out of the list; -1: there is none
-                top = __reduce_max_sync(0xffffffffu, best);
-                const int w = __ffs(__ballot_sync(0xffffffffu, best == top)) - 1;
-                const int e = w * VPL + __shfl_sync(0xffffffffu, at, w);
-                if (lane == w) {
-#pragma unroll
-                    for (int i = 0; i < VPL; ++i)
-                        if (i == at) key[i] = 0u;
-                    look();
-                }
-                return top ? e : -1;
-            };
-            look();
             for (int r = 0; r < top_k; ++r) {
                 uint32_t top;
                 const int e = take(top);
                 if (lane == r) { my_expert = e; my_key = top; }
             }
+            // ... and those behind the last one that are as good as it, as far as these scores can tell
+            const float v_last = unordered(__shfl_sync(0xffffffffu, my_key, top_k - 1));
+            int n = top_k;
+            for (; n < 32; ++n) {
+                uint32_t top;
+                const int e = take(top);
+                if (top == 0u || v_last - unordered(top) > near + fabsf(v_last) * HIDDEN) break;
+                if (lane == n) { my_expert = e; my_key = top; }
+            }
             float my_bias = 0.0f;
-            if (lane < top_k) {
+            if (lane < n) {
                 my_logit = logit<L>(row[my_expert]);
                 my_bias = bias ? bias[my_expert] : 0.0f;
             }
             // sure of the order: every gap is wide, or the two are equal in logit and bias (the lower expert came first)
             const float v = unordered(my_key), v_next = __shfl_down_sync(0xffffffffu, v, 1);
             const float l_next = __shfl_down_sync(0xffffffffu, my_logit, 1), b_next = __shfl_down_sync(0xffffffffu, my_bias, 1);
-            bool gap = v - v_next > near + fabsf(v) * 0x1p-22f || (my_logit == l_next && my_bias == b_next);
-            unsure = !__all_sync(0xffffffffu, lane >= top_k - 1 || gap);
-            const float v_last = __shfl_sync(0xffffffffu, v, top_k - 1), l_last = __shfl_sync(0xffffffffu, my_logit, top_k - 1);
-            const float b_last = __shfl_sync(0xffffffffu, my_bias, top_k - 1);
-            while (!unsure) {                                                  // those behind the last one, while they equal it
-                uint32_t top;
-                const int e = take(top);
-                if (e < 0 || v_last - unordered(top) > near + fabsf(v_last) * 0x1p-22f) break;
-                unsure = !(logit<L>(row[e]) == l_last && (!bias || bias[e] == b_last));
+            const bool same = my_logit == l_next && my_bias == b_next, gap = v - v_next > near + fabsf(v) * HIDDEN;
+            if (n == 32 && top_k < E) {
+                unsure = true;                                                 // (more of them than lanes)
+            } else if (!__all_sync(0xffffffffu, lane >= n - 1 || gap || same)) {
+                if (SOFTMAX && bias) {
+                    unsure = true;
+                } else {
+                    my_expert = rank_exact<SOFTMAX>(my_expert, my_logit, my_bias, m, n);
+                    if (lane < top_k) my_logit = logit<L>(row[my_expert]);
+                }
             }
         }
         if (unsure) {
@@ -558,8 +615,10 @@ route_scatter_kernel(const int* __restrict__ top_experts, const float* __restric
     pdl_wait();
     pdl_trigger();
     __shared__ int s_next[ROUTE_MAX_EXPERTS];                                  // next free row of every expert
+    __shared__ unsigned long long s_warps[ROUTE_MAX_EXPERTS];                  // of 256 pairs: how many of each warp are the expert's, a byte each
     __shared__ int s_warp[8];
     __shared__ int s_pos[ROUTE_MAX_TOKENS_PER_CTA * ROUTE_MAX_TOPK];
+    for (int e = threadIdx.x; e < E; e += 256) s_warps[e] = 0ull;
     {
         // thread i: experts 4 i .. 4 i + 3; their counts, the rows of earlier CTAs, and a scan of the counts
         int cnt[4], mine[4], sum = 0;
@@ -611,47 +670,40 @@ route_scatter_kernel(const int* __restrict__ top_experts, const float* __restric
     const int n_tok = min(tokens_per_cta, T - t_begin);
     const int n_pairs = n_tok * top_k;
     const int64_t pair0 = (int64_t)t_begin * top_k;
+    // A pair's row: the expert's next free one, behind those of lower warps and lower lanes that are the same expert's.  (Warp after warp, with a
+    // barrier between them: eight turns instead of three barriers.)
     for (int base = 0; base < n_pairs; base += 256) {
         const int p = base + threadIdx.x;
         const bool live = p < n_pairs;
         const int e = live ? top_experts[pair0 + p] : -1 - lane;              // dead lanes match nobody
-        const int turns = min(8, (n_pairs - base + 31) / 32);
-        for (int w = 0; w < turns; ++w) {                                      // warps take their turn: (token, slot) order
-            if (warp == w) {
-                const unsigned peers = __match_any_sync(0xffffffffu, e);
-                const int leader = __ffs(peers) - 1;
-                int row = 0;
-                if (live && lane == leader) {
-                    row = s_next[e];
-                    s_next[e] = row + __popc(peers);
-                }
-                row = __shfl_sync(0xffffffffu, row, leader) + __popc(peers & ((1u << lane) - 1u));
-                if (live) {
-                    s_pos[p] = row;
-                    token_indices[row] = t_begin + p / top_k;
-                    sorted_scores[row] = top_gates[pair0 + p];
-                    sorted_experts[row] = e;
-                }
-            }
-            __syncthreads();
+        const unsigned peers = __match_any_sync(0xffffffffu, e);
+        const bool leads = live && lane == __ffs(peers) - 1;
+        if (leads) atomicAdd(&s_warps[e], (unsigned long long)__popc(peers) << (8 * warp));
+        __syncthreads();
+        int row = 0, all = 0;
+        bool first = false;
+        if (live) {
+            const unsigned long long counts_of = s_warps[e], lower = counts_of & ((1ull << (8 * warp)) - 1ull);
+            const auto bytes = [](unsigned long long v) { return __dp4a((unsigned)v, 0x01010101u, __dp4a((unsigned)(v >> 32), 0x01010101u, 0u)); };
+            row = s_next[e] + (int)bytes(lower) + __popc(peers & ((1u << lane) - 1u));
+            all = (int)bytes(counts_of);
+            first = leads && lower == 0ull;
+            s_pos[p] = row;
+            token_indices[row] = t_begin + p / top_k;
+            sorted_scores[row] = top_gates[pair0 + p];
+            sorted_experts[row] = e;
         }
+        __syncthreads();
+        if (first) { s_next[e] += all; s_warps[e] = 0ull; }
+        __syncthreads();
     }
-    // per token: its rows in ascending order, gates alongside (insertion sort, k <= 32)
-    for (int tl = threadIdx.x; tl < n_tok; tl += 256) {
-        int pos[ROUTE_MAX_TOPK];
-        float gate[ROUTE_MAX_TOPK];
-        for (int j = 0; j < top_k; ++j) {
-            const int v = s_pos[tl * top_k + j];
-            const float g = top_gates[pair0 + tl * top_k + j];
-            int i = j;
-            while (i > 0 && pos[i - 1] > v) { pos[i] = pos[i - 1]; gate[i] = gate[i - 1]; --i; }
-            pos[i] = v;
-            gate[i] = g;
-        }
-        for (int j = 0; j < top_k; ++j) {
-            pair_pos[(int64_t)(t_begin + tl) * top_k + j] = pos[j];
-            pair_gate[(int64_t)(t_begin + tl) * top_k + j] = gate[j];
-        }
+    // per token: its rows in ascending order, gates alongside; a pair's place is how many of its token's rows come before its own
+    for (int p = threadIdx.x; p < n_pairs; p += 256) {
+        const int tl = p / top_k, mine = s_pos[p];
+        int place = 0;
+        for (int j = 0; j < top_k; ++j) place += s_pos[tl * top_k + j] < mine;
+        pair_pos[pair0 + tl * top_k + place] = mine;
+        pair_gate[pair0 + tl * top_k + place] = top_gates[pair0 + p];
     }
 }
 

@@ -157,6 +157,24 @@ def test_nan_infinities_and_banned_experts(n_groups, top_groups):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("low", [float("-inf"), torch.finfo(torch.float32).min, -1e31])
+def test_groups_whose_experts_are_banned(low):
+    """Masks of the lowest values: in some groups one expert is left, in some none; biases that cancel in a group's sum."""
+    from cinnamon_b200 import kernels as K
+    T, E = 300, 64
+    g = torch.Generator().manual_seed(8)
+    logits = torch.randn(T, E, generator=g)
+    bias = torch.randn(E, generator=g) * 0.1
+    bias[0:8], bias[9:16], bias[24:31] = low, low, low
+    for k, top_groups in ((4, 2), (20, 3), (33 - 1, 4)):
+        r = K.moe_route(logits.cuda(), bias.cuda(), k, n_groups=8, top_groups=top_groups, scale=2.0)
+        assert torch.equal(r["top_experts"].cpu(), _choose(logits, bias, k, "sigmoid", 8, top_groups)[1].int())
+    bias = torch.where(torch.arange(E) % 8 == 0, 4096.0, torch.where(torch.arange(E) % 8 == 1, -4095.0, -5000.0))
+    r = K.moe_route(logits.cuda(), bias.cuda(), 4, n_groups=8, top_groups=3, scale=2.0)
+    assert torch.equal(r["top_experts"].cpu(), _choose(logits, bias, 4, "sigmoid", 8, 3)[1].int())
+
+
+@pytest.mark.gpu
 def test_the_references_form_keeps_its_bits_and_gains_a_gradient():
     from cinnamon_b200 import kernels as K
     g = torch.Generator().manual_seed(1)
