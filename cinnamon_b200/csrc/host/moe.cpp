@@ -152,7 +152,7 @@ struct RouteNode : public torch::autograd::Function<RouteNode> {
         ctx->saved_data["scale"] = c->form.scale;
         ctx->set_materialize_grads(false);
         const int64_t T = logits.size(0);
-        return {top.view({T, c->top_k}), r.floats.narrow(0, r.pairs, r.pairs).view({T, c->top_k}), r.floats.narrow(0, 0, r.pairs)};
+        return {part_of(top, 0, {T, c->top_k}), part_of(r.floats, r.pairs, {T, c->top_k}), part_of(r.floats, 0, {r.pairs})};
     }
     static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
         const auto s = ctx->get_saved_variables();
@@ -198,21 +198,21 @@ void bind_moe(pybind11::module_& m) {
             top = v[0]; pair = v[1]; sorted = v[2];
         } else {
             c.out = route(logits, c.bias, top_k, c.form, &top);
-            top = top.view({T, top_k});
-            pair = c.out.floats.narrow(0, pairs, pairs).view({T, top_k});
-            sorted = c.out.floats.narrow(0, 0, pairs);
+            top = part_of(top, 0, {T, top_k});
+            pair = part_of(c.out.floats, pairs, {T, top_k});
+            sorted = part_of(c.out.floats, 0, {pairs});
         }
         const Routes& r = c.out;
         pybind11::dict out;
-        out["top_experts"] = r.top.view({T, top_k});
+        out["top_experts"] = part_of(r.top, 0, {T, top_k});
         out["top_gates"] = top;
-        out["token_indices"] = r.longs.narrow(0, 0, pairs);
+        out["token_indices"] = part_of(r.longs, 0, {pairs});
         out["sorted_scores"] = sorted;
-        out["sorted_experts"] = r.longs.narrow(0, pairs, pairs);
+        out["sorted_experts"] = part_of(r.longs, pairs, {pairs});
         out["counts"] = r.counts();
         out["starts"] = r.starts();
         out["ends"] = r.ends();
-        out["pair_pos"] = r.longs.narrow(0, 2 * pairs, pairs).view({T, top_k});
+        out["pair_pos"] = part_of(r.longs, 2 * pairs, {T, top_k});
         out["pair_gate"] = pair;
         return out;
     });
