@@ -29,7 +29,7 @@ namespace ce {
 
 __device__ int g_status = 0;               // 0, or (role << 8) | reason of a bounded wait that ran out
 
-enum Mode { STATS = 0, SOFT = 1, DX = 2, DW = 3, DW_PART = 4 };
+enum Mode { STATS = 0, SOFT = 1, DX = 2, DW = 3 };
 
 constexpr int M = 256, N = 256;            // the pair's tile
 constexpr int KE = 64;                     // elements of a K block: 128 bytes
@@ -52,9 +52,9 @@ struct Params {
     int T, V, d;
     int v0, vc;                            // the piece: its first word, how many
     int parts;                             // STATS: runs of words per tile of tokens
-    int splits;                            // DX, DW_PART: pieces of the reduction, each with sums of its own
-    int rows_pad;                          // rows of one split's sums
-    int add;                               // DX: add to the sums of earlier pieces
+    int dx_splits, dw_splits;              // pieces that the reductions are cut into, each with sums of its own; 0: not wanted
+    int dx_rows, dw_rows;                  // rows of one such piece's sums
+    int add;                               // dx: add to the sums of earlier pieces
     int per_row;                           // SOFT: gradients per token (reduction "none")
     int64_t part_ld;
     float2* part;                          // STATS: (parts * 2, part_ld) maximum and sum
@@ -165,22 +165,23 @@ struct Unit { int m0, n_first, n_last, kb0, KB, split; };
 // Work of one cluster at a time: a tile (a run of them along the words for STATS).  Groups of GROUP row tiles, rows fastest inside.
 template <int MODE>
 __device__ __forceinline__ int unit_count(const Params& p, int valid) {
-    const int rows = MODE >= DW ? p.vc : valid, cols = MODE == STATS ? p.V : MODE == SOFT ? p.vc : p.d;
+    const int rows = MODE == DW ? p.vc : valid, cols = MODE == STATS ? p.V : MODE == SOFT ? p.vc : p.d;
     const int tiles = ((rows + M - 1) / M) * (MODE == STATS ? p.parts : (cols + N - 1) / N);
-    return (MODE == DX || MODE == DW_PART) ? tiles * p.splits : tiles;
+    return MODE == DX ? tiles * p.dx_splits : MODE == DW ? tiles * p.dw_splits : tiles;
 }
 template <int MODE>
 __device__ __forceinline__ Unit unit_at(const Params& p, int valid, int u) {
-    const int rows = MODE >= DW ? p.vc : valid, cols = MODE == STATS ? p.V : MODE == SOFT ? p.vc : p.d;
+    const int rows = MODE == DW ? p.vc : valid, cols = MODE == STATS ? p.V : MODE == SOFT ? p.vc : p.d;
     const int m_tiles = (rows + M - 1) / M, n_tiles = (cols + N - 1) / N, across = MODE == STATS ? p.parts : n_tiles;
-    const int red = MODE == DX ? p.vc : MODE >= DW ? valid : p.d, blocks = (red + KE - 1) / KE;
+    const int red = MODE == DX ? p.vc : MODE == DW ? valid : p.d, blocks = (red + KE - 1) / KE;
     Unit r;
     r.split = 0; r.kb0 = 0; r.KB = blocks;
-    if constexpr (MODE == DX || MODE == DW_PART) {
+    if constexpr (MODE >= DX) {
+        const int splits = MODE == DX ? p.dx_splits : p.dw_splits;
         r.split = u / (m_tiles * across);
         u -= r.split * (m_tiles * across);
-        r.kb0 = (int)((int64_t)blocks * r.split / p.splits);
-        r.KB = (int)((int64_t)blocks * (r.split + 1) / p.splits) - r.kb0;
+        r.kb0 = (int)((int64_t)blocks * r.split / splits);
+        r.KB = (int)((int64_t)blocks * (r.split + 1) / splits) - r.kb0;
     }
     const int g = u / (GROUP * across), first = g * GROUP, size = min(GROUP, m_tiles - first);
     const int in = u - g * GROUP * across, n = in / size;
@@ -194,48 +195,123 @@ __device__ __forceinline__ Unit unit_at(const Params& p, int valid, int u) {
     return r;
 }
 
-// A: x (STATS, SOFT) or dz (DX: as stored; DW: its transpose, MN-major);  B: W (STATS, SOFT: as stored; DX: MN-major) or x (DW, MN-major).
-// xg: x's rows in use, gathered; read in x's place where some token is ignored.
+// The two gradients' tiles as one list for each cluster: first its share of those with the longer reduction; then, where the last round of
+// these leaves clusters over, the shorter ones that fit beside it; then the rest in turn.  (One kernel for each: 128 x 2 tiles of dx and 32 x 2
+// of dW on 74 pairs end in rounds that are half or nearly empty, 219 + 198 us of which 163 + 163 are products at the STATS kernel's rate.)
+struct Schedule {
+    int n_long, n_short, clusters, cluster, rem, pre, fit;
+    bool dx_long;
+    __device__ Schedule(const Params& p, int valid, int cluster_, int clusters_) : clusters(clusters_), cluster(cluster_) {
+        const int n_dx = unit_count<DX>(p, valid), n_dw = unit_count<DW>(p, valid);
+        const int l_dx = p.dx_splits ? ((p.vc + KE - 1) / KE + p.dx_splits - 1) / p.dx_splits : 0;
+        const int l_dw = p.dw_splits ? ((valid + KE - 1) / KE + p.dw_splits - 1) / p.dw_splits : 0;
+        dx_long = l_dx >= l_dw;
+        n_long = dx_long ? n_dx : n_dw;
+        n_short = dx_long ? n_dw : n_dx;
+        const int l_long = max(l_dx, l_dw), l_short = max(1, min(l_dx, l_dw));
+        rem = n_long % clusters;
+        fit = rem ? l_long / l_short : 0;
+        pre = rem ? (int)min((int64_t)n_short, (int64_t)(clusters - rem) * fit) : 0;
+    }
+    // this cluster's i-th tile: its number among dx's or dW's; false: there are no more
+    __device__ __forceinline__ bool at(int i, bool& dx, int& u) const {
+        const int longs = n_long > cluster ? (n_long - cluster + clusters - 1) / clusters : 0;
+        if (i < longs) { dx = dx_long; u = cluster + i * clusters; return true; }
+        i -= longs;
+        dx = !dx_long;
+        const int room = clusters - rem;
+        int here = 0;                                       // of the shorter ones beside the last long round
+        if (rem && cluster >= rem && pre > cluster - rem) here = (pre - (cluster - rem) + room - 1) / room;
+        if (i < here) { u = cluster - rem + i * room; return true; }
+        const int64_t v = pre + cluster + (int64_t)(i - here) * clusters;
+        if (v >= n_short) return false;
+        u = (int)v;
+        return true;
+    }
+};
+
+// What every product kernel sets up: barriers, tensor memory, the roles' view of both.
+template <int SMEM_C>
+struct Setup {
+    uint8_t *smem_a, *smem_b, *c_stage;
+    volatile int* abort_flag;
+    uint32_t full0, empty0, tfull0, tempty0, staged, taken, rank, tmem;
+    int warp, lane;
+
+    __device__ __forceinline__ Setup(uint8_t* raw) {
+        uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
+        smem_a = smem;
+        smem_b = smem + STAGES * SIDE;
+        c_stage = smem + STAGE_BYTES;
+        uint64_t* bars = reinterpret_cast<uint64_t*>(c_stage + SMEM_C);
+        // [0, S) full (used in the leader), [S, 2S) empty, then: tensor memory full (2), empty (2, leader), boxes staged, boxes taken
+        uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * STAGES + 6);
+        abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+        warp = threadIdx.x >> 5; lane = threadIdx.x & 31;
+        rank = cta_rank();
+        full0 = smem_u32(bars); empty0 = smem_u32(bars + STAGES);
+        tfull0 = smem_u32(bars + 2 * STAGES); tempty0 = smem_u32(bars + 2 * STAGES + 2);
+        staged = smem_u32(bars + 2 * STAGES + 4); taken = smem_u32(bars + 2 * STAGES + 5);
+        if (threadIdx.x == 0) *abort_flag = 0;
+        if (warp == W_TMA && lane == 0) {
+            for (int s = 0; s < STAGES; ++s) { mbar_init(full0 + 8 * s, 1); mbar_init(empty0 + 8 * s, 1); }
+            for (int b = 0; b < 2; ++b) { mbar_init(tfull0 + 8 * b, 1); mbar_init(tempty0 + 8 * b, 2 * EPI); }
+            mbar_init(staged, EPI);
+            mbar_init(taken, 1);
+            asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        }
+        if (warp == W_MMA) {
+            asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(512) : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+        }
+        pdl_wait();
+        if (warp == W_MMA) pdl_trigger();
+        tc_fence_before();
+        __syncthreads();
+        cluster_sync();
+        tc_fence_after();
+        tmem = *tmem_slot;
+    }
+    // nobody leaves while the other CTA may still read this CTA's shared memory or signal its barriers
+    __device__ __forceinline__ void finish() {
+        tc_fence_before();
+        __syncthreads();
+        cluster_sync();
+        if (warp == W_MMA) {
+            tc_fence_after();
+            asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+        }
+    }
+    // The producer gives up: time for the copies already issued to land (their barrier may be the other CTA's)
+    __device__ __forceinline__ void drain() {
+        const long long t0 = clock64();
+        while (clock64() - t0 < 2000000LL) { }
+    }
+    // by the MMA warp, after its last tile: every MMA issued must have retired before tensor memory is freed
+    __device__ __forceinline__ void retire(uint32_t tiles, bool alive) {
+        if (alive && tiles) wait(tfull0 + 8 * ((tiles - 1) & 1), (tiles - 1) >> 1 & 1, abort_flag, (12 << 8) | 3);
+    }
+};
+
+// 16 bytes of a box's row: 16-byte pieces, 128-byte swizzle
+__device__ __forceinline__ void stage16(uint32_t box, int row, int piece, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(box + row * 128 + ((piece ^ (row & 7)) << 4)), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+__device__ __forceinline__ uint64_t pair2(float a, float b) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+
+// The logits' product: A = x, B = W, both K-major.  STATS leaves maxima and sums of its runs, SOFT dz of the piece.  xg: x's rows in use,
+// gathered; read in x's place where some token is ignored.
 template <int MODE, bool BF16>
 __global__ void __launch_bounds__(THREADS, 1)
 product_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b, const __grid_constant__ CUtensorMap tm_xg,
                const __grid_constant__ CUtensorMap tm_c, const Params p) {
-    constexpr bool A_MN = MODE >= DW, B_MN = MODE >= DX;
     extern __shared__ uint8_t smem_raw[];
-    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-    uint8_t* smem_a = smem;
-    uint8_t* smem_b = smem + STAGES * SIDE;
-    uint8_t* c_stage = smem + STAGE_BYTES;
-    uint64_t* bars = reinterpret_cast<uint64_t*>(c_stage + (MODE == STATS ? 0 : C_BYTES));
-    // [0, S) full (used in the leader), [S, 2S) empty, then: tensor memory full (2), empty (2, leader), boxes staged, boxes taken
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * STAGES + 6);
-    volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const uint32_t rank = cta_rank();
-    const uint32_t full0 = smem_u32(bars), empty0 = smem_u32(bars + STAGES);
-    const uint32_t tfull0 = smem_u32(bars + 2 * STAGES), tempty0 = smem_u32(bars + 2 * STAGES + 2);
-    const uint32_t staged = smem_u32(bars + 2 * STAGES + 4), taken = smem_u32(bars + 2 * STAGES + 5);
-
-    if (threadIdx.x == 0) *abort_flag = 0;
-    if (warp == W_TMA && lane == 0) {
-        for (int s = 0; s < STAGES; ++s) { mbar_init(full0 + 8 * s, 1); mbar_init(empty0 + 8 * s, 1); }
-        for (int b = 0; b < 2; ++b) { mbar_init(tfull0 + 8 * b, 1); mbar_init(tempty0 + 8 * b, 2 * EPI); }
-        mbar_init(staged, EPI);
-        mbar_init(taken, 1);
-        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-    }
-    if (warp == W_MMA) {
-        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(512) : "memory");
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
-    }
-    pdl_wait();
-    if (warp == W_MMA) pdl_trigger();
-    tc_fence_before();
-    __syncthreads();
-    cluster_sync();
-    tc_fence_after();
-    const uint32_t tmem = *tmem_slot;
+    Setup<MODE == STATS ? 0 : C_BYTES> s(smem_raw);
+    const int warp = s.warp, lane = s.lane, rank = (int)s.rank;
     const int valid = *p.n_valid;
     const int n_units = unit_count<MODE>(p, valid);
     const int cluster = blockIdx.x >> 1, n_clusters = gridDim.x >> 1;
@@ -243,148 +319,103 @@ product_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__
     if (warp == W_TMA) {
         // ------------------------------ TMA producer (both CTAs) ------------------------------
         if (lane == 0) {
-            const uint32_t full_leader = mapa(full0, 0);
-            const CUtensorMap* map_a = (MODE <= SOFT && valid != p.T) ? &tm_xg : &tm_a;
-            const CUtensorMap* map_b = (MODE >= DW && valid != p.T) ? &tm_xg : &tm_b;
+            const uint32_t full_leader = mapa(s.full0, 0);
+            const CUtensorMap* map_a = valid != p.T ? &tm_xg : &tm_a;
             uint32_t it = 0;
             bool alive = true;
             for (int u = cluster; u < n_units && alive; u += n_clusters) {
                 const Unit w = unit_at<MODE>(p, valid, u);
                 for (int nt = w.n_first; nt < w.n_last && alive; ++nt) {
-                    const int ma = w.m0 + 128 * (int)rank, nb = nt * N + 128 * (int)rank;
+                    const int ma = w.m0 + 128 * rank, nb = p.v0 + nt * N + 128 * rank;
                     for (int kb = 0; kb < w.KB; ++kb, ++it) {
-                        const int s = it % STAGES;
-                        if (!wait(empty0 + 8 * s, (it / STAGES & 1) ^ 1, abort_flag, (11 << 8) | 1)) { alive = false; break; }
-                        if (rank == 0) mbar_expect_tx(full0 + 8 * s, 4 * SIDE);
-                        const uint32_t bar = full_leader + 8 * s, da = smem_u32(smem_a + s * SIDE), db = smem_u32(smem_b + s * SIDE);
-                        const int k = (w.kb0 + kb) * KE;
-                        if constexpr (!A_MN) {
-                            load_2d(map_a, bar, da, k, ma);
-                        } else {
-                            load_2d(map_a, bar, da, ma, k);
-                            load_2d(map_a, bar, da + SIDE / 2, ma + 64, k);
-                        }
-                        if constexpr (!B_MN) {
-                            load_2d(map_b, bar, db, k, p.v0 + nb);
-                        } else {
-                            const int y = MODE == DX ? p.v0 + k : k;
-                            load_2d(map_b, bar, db, nb, y);
-                            load_2d(map_b, bar, db + SIDE / 2, nb + 64, y);
-                        }
+                        const int st = it % STAGES;
+                        if (!wait(s.empty0 + 8 * st, (it / STAGES & 1) ^ 1, s.abort_flag, (11 << 8) | 1)) { alive = false; break; }
+                        if (rank == 0) mbar_expect_tx(s.full0 + 8 * st, 4 * SIDE);
+                        load_2d(map_a, full_leader + 8 * st, smem_u32(s.smem_a + st * SIDE), kb * KE, ma);
+                        load_2d(&tm_b, full_leader + 8 * st, smem_u32(s.smem_b + st * SIDE), kb * KE, nb);
                     }
                 }
             }
-            if (!alive) {                  // abandoned: time for the copies already issued to land
-                const long long t0 = clock64();
-                while (clock64() - t0 < 2000000LL) { }
-            }
+            if (!alive) s.drain();
         }
     } else if (warp == W_MMA) {
         // ------------------------------ MMA issuer (leader; a whole warp, one elected lane) ------------------------------
         if (rank == 0) {
-            constexpr uint32_t idesc = make_idesc_f16(BF16, M, N, A_MN, B_MN);
-            // K-major: a step of 16 elements is 32 bytes of the row.  MN-major: 16 rows of 128 bytes; the second 64 columns are a panel
-            // of their own, SIDE / 2 bytes on (the leading offset).
-            constexpr uint32_t LEAD = (SIDE / 2) >> 4;
-            const uint32_t a0 = ((smem_u32(smem_a) >> 4) & 0x3FFF) | ((A_MN ? LEAD : 1u) << 16);
-            const uint32_t b0 = ((smem_u32(smem_b) >> 4) & 0x3FFF) | ((B_MN ? LEAD : 1u) << 16);
-            const uint32_t tfull_own = mapa(tfull0, 0), tfull_peer = mapa(tfull0, 1);
-            const uint32_t empty_own = mapa(empty0, 0), empty_peer = mapa(empty0, 1);
+            constexpr uint32_t idesc = make_idesc_f16(BF16, M, N);
+            const uint32_t a0 = panel_desc(smem_u32(s.smem_a)), b0 = panel_desc(smem_u32(s.smem_b));
+            const uint32_t tfull_own = mapa(s.tfull0, 0), tfull_peer = mapa(s.tfull0, 1);
+            const uint32_t empty_own = mapa(s.empty0, 0), empty_peer = mapa(s.empty0, 1);
             uint32_t it = 0, tile = 0;
             bool alive = true;
             for (int u = cluster; u < n_units && alive; u += n_clusters) {
                 const Unit w = unit_at<MODE>(p, valid, u);
                 for (int nt = w.n_first; nt < w.n_last && alive; ++nt, ++tile) {
                     const uint32_t b = tile & 1;
-                    if (!wait_warp(tempty0 + 8 * b, (tile >> 1 & 1) ^ 1, abort_flag, (12 << 8) | 2)) { alive = false; break; }
+                    if (!wait_warp(s.tempty0 + 8 * b, (tile >> 1 & 1) ^ 1, s.abort_flag, (12 << 8) | 2)) { alive = false; break; }
                     tc_fence_after();
                     for (int kb = 0; kb < w.KB; ++kb, ++it) {
-                        const uint32_t s = it % STAGES;
-                        if (!wait_warp(full0 + 8 * s, it / STAGES & 1, abort_flag, (12 << 8) | 1)) { alive = false; break; }
+                        const uint32_t st = it % STAGES;
+                        if (!wait_warp(s.full0 + 8 * st, it / STAGES & 1, s.abort_flag, (12 << 8) | 1)) { alive = false; break; }
                         tc_fence_after();
-                        mma_block<A_MN ? 128 : 2, B_MN ? 128 : 2>(tmem + b * N, a0 + s * (SIDE >> 4), b0 + s * (SIDE >> 4), idesc, kb == 0);
-                        commit_pair(empty_own + 8 * s, empty_peer + 8 * s);
+                        mma_block<2, 2>(s.tmem + b * N, a0 + st * (SIDE >> 4), b0 + st * (SIDE >> 4), idesc, kb == 0);
+                        commit_pair(empty_own + 8 * st, empty_peer + 8 * st);
                     }
                     if (!alive) break;
                     commit_pair(tfull_own + 8 * b, tfull_peer + 8 * b);
                 }
             }
-            // every MMA issued above must have retired before tensor memory is freed
-            if (alive && tile) wait(tfull0 + 8 * ((tile - 1) & 1), (tile - 1) >> 1 & 1, abort_flag, (12 << 8) | 3);
+            s.retire(tile, alive);
         }
     } else if (warp == W_STORE) {
         // ------------------------------ finished boxes to the TMA unit (both CTAs) ------------------------------
-        if constexpr (MODE != STATS) {
-            constexpr bool F32 = MODE == DX || MODE == DW_PART;
-            constexpr int PER = F32 ? 32 : 64, ROUNDS = COLS / (2 * PER);        // elements of a box's row; rounds of a tile
+        if constexpr (MODE == SOFT) {
             const int w = lane >> 1, q = w & 3, h = w >> 2;
-            const int out_cols = MODE == SOFT ? p.vc : p.d;
             uint32_t round = 0;
-            bool alive = true;
-            for (int u = cluster; u < n_units && alive; u += n_clusters) {
+            for (int u = cluster; u < n_units; u += n_clusters, ++round) {
                 const Unit t = unit_at<MODE>(p, valid, u);
-                const int row = t.m0 + 128 * (int)rank + q * 32;
-                for (int r = 0; r < ROUNDS; ++r, ++round) {
-                    const int col = t.n_first * N + h * COLS + (r * 2 + (lane & 1)) * PER;
-                    if (!wait_warp(staged, round & 1, abort_flag, (14 << 8) | 1)) { alive = false; break; }
-                    if (lane < 2 * EPI) {
-                        const uint32_t box = smem_u32(c_stage) + lane * BOX;
-                        if (col < out_cols && (MODE != DW || p.v0 + row < p.V)) {
-                            if constexpr (F32) {
-                                if (p.add) add_2d(&tm_c, box, col, t.split * p.rows_pad + row);
-                                else tma_store_2d(&tm_c, box, col, t.split * p.rows_pad + row);
-                            } else {
-                                tma_store_2d(&tm_c, box, col, (MODE == DW ? p.v0 : 0) + row);
-                            }
-                        }
-                        tma_store_commit();
-                        tma_store_wait_read();
-                    }
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(taken);
+                const int row = t.m0 + 128 * rank + q * 32, col = t.n_first * N + h * COLS + (lane & 1) * 64;
+                if (!wait_warp(s.staged, round & 1, s.abort_flag, (14 << 8) | 1)) break;
+                if (lane < 2 * EPI) {
+                    if (col < p.vc) tma_store_2d(&tm_c, smem_u32(s.c_stage) + lane * BOX, col, row);
+                    tma_store_commit();
+                    tma_store_wait_read();
                 }
+                __syncwarp();
+                if (lane == 0) mbar_arrive(s.taken);
             }
             if (lane < 2 * EPI) tma_store_wait_all();
         }
     } else {
         // ------------------------------ epilogue (both CTAs) ------------------------------
         const int q = warp & 3, h = warp >> 2;
-        const uint32_t tempty_leader = mapa(tempty0, 0);
-        uint32_t tile = 0, round = 0;
+        const uint32_t tempty_leader = mapa(s.tempty0, 0);
+        uint32_t tile = 0;
         bool alive = true;
-        float scale = 1.0f;
-        if constexpr (MODE == DW) scale = final_scale(p, BF16);
-        float rel_of = 1.0f;                               // SOFT, gradients per token: one over the largest
+        float most = 0.0f;                                 // SOFT, gradients per token: the largest
         if constexpr (MODE == SOFT) {
-            if (p.per_row) {
-                const float most = __uint_as_float(*p.grad_max);
-                rel_of = most == 0.0f ? 0.0f : most;
-            }
+            if (p.per_row) most = __uint_as_float(*p.grad_max);
         }
         for (int u = cluster; u < n_units && alive; u += n_clusters) {
             const Unit w = unit_at<MODE>(p, valid, u);
-            const int row = w.m0 + 128 * (int)rank + q * 32 + lane;
+            const int row = w.m0 + 128 * rank + q * 32 + lane;
             const bool live = row < valid;
             float mx = -INFINITY, sum = 0.0f, rel = 0.0f;
             int target = -1;
-            if constexpr (MODE == STATS) {
-                if (live) target = p.target[row];
-            }
-            if constexpr (MODE == SOFT) {
-                if (live) {
+            if (live) {
+                target = p.target[row];
+                if constexpr (MODE == SOFT) {
                     const float2 st = p.stat[row];
                     mx = st.x; sum = st.y;
-                    target = p.target[row];
-                    rel = p.per_row ? (rel_of == 0.0f ? 0.0f : p.grad[p.rows[row]] / rel_of) : 1.0f;
+                    rel = p.per_row ? (most == 0.0f ? 0.0f : p.grad[p.rows[row]] / most) : 1.0f;
                     if (!BF16) rel *= FP16_SCALE;
                 }
             }
             for (int nt = w.n_first; nt < w.n_last; ++nt, ++tile) {
                 const uint32_t b = tile & 1;
-                if (!wait_warp(tfull0 + 8 * b, tile >> 1 & 1, abort_flag, (13 << 8) | 1)) { alive = false; break; }
+                if (!wait_warp(s.tfull0 + 8 * b, tile >> 1 & 1, s.abort_flag, (13 << 8) | 1)) { alive = false; break; }
                 tc_fence_after();
-                const uint32_t taddr = tmem + ((uint32_t)(q * 32) << 16) + b * N + h * COLS;
-                const int col0 = (MODE == STATS || MODE == SOFT ? p.v0 : 0) + nt * N + h * COLS;      // of this warp, among all words
+                const uint32_t taddr = s.tmem + ((uint32_t)(q * 32) << 16) + b * N + h * COLS;
+                const int col0 = p.v0 + nt * N + h * COLS;                     // of this warp, among all words
                 if constexpr (MODE == STATS) {
 #pragma unroll 1
                     for (int c = 0; c < COLS / 32; ++c) {
@@ -418,76 +449,63 @@ product_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__
                     tc_fence_before();
                     __syncwarp();
                     if (lane == 0) arrive_remote(tempty_leader + 8 * b);
-                } else if constexpr (MODE == SOFT || MODE == DW) {
-                    const uint32_t slot = smem_u32(c_stage) + warp * 2 * BOX;
-                    if (!wait_warp(taken, (round & 1) ^ 1, abort_flag, (13 << 8) | 2)) { alive = false; break; }
+                } else {
+                    const uint32_t slot = smem_u32(s.c_stage) + warp * 2 * BOX;
+                    const uint64_t minus = pair2(-mx, -mx), scale = pair2(LOG2E, LOG2E), logs = pair2(-sum, -sum), rels = pair2(rel, rel);
+                    uint32_t r[2][32];                     // a chunk of 32 words at work, the next one on its way
+                    ld32(taddr, r[0]);
+                    if (!wait_warp(s.taken, (tile & 1) ^ 1, s.abort_flag, (13 << 8) | 2)) alive = false;
 #pragma unroll
                     for (int c = 0; c < COLS / 32; ++c) {
-                        uint32_t r[32];
-                        ld32(taddr + c * 32, r);
                         ld_wait();
-                        if constexpr (MODE == SOFT) {
-                            const int hit = target - (col0 + c * 32);
-                            const int left = p.v0 + p.vc - (col0 + c * 32);        // words of the piece from here on
+                        if (c + 1 < COLS / 32) ld32(taddr + (c + 1) * 32, r[(c + 1) & 1]);
+                        else {
+                            tc_fence_before();
+                            __syncwarp();
+                            if (lane == 0) arrive_remote(tempty_leader + 8 * b);       // all of the tile is in registers
+                        }
+                        uint32_t(&z)[32] = r[c & 1];
+                        const int hit = target - (col0 + c * 32), left = p.v0 + p.vc - (col0 + c * 32);      // words of the piece from here on
+                        // two at a time: e^(z - lse), rounded once in the difference and once with the logarithm of the sum
 #pragma unroll
-                            for (int j = 0; j < 32; ++j) r[j] = __float_as_uint(exp2_approx((__uint_as_float(r[j]) - mx) * LOG2E - sum));
-                            if ((unsigned)hit < 32u) {
+                        for (int j = 0; j < 32; j += 2)
+                            asm("{\n\t.reg .b64 a;\n\t"
+                                "mov.b64 a, {%0, %1};\n\t"
+                                "add.rn.f32x2 a, a, %2;\n\t"
+                                "fma.rn.f32x2 a, a, %3, %4;\n\t"
+                                "mov.b64 {%0, %1}, a;\n\t"
+                                "ex2.approx.ftz.f32 %0, %0;\n\tex2.approx.ftz.f32 %1, %1;\n\t}"
+                                : "+r"(z[j]), "+r"(z[j + 1]) : "l"(minus), "l"(scale), "l"(logs));
+                        if ((unsigned)hit < 32u) {
 #pragma unroll
-                                for (int j = 0; j < 32; ++j)
-                                    if (j == hit) r[j] = __float_as_uint(__uint_as_float(r[j]) - 1.0f);
-                            }
+                            for (int j = 0; j < 32; ++j)
+                                if (j == hit) z[j] = __float_as_uint(__uint_as_float(z[j]) - 1.0f);
+                        }
+                        if (!BF16 || p.per_row) {
 #pragma unroll
-                            for (int j = 0; j < 32; ++j) r[j] = __float_as_uint(__uint_as_float(r[j]) * rel);
-                            if (!live || left < 32) {
+                            for (int j = 0; j < 32; j += 2)
+                                asm("{\n\t.reg .b64 a;\n\t"
+                                    "mov.b64 a, {%0, %1};\n\t"
+                                    "mul.rn.f32x2 a, a, %2;\n\t"
+                                    "mov.b64 {%0, %1}, a;\n\t}" : "+r"(z[j]), "+r"(z[j + 1]) : "l"(rels));
+                        }
+                        if (!live || left < 32) {
 #pragma unroll
-                                for (int j = 0; j < 32; ++j)
-                                    if (!live || j >= left) r[j] = 0u;
-                            }
-                        } else {
-#pragma unroll
-                            for (int j = 0; j < 32; ++j) r[j] = w.KB ? __float_as_uint(__uint_as_float(r[j]) * scale) : 0u;
+                            for (int j = 0; j < 32; ++j)
+                                if (!live || j >= left) z[j] = 0u;
                         }
 #pragma unroll
                         for (int j = 0; j < 4; ++j) {      // 16 bytes: 8 elements
                             uint32_t v[4];
 #pragma unroll
-                            for (int i = 0; i < 4; ++i) v[i] = pack2<BF16>(__uint_as_float(r[j * 8 + 2 * i]), __uint_as_float(r[j * 8 + 2 * i + 1]));
-                            const int chunk = (c & 1) * 4 + j;
-                            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};"
-                                         ::"r"(slot + (c >> 1) * BOX + lane * 128 + ((chunk ^ (lane & 7)) << 4)), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]) : "memory");
-                        }
-                    }
-                    tc_fence_before();
-                    fence_async_smem();
-                    __syncwarp();
-                    if (lane == 0) { arrive_remote(tempty_leader + 8 * b); mbar_arrive(staged); }
-                    ++round;
-                } else {
-                    const uint32_t slot = smem_u32(c_stage) + warp * 2 * BOX;
-#pragma unroll
-                    for (int half = 0; half < 2; ++half, ++round) {
-                        if (!wait_warp(taken, (round & 1) ^ 1, abort_flag, (13 << 8) | 2)) { alive = false; break; }
-#pragma unroll
-                        for (int c = 0; c < 2; ++c) {
-                            uint32_t r[32];
-                            ld32(taddr + half * 64 + c * 32, r);
-                            ld_wait();
-#pragma unroll
-                            for (int j = 0; j < 8; ++j) {
-                                if (!w.KB) r[4 * j] = r[4 * j + 1] = r[4 * j + 2] = r[4 * j + 3] = 0u;
-                                asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};"
-                                             ::"r"(slot + c * BOX + lane * 128 + ((j ^ (lane & 7)) << 4)), "r"(r[4 * j]), "r"(r[4 * j + 1]), "r"(r[4 * j + 2]), "r"(r[4 * j + 3]) : "memory");
-                            }
-                        }
-                        if (half == 1) tc_fence_before();
-                        fence_async_smem();
-                        __syncwarp();
-                        if (lane == 0) {
-                            if (half == 1) arrive_remote(tempty_leader + 8 * b);
-                            mbar_arrive(staged);
+                            for (int i = 0; i < 4; ++i) v[i] = pack2<BF16>(__uint_as_float(z[j * 8 + 2 * i]), __uint_as_float(z[j * 8 + 2 * i + 1]));
+                            if (alive) stage16(slot + (c >> 1) * BOX, lane, (c & 1) * 4 + j, v[0], v[1], v[2], v[3]);
                         }
                     }
                     if (!alive) break;
+                    fence_async_smem();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(s.staged);
                 }
             }
             if constexpr (MODE == STATS) {
@@ -499,15 +517,172 @@ product_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__
             }
         }
     }
+    s.finish();
+}
 
-    // nobody leaves while the other CTA may still read this CTA's shared memory or signal its barriers
-    tc_fence_before();
-    __syncthreads();
-    cluster_sync();
-    if (warp == W_MMA) {
-        tc_fence_after();
-        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+// Both gradients of a piece.  dx tiles: A = dz as stored, B = W, MN-major; fp32 sums, stored or added (the pieces run one after the other, so
+// the order of a sum is always the same).  dW tiles: A = dz's transpose, B = x, both MN-major; the piece's rows of dW, complete, scaled and
+// rounded, or with DW_SUMS the fp32 sums of a cut reduction.
+struct GradMaps { CUtensorMap z_rows, z_cols, w_cols, x_cols, xg_cols, c_dx, c_dw; };
+
+template <bool BF16, bool DW_SUMS>
+__global__ void __launch_bounds__(THREADS, 1)
+grads_kernel(const __grid_constant__ GradMaps maps, const Params p) {
+    extern __shared__ uint8_t smem_raw[];
+    Setup<C_BYTES> s(smem_raw);
+    const int warp = s.warp, lane = s.lane, rank = (int)s.rank;
+    const int valid = *p.n_valid;
+    const Schedule plan(p, valid, blockIdx.x >> 1, gridDim.x >> 1);
+    bool dx;
+    int u;
+
+    if (warp == W_TMA) {
+        // ------------------------------ TMA producer (both CTAs) ------------------------------
+        if (lane == 0) {
+            const uint32_t full_leader = mapa(s.full0, 0);
+            const CUtensorMap* map_x = valid != p.T ? &maps.xg_cols : &maps.x_cols;
+            uint32_t it = 0;
+            bool alive = true;
+            for (int i = 0; alive && plan.at(i, dx, u); ++i) {
+                const Unit w = dx ? unit_at<DX>(p, valid, u) : unit_at<DW>(p, valid, u);
+                const int ma = w.m0 + 128 * rank, nb = w.n_first * N + 128 * rank;
+                const CUtensorMap* map_b = dx ? &maps.w_cols : map_x;
+                for (int kb = 0; kb < w.KB; ++kb, ++it) {
+                    const int st = it % STAGES;
+                    if (!wait(s.empty0 + 8 * st, (it / STAGES & 1) ^ 1, s.abort_flag, (11 << 8) | 2)) { alive = false; break; }
+                    if (rank == 0) mbar_expect_tx(s.full0 + 8 * st, 4 * SIDE);
+                    const uint32_t bar = full_leader + 8 * st, da = smem_u32(s.smem_a + st * SIDE), db = smem_u32(s.smem_b + st * SIDE);
+                    const int k = (w.kb0 + kb) * KE, y = dx ? p.v0 + k : k;
+                    if (dx) {
+                        load_2d(&maps.z_rows, bar, da, k, ma);
+                    } else {
+                        load_2d(&maps.z_cols, bar, da, ma, k);
+                        load_2d(&maps.z_cols, bar, da + SIDE / 2, ma + 64, k);
+                    }
+                    load_2d(map_b, bar, db, nb, y);
+                    load_2d(map_b, bar, db + SIDE / 2, nb + 64, y);
+                }
+            }
+            if (!alive) s.drain();
+        }
+    } else if (warp == W_MMA) {
+        // ------------------------------ MMA issuer (leader; a whole warp, one elected lane) ------------------------------
+        if (rank == 0) {
+            constexpr uint32_t idesc_dx = make_idesc_f16(BF16, M, N, false, true), idesc_dw = make_idesc_f16(BF16, M, N, true, true);
+            // K-major: a step of 16 elements is 32 bytes of the row.  MN-major: 16 rows of 128 bytes; the second 64 columns are a panel
+            // of their own, SIDE / 2 bytes on (the leading offset).
+            constexpr uint32_t LEAD = (SIDE / 2) >> 4;
+            const uint32_t a0 = (smem_u32(s.smem_a) >> 4) & 0x3FFF, b0 = ((smem_u32(s.smem_b) >> 4) & 0x3FFF) | (LEAD << 16);
+            const uint32_t tfull_own = mapa(s.tfull0, 0), tfull_peer = mapa(s.tfull0, 1);
+            const uint32_t empty_own = mapa(s.empty0, 0), empty_peer = mapa(s.empty0, 1);
+            uint32_t it = 0, tile = 0;
+            bool alive = true;
+            for (; alive && plan.at((int)tile, dx, u); ++tile) {
+                const Unit w = dx ? unit_at<DX>(p, valid, u) : unit_at<DW>(p, valid, u);
+                const uint32_t b = tile & 1;
+                if (!wait_warp(s.tempty0 + 8 * b, (tile >> 1 & 1) ^ 1, s.abort_flag, (12 << 8) | 5)) { alive = false; break; }
+                tc_fence_after();
+                for (int kb = 0; kb < w.KB; ++kb, ++it) {
+                    const uint32_t st = it % STAGES;
+                    if (!wait_warp(s.full0 + 8 * st, it / STAGES & 1, s.abort_flag, (12 << 8) | 4)) { alive = false; break; }
+                    tc_fence_after();
+                    if (dx) mma_block<2, 128>(s.tmem + b * N, (a0 + st * (SIDE >> 4)) | (1u << 16), b0 + st * (SIDE >> 4), idesc_dx, kb == 0);
+                    else mma_block<128, 128>(s.tmem + b * N, (a0 + st * (SIDE >> 4)) | (LEAD << 16), b0 + st * (SIDE >> 4), idesc_dw, kb == 0);
+                    commit_pair(empty_own + 8 * st, empty_peer + 8 * st);
+                }
+                if (!alive) break;
+                commit_pair(tfull_own + 8 * b, tfull_peer + 8 * b);
+            }
+            s.retire(tile, alive);
+        }
+    } else if (warp == W_STORE) {
+        // ------------------------------ finished boxes to the TMA unit (both CTAs) ------------------------------
+        const int w = lane >> 1, q = w & 3, h = w >> 2;
+        uint32_t round = 0;
+        bool alive = true;
+        for (int i = 0; alive && plan.at(i, dx, u); ++i) {
+            const Unit t = dx ? unit_at<DX>(p, valid, u) : unit_at<DW>(p, valid, u);
+            const int row = t.m0 + 128 * rank + q * 32;
+            const bool sums = dx || DW_SUMS;
+            const int per = sums ? 32 : 64, rounds = sums ? 2 : 1;             // elements of a box's row; rounds of a tile
+            for (int r = 0; r < rounds; ++r, ++round) {
+                const int col = t.n_first * N + h * COLS + (r * 2 + (lane & 1)) * per;
+                if (!wait_warp(s.staged, round & 1, s.abort_flag, (14 << 8) | 2)) { alive = false; break; }
+                if (lane < 2 * EPI) {
+                    const uint32_t box = smem_u32(s.c_stage) + lane * BOX;
+                    if (col < p.d) {
+                        if (dx) {
+                            if (p.add) add_2d(&maps.c_dx, box, col, t.split * p.dx_rows + row);
+                            else tma_store_2d(&maps.c_dx, box, col, t.split * p.dx_rows + row);
+                        } else if (DW_SUMS) {
+                            tma_store_2d(&maps.c_dw, box, col, t.split * p.dw_rows + row);
+                        } else if (p.v0 + row < p.V) {
+                            tma_store_2d(&maps.c_dw, box, col, p.v0 + row);
+                        }
+                    }
+                    tma_store_commit();
+                    tma_store_wait_read();
+                }
+                __syncwarp();
+                if (lane == 0) mbar_arrive(s.taken);
+            }
+        }
+        if (lane < 2 * EPI) tma_store_wait_all();
+    } else {
+        // ------------------------------ epilogue (both CTAs) ------------------------------
+        const int q = warp & 3, h = warp >> 2;
+        const uint32_t tempty_leader = mapa(s.tempty0, 0), slot = smem_u32(s.c_stage) + warp * 2 * BOX;
+        uint32_t round = 0;
+        bool alive = true;
+        const float scale = DW_SUMS ? 1.0f : final_scale(p, BF16);
+        for (int i = 0; alive && plan.at(i, dx, u); ++i) {
+            const Unit w = dx ? unit_at<DX>(p, valid, u) : unit_at<DW>(p, valid, u);
+            const uint32_t b = i & 1;
+            if (!wait_warp(s.tfull0 + 8 * b, i >> 1 & 1, s.abort_flag, (13 << 8) | 3)) { alive = false; break; }
+            tc_fence_after();
+            const uint32_t taddr = s.tmem + ((uint32_t)(q * 32) << 16) + b * N + h * COLS;
+            const int rounds = dx || DW_SUMS ? 2 : 1;
+            for (int r = 0; r < rounds; ++r, ++round) {
+                if (!wait_warp(s.taken, (round & 1) ^ 1, s.abort_flag, (13 << 8) | 4)) { alive = false; break; }
+                if (rounds == 2) {
+#pragma unroll
+                    for (int c = 0; c < 2; ++c) {
+                        uint32_t v[32];
+                        ld32(taddr + r * 64 + c * 32, v);
+                        ld_wait();
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) {
+                            if (!w.KB) v[4 * j] = v[4 * j + 1] = v[4 * j + 2] = v[4 * j + 3] = 0u;         // nothing to sum: no product either
+                            stage16(slot + c * BOX, lane, j, v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+                        }
+                    }
+                } else {
+#pragma unroll
+                    for (int c = 0; c < COLS / 32; ++c) {
+                        uint32_t v[32];
+                        ld32(taddr + c * 32, v);
+                        ld_wait();
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            uint32_t o[4];
+#pragma unroll
+                            for (int k = 0; k < 4; ++k)
+                                o[k] = w.KB ? pack2<BF16>(__uint_as_float(v[j * 8 + 2 * k]) * scale, __uint_as_float(v[j * 8 + 2 * k + 1]) * scale) : 0u;
+                            stage16(slot + (c >> 1) * BOX, lane, (c & 1) * 4 + j, o[0], o[1], o[2], o[3]);
+                        }
+                    }
+                }
+                if (r + 1 == rounds) tc_fence_before();
+                fence_async_smem();
+                __syncwarp();
+                if (lane == 0) {
+                    if (r + 1 == rounds) arrive_remote(tempty_leader + 8 * b);
+                    mbar_arrive(s.staged);
+                }
+            }
+        }
     }
+    s.finish();
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
@@ -781,21 +956,19 @@ static Backward carve_backward(void* mem, const Plan& r, bool want_dx, bool want
     return b;
 }
 
-template <int MODE, bool BF16>
-static int launch(const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& xg, const CUtensorMap& c, const Params& p, cudaStream_t st) {
-    constexpr auto kern = product_kernel<MODE, BF16>;
-    constexpr size_t smem = MODE == STATS ? SMEM_STATS : SMEM;
-    int rc = allow_smem_once<kern>(smem);
+template <auto KERN, size_t SMEM_BYTES, typename... A>
+static int launch(cudaStream_t st, A&&... args) {
+    int rc = allow_smem_once<KERN>(SMEM_BYTES);
     if (rc) return rc;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(2 * std::max(1, gemm_sm_count() / 2)); cfg.blockDim = dim3(THREADS); cfg.dynamicSmemBytes = smem; cfg.stream = st;
+    cfg.gridDim = dim3(2 * std::max(1, gemm_sm_count() / 2)); cfg.blockDim = dim3(THREADS); cfg.dynamicSmemBytes = SMEM_BYTES; cfg.stream = st;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = 2; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
     attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr; cfg.numAttrs = 2;
-    CINN_CHECK_CUDA(cudaLaunchKernelEx(&cfg, kern, a, b, xg, c, p));
+    CINN_CHECK_CUDA(cudaLaunchKernelEx(&cfg, KERN, args...));
     CINN_CHECK_LAUNCH();
     return CINN_OK;
 }
@@ -846,7 +1019,7 @@ static int forward(const void* x, int64_t ldx, const void* w, int64_t ldw, const
     Params p{};
     p.n_valid = s.n_valid; p.T = (int)r.T; p.V = (int)r.V; p.d = (int)r.d; p.parts = r.parts;
     p.part = f.part; p.part_ld = r.Tp; p.target_logit = f.target_logit; p.target = s.target;
-    if ((rc = launch<STATS, BF16>(ta, tb, tx, ta, p, st))) return rc;
+    if ((rc = launch<product_kernel<STATS, BF16>, SMEM_STATS>(st, ta, tb, tx, ta, p))) return rc;
     launch_dependent(loss_kernel, dim3((unsigned)ceil_div(r.T, 32)), dim3(32 * JOIN), 0, st, f.part, r.Tp, 2 * r.parts, f.target_logit, s, (int)r.T,
                      reduction, f.block_sum, loss);
     CINN_CHECK_LAUNCH();
@@ -867,40 +1040,37 @@ static int backward(const void* x, int64_t ldx, const void* w, int64_t ldw, cons
         launch_dependent(grad_max_kernel, dim3(grid_for(r.T, 1024)), dim3(256), 0, st, grad, s.slot, (int)r.T, b.grad_max);
         CINN_CHECK_LAUNCH();
     }
-    CUtensorMap x_rows, xg_rows, x_cols, xg_cols, w_rows, w_cols, c_dw, c_dx;
+    CUtensorMap x_rows, xg_rows, w_rows;
+    GradMaps g;
     if ((rc = map16(&x_rows, x, r.d, r.T, ldx, 128, BF16))) return rc;
     if ((rc = map16(&xg_rows, b.xg, r.d, up(r.T, KE), r.d, 128, BF16))) return rc;
-    if ((rc = map16(&x_cols, x, r.d, r.T, ldx, 64, BF16))) return rc;
-    if ((rc = map16(&xg_cols, b.xg, r.d, up(r.T, KE), r.d, 64, BF16))) return rc;
     if ((rc = map16(&w_rows, w, r.d, r.V, ldw, 128, BF16))) return rc;
-    if ((rc = map16(&w_cols, w, r.d, r.V, ldw, 64, BF16))) return rc;
+    if ((rc = map16(&g.x_cols, x, r.d, r.T, ldx, 64, BF16))) return rc;
+    if ((rc = map16(&g.xg_cols, b.xg, r.d, up(r.T, KE), r.d, 64, BF16))) return rc;
+    if ((rc = map16(&g.w_cols, w, r.d, r.V, ldw, 64, BF16))) return rc;
     auto sums = [&](CUtensorMap* m, float* base, int64_t rows) {
         return encode_map_2d(m, base, (uint64_t)r.d, (uint64_t)rows, (uint64_t)r.d * 4, 32, 32, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, CU_TENSOR_MAP_SWIZZLE_128B);
     };
-    if (dx && (rc = sums(&c_dx, b.dx, r.dx_splits * r.Tp))) return rc;
+    g.c_dx = g.c_dw = g.x_cols;            // (one that is not wanted is not used)
+    if (dx && (rc = sums(&g.c_dx, b.dx, r.dx_splits * r.Tp))) return rc;
     if (dw) {
-        if (r.dw_splits > 1) rc = sums(&c_dw, b.dw, r.dw_splits * up(r.V, M));
-        else rc = map16(&c_dw, dw, r.d, r.V, r.d, 32, BF16);
+        if (r.dw_splits > 1) rc = sums(&g.c_dw, b.dw, r.dw_splits * up(r.V, M));
+        else rc = map16(&g.c_dw, dw, r.d, r.V, r.d, 32, BF16);
         if (rc) return rc;
     }
+    p.dx_splits = dx ? r.dx_splits : 0; p.dx_rows = (int)r.Tp;
+    p.dw_splits = dw ? r.dw_splits : 0; p.dw_rows = (int)up(r.V, M);
     for (int i = 0; i < r.pieces; ++i) {
         p.v0 = (int)(i * r.vc);
         p.vc = (int)std::min<int64_t>(r.vc, r.V - p.v0);
-        CUtensorMap z_store, z_rows, z_cols;
+        p.add = i > 0;
+        CUtensorMap z_store;
         if ((rc = map16(&z_store, b.dz, p.vc, r.Tp, r.dz_ld, 32, BF16))) return rc;
-        if ((rc = map16(&z_rows, b.dz, p.vc, r.Tp, r.dz_ld, 128, BF16))) return rc;
-        if ((rc = map16(&z_cols, b.dz, p.vc, r.Tp, r.dz_ld, 64, BF16))) return rc;
-        if ((rc = launch<SOFT, BF16>(x_rows, w_rows, xg_rows, z_store, p, st))) return rc;
-        if (dx) {
-            p.add = i > 0; p.splits = r.dx_splits; p.rows_pad = (int)r.Tp;
-            if ((rc = launch<DX, BF16>(z_rows, w_cols, xg_rows, c_dx, p, st))) return rc;
-        }
-        if (dw) {
-            p.add = 0; p.splits = r.dw_splits; p.rows_pad = (int)up(r.V, M);
-            rc = r.dw_splits > 1 ? launch<DW_PART, BF16>(z_cols, x_cols, xg_cols, c_dw, p, st)
-                                 : launch<DW, BF16>(z_cols, x_cols, xg_cols, c_dw, p, st);
-            if (rc) return rc;
-        }
+        if ((rc = map16(&g.z_rows, b.dz, p.vc, r.Tp, r.dz_ld, 128, BF16))) return rc;
+        if ((rc = map16(&g.z_cols, b.dz, p.vc, r.Tp, r.dz_ld, 64, BF16))) return rc;
+        if ((rc = launch<product_kernel<SOFT, BF16>, SMEM>(st, x_rows, w_rows, xg_rows, z_store, p))) return rc;
+        rc = r.dw_splits > 1 ? launch<grads_kernel<BF16, true>, SMEM>(st, g, p) : launch<grads_kernel<BF16, false>, SMEM>(st, g, p);
+        if (rc) return rc;
     }
     if (dx) {
         launch_dependent(finish_kernel<BF16>, dim3(grid_for(r.T * (r.d / 4), 256)), dim3(256), 0, st, b.dx, r.dx_splits, r.Tp * r.d, (int)r.T, (int)r.d,
