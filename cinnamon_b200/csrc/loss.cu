@@ -36,9 +36,9 @@ constexpr int KE = 64;                     // elements of a K block: 128 bytes
 constexpr int STAGES = 4;
 constexpr int SIDE = 128 * 128;            // bytes of one operand's stage in one CTA: 128 rows (or columns) x 64 elements
 constexpr int EPI = 8, COLS = 128;         // epilogue warps: four lane quarters x two halves of the columns
-constexpr int W_TMA = EPI, W_MMA = EPI + 1, W_STORE = EPI + 2;
-constexpr int THREADS = (EPI + 3) * 32;
-constexpr int BOX = 32 * 128;              // a TMA-store box: 32 rows of 128 bytes; two per epilogue warp
+constexpr int W_TMA = EPI, W_MMA = EPI + 1;
+constexpr int THREADS = (EPI + 2) * 32;
+constexpr int BOX = 32 * 128;              // a TMA-store box: 32 rows of 128 bytes; two per epilogue warp, filled in turn
 constexpr int STAGE_BYTES = STAGES * 2 * SIDE;
 constexpr int C_BYTES = EPI * 2 * BOX;
 constexpr size_t SMEM_STATS = (size_t)STAGE_BYTES + 256 + 1024, SMEM = SMEM_STATS + C_BYTES;
@@ -235,7 +235,7 @@ template <int SMEM_C>
 struct Setup {
     uint8_t *smem_a, *smem_b, *c_stage;
     volatile int* abort_flag;
-    uint32_t full0, empty0, tfull0, tempty0, staged, taken, rank, tmem;
+    uint32_t full0, empty0, tfull0, tempty0, rank, tmem;
     int warp, lane;
 
     __device__ __forceinline__ Setup(uint8_t* raw) {
@@ -244,20 +244,17 @@ struct Setup {
         smem_b = smem + STAGES * SIDE;
         c_stage = smem + STAGE_BYTES;
         uint64_t* bars = reinterpret_cast<uint64_t*>(c_stage + SMEM_C);
-        // [0, S) full (used in the leader), [S, 2S) empty, then: tensor memory full (2), empty (2, leader), boxes staged, boxes taken
-        uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * STAGES + 6);
+        // [0, S) full (used in the leader), [S, 2S) empty, then: tensor memory full (2), empty (2, leader)
+        uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * STAGES + 4);
         abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
         warp = threadIdx.x >> 5; lane = threadIdx.x & 31;
         rank = cta_rank();
         full0 = smem_u32(bars); empty0 = smem_u32(bars + STAGES);
         tfull0 = smem_u32(bars + 2 * STAGES); tempty0 = smem_u32(bars + 2 * STAGES + 2);
-        staged = smem_u32(bars + 2 * STAGES + 4); taken = smem_u32(bars + 2 * STAGES + 5);
         if (threadIdx.x == 0) *abort_flag = 0;
         if (warp == W_TMA && lane == 0) {
             for (int s = 0; s < STAGES; ++s) { mbar_init(full0 + 8 * s, 1); mbar_init(empty0 + 8 * s, 1); }
             for (int b = 0; b < 2; ++b) { mbar_init(tfull0 + 8 * b, 1); mbar_init(tempty0 + 8 * b, 2 * EPI); }
-            mbar_init(staged, EPI);
-            mbar_init(taken, 1);
             asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         }
         if (warp == W_MMA) {
@@ -297,6 +294,32 @@ struct Setup {
 __device__ __forceinline__ void stage16(uint32_t box, int row, int piece, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
     asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(box + row * 128 + ((piece ^ (row & 7)) << 4)), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
+// An epilogue warp's two boxes, in turn: `open` waits until the one to be filled has been read by its last store (the one after may still
+// be on its way), `send` hands it over.  (All boxes of a tile by a warp of their own, behind a barrier of all warps: dz of 32768 x 8192 words took
+// 227 us, the tile's conversion and its stores one after the other.)
+struct Boxes {
+    uint32_t slot, turn = 0;
+    __device__ __forceinline__ Boxes(uint32_t s) : slot(s) {}
+    __device__ __forceinline__ uint32_t open(int lane) {
+        if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
+        __syncwarp();
+        return slot + (turn & 1) * BOX;
+    }
+    __device__ __forceinline__ void send(int lane, const CUtensorMap* map, int col, int row, bool store, bool add) {
+        fence_async_smem();
+        __syncwarp();
+        if (lane == 0) {
+            const uint32_t box = slot + (turn & 1) * BOX;
+            if (store) {
+                if (add) add_2d(map, box, col, row);
+                else tma_store_2d(map, box, col, row);
+            }
+            tma_store_commit();
+        }
+        ++turn;
+    }
+    __device__ __forceinline__ void drain(int lane) { if (lane == 0) tma_store_wait_all(); }
+};
 __device__ __forceinline__ uint64_t pair2(float a, float b) {
     uint64_t r;
     asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
@@ -366,29 +389,11 @@ product_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__
             }
             s.retire(tile, alive);
         }
-    } else if (warp == W_STORE) {
-        // ------------------------------ finished boxes to the TMA unit (both CTAs) ------------------------------
-        if constexpr (MODE == SOFT) {
-            const int w = lane >> 1, q = w & 3, h = w >> 2;
-            uint32_t round = 0;
-            for (int u = cluster; u < n_units; u += n_clusters, ++round) {
-                const Unit t = unit_at<MODE>(p, valid, u);
-                const int row = t.m0 + 128 * rank + q * 32, col = t.n_first * N + h * COLS + (lane & 1) * 64;
-                if (!wait_warp(s.staged, round & 1, s.abort_flag, (14 << 8) | 1)) break;
-                if (lane < 2 * EPI) {
-                    if (col < p.vc) tma_store_2d(&tm_c, smem_u32(s.c_stage) + lane * BOX, col, row);
-                    tma_store_commit();
-                    tma_store_wait_read();
-                }
-                __syncwarp();
-                if (lane == 0) mbar_arrive(s.taken);
-            }
-            if (lane < 2 * EPI) tma_store_wait_all();
-        }
     } else {
         // ------------------------------ epilogue (both CTAs) ------------------------------
         const int q = warp & 3, h = warp >> 2;
         const uint32_t tempty_leader = mapa(s.tempty0, 0);
+        Boxes boxes(smem_u32(s.c_stage) + warp * 2 * BOX);
         uint32_t tile = 0;
         bool alive = true;
         float most = 0.0f;                                 // SOFT, gradients per token: the largest
@@ -450,11 +455,10 @@ product_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__
                     __syncwarp();
                     if (lane == 0) arrive_remote(tempty_leader + 8 * b);
                 } else {
-                    const uint32_t slot = smem_u32(s.c_stage) + warp * 2 * BOX;
+                    uint32_t box = 0;
                     const uint64_t minus = pair2(-mx, -mx), scale = pair2(LOG2E, LOG2E), logs = pair2(-sum, -sum), rels = pair2(rel, rel);
                     uint32_t r[2][32];                     // a chunk of 32 words at work, the next one on its way
                     ld32(taddr, r[0]);
-                    if (!wait_warp(s.taken, (tile & 1) ^ 1, s.abort_flag, (13 << 8) | 2)) alive = false;
 #pragma unroll
                     for (int c = 0; c < COLS / 32; ++c) {
                         ld_wait();
@@ -464,6 +468,7 @@ product_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__
                             __syncwarp();
                             if (lane == 0) arrive_remote(tempty_leader + 8 * b);       // all of the tile is in registers
                         }
+                        if ((c & 1) == 0) box = boxes.open(lane);
                         uint32_t(&z)[32] = r[c & 1];
                         const int hit = target - (col0 + c * 32), left = p.v0 + p.vc - (col0 + c * 32);      // words of the piece from here on
                         // two at a time: e^(z - lse), rounded once in the difference and once with the logarithm of the sum
@@ -499,13 +504,13 @@ product_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__
                             uint32_t v[4];
 #pragma unroll
                             for (int i = 0; i < 4; ++i) v[i] = pack2<BF16>(__uint_as_float(z[j * 8 + 2 * i]), __uint_as_float(z[j * 8 + 2 * i + 1]));
-                            if (alive) stage16(slot + (c >> 1) * BOX, lane, (c & 1) * 4 + j, v[0], v[1], v[2], v[3]);
+                            stage16(box, lane, (c & 1) * 4 + j, v[0], v[1], v[2], v[3]);
+                        }
+                        if (c & 1) {
+                            const int col = nt * N + h * COLS + (c >> 1) * 64;
+                            boxes.send(lane, &tm_c, col, row - lane, col < p.vc, false);
                         }
                     }
-                    if (!alive) break;
-                    fence_async_smem();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(s.staged);
                 }
             }
             if constexpr (MODE == STATS) {
@@ -516,6 +521,7 @@ product_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__
                 if (alive && live) p.part[(int64_t)(n * 2 + h) * p.part_ld + row] = make_float2(mx, sum);
             }
         }
+        if constexpr (MODE == SOFT) boxes.drain(lane);
     }
     s.finish();
 }
@@ -595,92 +601,60 @@ grads_kernel(const __grid_constant__ GradMaps maps, const Params p) {
             }
             s.retire(tile, alive);
         }
-    } else if (warp == W_STORE) {
-        // ------------------------------ finished boxes to the TMA unit (both CTAs) ------------------------------
-        const int w = lane >> 1, q = w & 3, h = w >> 2;
-        uint32_t round = 0;
-        bool alive = true;
-        for (int i = 0; alive && plan.at(i, dx, u); ++i) {
-            const Unit t = dx ? unit_at<DX>(p, valid, u) : unit_at<DW>(p, valid, u);
-            const int row = t.m0 + 128 * rank + q * 32;
-            const bool sums = dx || DW_SUMS;
-            const int per = sums ? 32 : 64, rounds = sums ? 2 : 1;             // elements of a box's row; rounds of a tile
-            for (int r = 0; r < rounds; ++r, ++round) {
-                const int col = t.n_first * N + h * COLS + (r * 2 + (lane & 1)) * per;
-                if (!wait_warp(s.staged, round & 1, s.abort_flag, (14 << 8) | 2)) { alive = false; break; }
-                if (lane < 2 * EPI) {
-                    const uint32_t box = smem_u32(s.c_stage) + lane * BOX;
-                    if (col < p.d) {
-                        if (dx) {
-                            if (p.add) add_2d(&maps.c_dx, box, col, t.split * p.dx_rows + row);
-                            else tma_store_2d(&maps.c_dx, box, col, t.split * p.dx_rows + row);
-                        } else if (DW_SUMS) {
-                            tma_store_2d(&maps.c_dw, box, col, t.split * p.dw_rows + row);
-                        } else if (p.v0 + row < p.V) {
-                            tma_store_2d(&maps.c_dw, box, col, p.v0 + row);
-                        }
-                    }
-                    tma_store_commit();
-                    tma_store_wait_read();
-                }
-                __syncwarp();
-                if (lane == 0) mbar_arrive(s.taken);
-            }
-        }
-        if (lane < 2 * EPI) tma_store_wait_all();
     } else {
         // ------------------------------ epilogue (both CTAs) ------------------------------
         const int q = warp & 3, h = warp >> 2;
-        const uint32_t tempty_leader = mapa(s.tempty0, 0), slot = smem_u32(s.c_stage) + warp * 2 * BOX;
-        uint32_t round = 0;
-        bool alive = true;
+        const uint32_t tempty_leader = mapa(s.tempty0, 0);
+        Boxes boxes(smem_u32(s.c_stage) + warp * 2 * BOX);
         const float scale = DW_SUMS ? 1.0f : final_scale(p, BF16);
-        for (int i = 0; alive && plan.at(i, dx, u); ++i) {
+        for (int i = 0; plan.at(i, dx, u); ++i) {
             const Unit w = dx ? unit_at<DX>(p, valid, u) : unit_at<DW>(p, valid, u);
             const uint32_t b = i & 1;
-            if (!wait_warp(s.tfull0 + 8 * b, i >> 1 & 1, s.abort_flag, (13 << 8) | 3)) { alive = false; break; }
+            if (!wait_warp(s.tfull0 + 8 * b, i >> 1 & 1, s.abort_flag, (13 << 8) | 3)) break;
             tc_fence_after();
             const uint32_t taddr = s.tmem + ((uint32_t)(q * 32) << 16) + b * N + h * COLS;
-            const int rounds = dx || DW_SUMS ? 2 : 1;
-            for (int r = 0; r < rounds; ++r, ++round) {
-                if (!wait_warp(s.taken, (round & 1) ^ 1, s.abort_flag, (13 << 8) | 4)) { alive = false; break; }
-                if (rounds == 2) {
+            const int row = w.m0 + 128 * rank + q * 32, col0 = w.n_first * N + h * COLS;
+            const bool sums = dx || DW_SUMS;
+            uint32_t box = 0, r[2][32];                    // 32 columns at work, the next ones on their way
+            ld32(taddr, r[0]);
 #pragma unroll
-                    for (int c = 0; c < 2; ++c) {
-                        uint32_t v[32];
-                        ld32(taddr + r * 64 + c * 32, v);
-                        ld_wait();
-#pragma unroll
-                        for (int j = 0; j < 8; ++j) {
-                            if (!w.KB) v[4 * j] = v[4 * j + 1] = v[4 * j + 2] = v[4 * j + 3] = 0u;         // nothing to sum: no product either
-                            stage16(slot + c * BOX, lane, j, v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
-                        }
-                    }
-                } else {
-#pragma unroll
-                    for (int c = 0; c < COLS / 32; ++c) {
-                        uint32_t v[32];
-                        ld32(taddr + c * 32, v);
-                        ld_wait();
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-                            uint32_t o[4];
-#pragma unroll
-                            for (int k = 0; k < 4; ++k)
-                                o[k] = w.KB ? pack2<BF16>(__uint_as_float(v[j * 8 + 2 * k]) * scale, __uint_as_float(v[j * 8 + 2 * k + 1]) * scale) : 0u;
-                            stage16(slot + (c >> 1) * BOX, lane, (c & 1) * 4 + j, o[0], o[1], o[2], o[3]);
-                        }
-                    }
+            for (int c = 0; c < COLS / 32; ++c) {
+                ld_wait();
+                if (c + 1 < COLS / 32) ld32(taddr + (c + 1) * 32, r[(c + 1) & 1]);
+                else {
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) arrive_remote(tempty_leader + 8 * b);       // all of the tile is in registers
                 }
-                if (r + 1 == rounds) tc_fence_before();
-                fence_async_smem();
-                __syncwarp();
-                if (lane == 0) {
-                    if (r + 1 == rounds) arrive_remote(tempty_leader + 8 * b);
-                    mbar_arrive(s.staged);
+                uint32_t(&v)[32] = r[c & 1];
+                if (!w.KB) {                               // nothing to sum: no product either
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) v[j] = 0u;
+                }
+                if (sums) {                                // a box: 32 columns
+                    box = boxes.open(lane);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) stage16(box, lane, j, v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+                    const int col = col0 + c * 32;
+                    if (dx) boxes.send(lane, &maps.c_dx, col, w.split * p.dx_rows + row, col < p.d, p.add);
+                    else boxes.send(lane, &maps.c_dw, col, w.split * p.dw_rows + row, col < p.d, false);
+                } else {                                   // 64 columns
+                    if ((c & 1) == 0) box = boxes.open(lane);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        uint32_t o[4];
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) o[k] = pack2<BF16>(__uint_as_float(v[j * 8 + 2 * k]) * scale, __uint_as_float(v[j * 8 + 2 * k + 1]) * scale);
+                        stage16(box, lane, (c & 1) * 4 + j, w.KB ? o[0] : 0u, w.KB ? o[1] : 0u, w.KB ? o[2] : 0u, w.KB ? o[3] : 0u);
+                    }
+                    if (c & 1) {
+                        const int col = col0 + (c >> 1) * 64;
+                        boxes.send(lane, &maps.c_dw, col, p.v0 + row, col < p.d && p.v0 + row < p.V, false);
+                    }
                 }
             }
         }
+        boxes.drain(lane);
     }
     s.finish();
 }
