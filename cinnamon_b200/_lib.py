@@ -104,6 +104,7 @@ SIGNATURES = {
     "cinn_linear_ce_forward": [_vp, _i64, _vp, _i64, _i32, _vp, _i64, _i64, _i64, _i64, _i32, _vp, _vp, _vp, _i64, _vp],
     "cinn_linear_ce_backward": [_vp, _i64, _vp, _i64, _i32, _vp, _i64, _i64, _i64, _i32, _vp, _vp, _vp, _vp, _i64, _vp],
     "cinn_rotary": [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i32, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i32, _i32, ctypes.c_float, _vp],
+    "cinn_moe_route_form_workspace_ints": [_i64, _i32],
     "cinn_moe_route_form": [_vp, _i32, _vp, _i64, _i32, _i32, _i32, _i32, _i32, _i32, ctypes.c_float] + [_vp] * 12,
     "cinn_moe_route_form_backward": [_vp, _i32] + [_vp] * 6 + [_i64, _i32, _i32, _i32, _i32, ctypes.c_float, _vp, _vp],
     "cinn_launch_count": [],
@@ -128,7 +129,7 @@ def _load() -> ctypes.CDLL:
         fn.argtypes = argtypes
         fn.restype = (ctypes.c_char_p if name == "cinn_last_error"
                       else ctypes.c_longlong if name == "cinn_set_wait_limit_cycles"
-                      else ctypes.c_int64 if name in ("cinn_moe_route_workspace_ints", "cinn_moe_route_static_max_ints", "cinn_fp8_gemm_workspace_bytes", "cinn_moe_balance_workspace_bytes",
+                      else ctypes.c_int64 if name in ("cinn_moe_route_workspace_ints", "cinn_moe_route_form_workspace_ints", "cinn_moe_route_static_max_ints", "cinn_fp8_gemm_workspace_bytes", "cinn_moe_balance_workspace_bytes",
                                                  "cinn_sparse_attn_workspace_bytes", "cinn_launch_count",
                                                  "cinn_fp8_grouped_wgrad_scratch_bytes", "cinn_fp8_grouped_wgrad_fused_scratch_bytes",
                                                  "cinn_quant_segments_bytes", "cinn_fp8_grouped_wgrad_segments_scratch_bytes",

@@ -139,6 +139,7 @@ int gates_backward(const void* logits, int dtype, const int64_t* sorted_experts,
 int rotary(const void* const* in, void* const* out, const int64_t* in_strides, const int64_t* out_strides, const int64_t* heads, const int64_t* d,
            const int64_t* start, int dtype, int64_t B, int64_t L, const int64_t* positions, int64_t pos_b, int64_t pos_l, const double* freq, int64_t pairs,
            int interleaved, int inverse, float magnitude, cudaStream_t st);
+int64_t moe_route_form_workspace_ints(int64_t T, int E);
 int moe_route_form(const void* logits, int logits_dtype, const float* bias, int64_t T, int E, int top_k, int scores, int n_groups, int top_groups,
                    int renormalise, float scale, int* workspace, int* top_experts, float* top_gates, int64_t* token_indices, float* sorted_scores,
                    int64_t* sorted_experts, int64_t* counts, int64_t* starts, int64_t* ends, int64_t* pair_pos, float* pair_gate, cudaStream_t st);
@@ -394,6 +395,7 @@ int cinn_rotary(const void* const* in, void* const* out, const int64_t* in_strid
                         interleaved, inverse, magnitude, (cudaStream_t)stream);
 }
 
+int64_t cinn_moe_route_form_workspace_ints(int64_t n_tokens, int n_experts) { return cinn::moe_route_form_workspace_ints(n_tokens, n_experts); }
 int cinn_moe_route_form(const void* logits, int logits_dtype, const float* bias, int64_t n_tokens, int n_experts, int top_k, int scores,
                         int n_groups, int top_groups, int renormalise, float scale, int* workspace, int* top_experts, float* top_gates,
                         int64_t* token_indices, float* sorted_scores, int64_t* sorted_experts, int64_t* counts, int64_t* starts, int64_t* ends,

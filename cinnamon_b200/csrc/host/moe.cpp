@@ -50,7 +50,8 @@ Routes route(const Tensor& logits_in, const Tensor& bias, int64_t top_k, const R
     r.longs = empty({3 * r.pairs + 3 * E}, at::kLong, dev);
     r.floats = empty({2 * r.pairs}, at::kFloat, dev);
     r.top = empty({r.pairs}, at::kInt, dev);
-    Tensor ws = empty({std::max<int64_t>(1, api.cinn_moe_route_workspace_ints(T, (int)E))}, at::kInt, dev);
+    const int64_t need = form.reference ? api.cinn_moe_route_workspace_ints(T, (int)E) : api.cinn_moe_route_form_workspace_ints(T, (int)E);
+    Tensor ws = empty({std::max<int64_t>(1, need)}, at::kInt, dev);
     Tensor top_gates = empty({r.pairs}, at::kFloat, dev);
     if (gates_by_slot) *gates_by_slot = top_gates;
     if (form.reference)

@@ -6,8 +6,7 @@
 //   route_topk_kernel     one warp per token: sigmoid scores, the k largest of score + bias (ties: the lower
 //                         expert id), gates = score / (sum of the k scores + 1e-9); every CTA also leaves a histogram
 //                         of the experts its tokens selected in the workspace
-//   route_scan_kernel     one warp per expert: the running sum of those histograms over the CTAs (the histograms
-//                         become offsets) -> counts.  With 32 CTAs or fewer the scatter kernel does this itself.
+//   route_scan_kernel     the running sum of those histograms over the CTAs (the histograms become offsets) -> counts.  With 32 CTAs or fewer the scatter kernel does this itself.
 //   route_scatter_kernel  the same CTAs again: an exclusive scan of the counts gives every expert's first row, and every
 //                         pair gets the next free row of its expert, pairs taken in (token, slot) order, so the order is
 //                         that of a stable sort and the same on every run; writes token_indices / sorted_scores /
@@ -139,7 +138,7 @@ constexpr int ROUTE_MAX_GROUPS = 32;
 
 __device__ __forceinline__ uint32_t ordered(float v) {
     const uint32_t b = __float_as_uint(v);
-    return b & 0x80000000u ? ~b : b | 0x80000000u;
+    return b ^ ((uint32_t)((int)b >> 31) | 0x80000000u);
 }
 __device__ __forceinline__ float unordered(uint32_t k) { return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k); }
 __device__ __forceinline__ float warp_sum(float v) {
@@ -297,32 +296,52 @@ __device__ __forceinline__ void load_logits(const L* __restrict__ row, int e0, i
     }
 }
 
-// VPL keys in falling order (odd-even merges)
-template <int VPL>
-__device__ __forceinline__ void sort_keys(uint32_t (&k)[VPL]) {
+constexpr int ROUTE_KEPT = 8;                                // keys that a lane keeps, at most
+
+__device__ __forceinline__ void order_keys(uint32_t& a, uint32_t& b) { const uint32_t hi = max(a, b); b = min(a, b); a = hi; }
+
+// The largest KEEP of VPL keys, in falling order: pieces of KEEP sorted (odd-even merges), and merged by their larger halves (bitonic)
+template <int VPL, int KEEP>
+__device__ __forceinline__ void largest_keys(const uint32_t (&k)[VPL], uint32_t (&out)[KEEP]) {
 #pragma unroll
-    for (int p = 1; p < VPL; p *= 2)
+    for (int at = 0; at < VPL; at += KEEP) {
+        uint32_t q[KEEP];
 #pragma unroll
-        for (int q = p; q >= 1; q /= 2)
+        for (int i = 0; i < KEEP; ++i) q[i] = k[at + i];
 #pragma unroll
-            for (int j = q % p; j + q < VPL; j += 2 * q)
+        for (int p = 1; p < KEEP; p *= 2)
 #pragma unroll
-                for (int i = 0; i < q; ++i)
-                    if (j + i + q < VPL && (j + i) / (2 * p) == (j + i + q) / (2 * p)) {
-                        const uint32_t hi = max(k[j + i], k[j + i + q]), lo = min(k[j + i], k[j + i + q]);
-                        k[j + i] = hi;
-                        k[j + i + q] = lo;
-                    }
+            for (int w = p; w >= 1; w /= 2)
+#pragma unroll
+                for (int j = w % p; j + w < KEEP; j += 2 * w)
+#pragma unroll
+                    for (int i = 0; i < w; ++i)
+                        if (j + i + w < KEEP && (j + i) / (2 * p) == (j + i + w) / (2 * p)) order_keys(q[j + i], q[j + i + w]);
+        if (at == 0) {
+#pragma unroll
+            for (int i = 0; i < KEEP; ++i) out[i] = q[i];
+        } else {
+#pragma unroll
+            for (int i = 0; i < KEEP; ++i) out[i] = max(out[i], q[KEEP - 1 - i]);
+#pragma unroll
+            for (int w = KEEP / 2; w >= 1; w /= 2)
+#pragma unroll
+                for (int i = 0; i < KEEP; ++i)
+                    if ((i & w) == 0) order_keys(out[i], out[i + w]);
+        }
+    }
 }
 
-// A lane holds VPL neighbouring experts as keys: score + bias as an ordered integer whose last bits are the expert's number in the lane (the
-// lower one larger), sorted.  A round is the largest key without those bits among the warp's, and the lowest expert that has it: two
-// warp-wide reductions and a shift of the winner's keys.  (Unsorted, with a vote and a look through the winner's keys: 1280
-// instructions a token for 8 of 256 experts, 83 us for 32768 tokens.)
+// What bounds it are the integer units, at half the rate of the floating-point ones: selections, comparisons, minima.  So a lane's VPL
+// neighbouring experts are keys that need little of them: score + bias, made positive by a common offset, is a float whose bits are in order
+// as they are, and its last bits are the expert's number in the lane (the lower one larger).  A lane keeps its eight largest, sorted; should
+// one run out of them, the token is chosen in 64 bits.  A round is one reduction, a vote and a shift of the winner's keys.  8 of 256 experts,
+// 32768 tokens, 46 us, 760 instructions a token, 16 of them a round.  (All keys of a lane unsorted, with a look through the winner's: 1280
+// and 83 us; 1024 experts, all 32 keys of a lane sorted: 281 us in all, like this 110.)
 //
 // Errors of the quick scores.  Sigmoid: the exponent's rounding is |x| 2^-24 of e^-x, its part in the score s (1 - s) |x| 2^-24 < 2^-26, and
-// ex2, the sum and rcp add less than 2^-22: two scores are sure to be in order when they are 2^-20 apart (and 2^-22 of themselves, for
-// the bias's sum, and what the key's last bits hide).  Softmax: p |x - max| 2^-24 is below 2^-25 of the largest p, ex2, the sum and the
+// ex2, the sum and rcp add less than 2^-22: two scores are sure to be in order when they are 2^-20 apart, and HIDDEN of the key: what
+// its last bits hide, and the sum with the bias.  Softmax: p |x - max| 2^-24 is below 2^-25 of the largest p, ex2, the sum and the
 // quotient are 2^-21 of p: 2^-19 of the largest p.  A group's sum of two: twice as much.
 template <int VPL, typename L, bool SOFTMAX>                 // E <= 32 * VPL
 __global__ void __launch_bounds__(256, VPL <= 8 ? 5 : 2)
@@ -331,29 +350,35 @@ route_form_kernel(const L* __restrict__ logits, const float* __restrict__ bias, 
     pdl_wait();
     pdl_trigger();
     __shared__ int s_hist[ROUTE_MAX_EXPERTS];
+    __shared__ uint2 s_list[8][32];                                            // per warp: the chosen keys and their lanes
     for (int e = threadIdx.x; e < E; e += 256) s_hist[e] = 0;
     __syncthreads();
-    constexpr int BITS = VPL == 1 ? 0 : VPL == 2 ? 1 : VPL == 4 ? 2 : VPL == 8 ? 3 : VPL == 16 ? 4 : 5;
+    constexpr int KEEP = VPL < ROUTE_KEPT ? VPL : ROUTE_KEPT;
     constexpr uint32_t INDEX = VPL - 1;
-    constexpr float HIDDEN = (float)(2 * VPL + 2) * 0x1p-23f;                  // of a score + bias: its rounding and what the last bits hide
+    constexpr float HIDDEN = (float)(2 * VPL + 4) * 0x1p-23f;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, e0 = lane * VPL;
+    const uint32_t below = (1u << lane) - 1u;
     const int t_end = min((int)(blockIdx.x + 1) * tokens_per_cta, T);
     const int per = E / form.n_groups, lanes_per = per / VPL;                  // a group's experts; its lanes, where they are whole
     const bool whole = per % VPL == 0 && (lanes_per & (lanes_per - 1)) == 0;
-    float b[VPL];
+    const unsigned my_group = whole ? (unsigned)lane / (unsigned)lanes_per & 31u : 0u;
+    float b[VPL], lowest = 0.0f;
+    bool bans = false;                                                         // biases that keep experts out
 #pragma unroll
-    for (int i = 0; i < VPL; ++i) b[i] = bias && e0 + i < E ? bias[e0 + i] : 0.0f;
-    float bias_most = 0.0f;                                                    // what can cancel in a group's sum: not the biases that ban experts
-    if (form.n_groups > 1) {
-#pragma unroll
-        for (int i = 0; i < VPL; ++i) bias_most = fmaxf(bias_most, b[i] > -1e30f ? fabsf(b[i]) : 0.0f);
-        bias_most = warp_max(bias_most);
+    for (int i = 0; i < VPL; ++i) {
+        b[i] = bias && e0 + i < E ? bias[e0 + i] : 0.0f;
+        if (b[i] <= -1e30f) { b[i] = -1e30f; bans = true; }
+        else lowest = fminf(lowest, b[i]);
     }
+    bans = __any_sync(0xffffffffu, bans);
+    lowest = -warp_max(-lowest);
+#pragma unroll
+    for (int i = 0; i < VPL; ++i) b[i] -= lowest;
     for (int t = blockIdx.x * tokens_per_cta + warp; t < t_end; t += 8) {
         const L* row = logits + (int64_t)t * E;
         float m = 0.0f, sum = 1.0f, near;
         uint32_t key[VPL];                                                     // 0: not to be chosen
-        bool unsure = false;
+        float odd = 0.0f;                                                      // a NaN where a score is a NaN or infinite
         {
             float x[VPL];
             load_logits<VPL, L>(row, e0, E, vec, x);
@@ -379,23 +404,32 @@ route_form_kernel(const L* __restrict__ logits, const float* __restrict__ bias, 
                 for (int i = 0; i < VPL; ++i) x[i] = rcp_approx(1.0f + exp2_approx(x[i] * -1.4426950408889634f)) + b[i];
             }
 #pragma unroll
-            for (int i = 0; i < VPL; ++i) {
-                unsure |= x[i] != x[i];
-                key[i] = e0 + i < E ? (ordered(x[i]) & ~INDEX) | (INDEX - i) : 0u;
+            for (int i = 0; i < VPL; ++i) odd = fmaf(x[i], 0.0f, odd);
+            if (bans) {
+#pragma unroll
+                for (int i = 0; i < VPL; ++i) x[i] = fmaxf(x[i], 0.0f);
+            }
+#pragma unroll
+            for (int i = 0; i < VPL; ++i) key[i] = (__float_as_uint(x[i]) & ~INDEX) | (INDEX - i);
+            if (e0 + VPL > E) {
+#pragma unroll
+                for (int i = 0; i < VPL; ++i) key[i] = e0 + i < E ? key[i] : 0u;
             }
         }
-        unsure = __any_sync(0xffffffffu, unsure);
-        if (whole) sort_keys<VPL>(key);
+        // (a group's sum with a banned expert in it is not what these keys add up to)
+        bool unsure = __any_sync(0xffffffffu, odd != odd) || (bans && form.n_groups > 1);
+        uint32_t best[KEEP];
+        if (whole) largest_keys<VPL, KEEP>(key, best);
         if (form.n_groups > 1 && !unsure) {
-            float mine = -INFINITY;                                            // lane g: group g's score
+            float mine = -1.0f;                                                // lane g: group g's score
             if (whole) {
-                uint32_t a = key[0] & ~INDEX, c = VPL > 1 ? key[VPL > 1] & ~INDEX : 0u;        // the lane's two best, then the group's
+                uint32_t a = best[0] & ~INDEX, c = KEEP > 1 ? best[KEEP > 1] & ~INDEX : 0u;    // the lane's two best, then the group's
                 for (int o = 1; o < lanes_per; o <<= 1) {
                     const uint32_t oa = __shfl_xor_sync(0xffffffffu, a, o), oc = __shfl_xor_sync(0xffffffffu, c, o);
                     c = max(min(a, oa), max(c, oc));
                     a = max(a, oa);
                 }
-                const float score = per > 1 ? unordered(a) + unordered(c) : unordered(a);
+                const float score = __uint_as_float(a) + __uint_as_float(c);
                 const float of_group = __shfl_sync(0xffffffffu, score, (lane * lanes_per) & 31);
                 if (lane < form.n_groups) mine = of_group;
             } else {
@@ -403,75 +437,79 @@ route_form_kernel(const L* __restrict__ logits, const float* __restrict__ bias, 
                     uint32_t a = 0, c = 0;
 #pragma unroll
                     for (int i = 0; i < VPL; ++i) {
-                        const uint32_t k = e0 + i >= g * per && e0 + i < (g + 1) * per ? key[i] : 0u;
+                        const uint32_t k = e0 + i >= g * per && e0 + i < (g + 1) * per ? key[i] & ~INDEX : 0u;
                         c = max(c, min(a, k));
                         a = max(a, k);
                     }
                     const uint32_t top = __reduce_max_sync(0xffffffffu, a);
                     const int owner = __ffs(__ballot_sync(0xffffffffu, a == top)) - 1;
                     const uint32_t next = __reduce_max_sync(0xffffffffu, lane == owner ? c : a);
-                    if (lane == g) mine = per > 1 ? unordered(top & ~INDEX) + unordered(next & ~INDEX) : unordered(top & ~INDEX);
+                    if (lane == g) mine = __uint_as_float(top) + __uint_as_float(next);
                 }
             }
-            unsure = __any_sync(0xffffffffu, mine != mine);
             const unsigned groups = best_groups(mine, form.n_groups, form.top_groups, lane);
             const bool in = groups >> lane & 1;
-            const float worst = unordered(__reduce_min_sync(0xffffffffu, in ? ordered(mine) : 0xffffffffu));
-            const float next = unordered(__reduce_max_sync(0xffffffffu, in || lane >= form.n_groups ? ordered(-INFINITY) : ordered(mine)));
-            // (a sum's two scores + biases may cancel: what is hidden of them goes by the largest bias)
-            const float hidden = (4.0f + 4.0f * bias_most + 2.0f * fabsf(worst) + (next > -INFINITY ? 2.0f * fabsf(next) : 0.0f)) * HIDDEN;
-            if (form.top_groups < form.n_groups && !(worst - next > 2.0f * near + hidden)) unsure = true;
+            // (positive floats are in order as integers)
+            const float worst = __uint_as_float(__reduce_min_sync(0xffffffffu, in ? __float_as_uint(mine) : 0x7f800000u));
+            const float next = __uint_as_float(__reduce_max_sync(0xffffffffu, in || lane >= form.n_groups ? 0u : __float_as_uint(mine)));
+            if (form.top_groups < form.n_groups && !(worst - next > 2.0f * near + (worst + next) * HIDDEN)) unsure = true;
             if (whole) {
-                const bool open = groups >> ((unsigned)lane / (unsigned)lanes_per & 31u) & 1;
+                const bool open = groups >> my_group & 1;
 #pragma unroll
-                for (int i = 0; i < VPL; ++i) key[i] = open ? key[i] : 0u;
+                for (int i = 0; i < KEEP; ++i) best[i] = open ? best[i] : 0u;
             } else {
 #pragma unroll
                 for (int i = 0; i < VPL; ++i)
                     if (e0 + i < E && !(groups >> ((unsigned)(e0 + i) / (unsigned)per) & 1)) key[i] = 0u;
             }
         }
-        if (!whole) sort_keys<VPL>(key);
+        if (!whole) largest_keys<VPL, KEEP>(key, best);
         int my_expert = 0;
         float my_logit = 0.0f;
         if (!unsure) {
-            uint32_t my_key = 0;
-            auto take = [&](uint32_t& top) {                                   // the best expert left, out of the list; top 0: there is none
-                const uint32_t head = key[0] & ~INDEX;
-                top = __reduce_max_sync(0xffffffffu, head);
-                const int e = (int)__reduce_min_sync(0xffffffffu, head == top ? (unsigned)(e0 + (int)(INDEX - (key[0] & INDEX))) : 0xffffffffu);
-                const bool won = e >> BITS == lane;
+            const bool more = VPL > KEEP && best[KEEP - 1] != 0u;              // (there may be keys that were not kept)
+            // the n-th of the list is the best key left (and off it goes); returns it without its last bits, 0: there is none
+            auto take = [&](int n) {
+                const uint32_t head = best[0] & ~INDEX, top = __reduce_max_sync(0xffffffffu, head);
+                const bool equal = head == top;
+                const unsigned all = __ballot_sync(0xffffffffu, equal);
+                if (equal && !(all & below)) {                                 // of equal keys the lowest lane's: the lower expert
+                    s_list[warp][n] = make_uint2(best[0], lane);
 #pragma unroll
-                for (int i = 0; i + 1 < VPL; ++i) key[i] = won ? key[i + 1] : key[i];
-                key[VPL - 1] = won ? 0u : key[VPL - 1];
-                return e;
+                    for (int i = 0; i + 1 < KEEP; ++i) best[i] = best[i + 1];
+                    best[KEEP - 1] = 0u;
+                }
+                return top;
             };
+            uint32_t top = 0;
             for (int r = 0; r < top_k; ++r) {
-                uint32_t top;
-                const int e = take(top);
-                if (lane == r) { my_expert = e; my_key = top; }
+                top = take(r);
+                if (top == 0u) unsure = true;
             }
             // ... and those behind the last one that are as good as it, as far as these scores can tell
-            const float v_last = unordered(__shfl_sync(0xffffffffu, my_key, top_k - 1));
+            const float v_last = __uint_as_float(top), wide = near + v_last * HIDDEN;
             int n = top_k;
             for (; n < 32; ++n) {
-                uint32_t top;
-                const int e = take(top);
-                if (top == 0u || v_last - unordered(top) > near + fabsf(v_last) * HIDDEN) break;
-                if (lane == n) { my_expert = e; my_key = top; }
+                const uint32_t next = take(n);
+                if (v_last - __uint_as_float(next) > wide) break;
+                if (next == 0u) { unsure = n < E; break; }
             }
-            float my_bias = 0.0f;
+            if (n == 32 && top_k < E) unsure = true;                           // (more of them than lanes)
+            if (__any_sync(0xffffffffu, more && best[0] == 0u)) unsure = true;
+            __syncwarp();
+            float v = 0.0f, my_bias = 0.0f;
             if (lane < n) {
+                const uint2 chosen = s_list[warp][lane];
+                my_expert = min((int)chosen.y * VPL + (int)(INDEX - (chosen.x & INDEX)), E - 1);
+                v = __uint_as_float(chosen.x & ~INDEX);
                 my_logit = logit<L>(row[my_expert]);
                 my_bias = bias ? bias[my_expert] : 0.0f;
             }
             // sure of the order: every gap is wide, or the two are equal in logit and bias (the lower expert came first)
-            const float v = unordered(my_key), v_next = __shfl_down_sync(0xffffffffu, v, 1);
+            const float v_next = __shfl_down_sync(0xffffffffu, v, 1);
             const float l_next = __shfl_down_sync(0xffffffffu, my_logit, 1), b_next = __shfl_down_sync(0xffffffffu, my_bias, 1);
-            const bool same = my_logit == l_next && my_bias == b_next, gap = v - v_next > near + fabsf(v) * HIDDEN;
-            if (n == 32 && top_k < E) {
-                unsure = true;                                                 // (more of them than lanes)
-            } else if (!__all_sync(0xffffffffu, lane >= n - 1 || gap || same)) {
+            const bool same = my_logit == l_next && my_bias == b_next, gap = v - v_next > near + v * HIDDEN;
+            if (!unsure && !__all_sync(0xffffffffu, lane >= n - 1 || gap || same)) {
                 if (SOFTMAX && bias) {
                     unsure = true;
                 } else {
@@ -479,6 +517,7 @@ route_form_kernel(const L* __restrict__ logits, const float* __restrict__ bias, 
                     if (lane < top_k) my_logit = logit<L>(row[my_expert]);
                 }
             }
+            __syncwarp();
         }
         if (unsure) {
             my_expert = route_exact<VPL, L, SOFTMAX>(row, bias, E, top_k, form.n_groups, form.top_groups);
@@ -605,6 +644,44 @@ route_scan_kernel(int* __restrict__ hist, int n_ctas, int E, int* __restrict__ t
     if (lane == 0) totals[e] = carry;
 }
 
+// The same where there is much of it: a CTA takes 32 experts, a lane each, and a warp a 32nd of the histograms: their sums, where each warp begins,
+// then the running sums.  A warp for each expert reads 32 lines with every load: routing 32768 tokens to 256 experts 97 us so, 85 like this;
+// to 16 experts 23 and 30, 8192 tokens to 64 21 and 23 (a CTA or two do all of it).  From 2^16 counts on.
+__global__ void __launch_bounds__(1024)
+route_scan_wide_kernel(int* __restrict__ hist, int n_ctas, int E, int* __restrict__ totals) {
+    pdl_wait();
+    pdl_trigger();
+    __shared__ int s_sum[32][33];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, e = blockIdx.x * 32 + lane;
+    const int first = (int)((int64_t)n_ctas * warp / 32), last = (int)((int64_t)n_ctas * (warp + 1) / 32);
+    int sum = 0;
+    if (e < E) {
+#pragma unroll 8
+        for (int b = first; b < last; ++b) sum += hist[(int64_t)b * E + e];
+    }
+    s_sum[warp][lane] = sum;
+    __syncthreads();
+    int carry = 0, all = 0;
+#pragma unroll
+    for (int w = 0; w < 32; ++w) {
+        const int v = s_sum[w][lane];
+        carry += w < warp ? v : 0;
+        all += v;
+    }
+    if (e >= E) return;
+    for (int b0 = first; b0 < last; b0 += 8) {               // eight histograms in flight
+        int v[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) v[u] = b0 + u < last ? hist[(int64_t)(b0 + u) * E + e] : 0;
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+            if (b0 + u < last) hist[(int64_t)(b0 + u) * E + e] = carry;
+            carry += v[u];
+        }
+    }
+    if (warp == 0) totals[e] = all;
+}
+
 // totals: per-expert counts from route_scan_kernel, with `hist` turned into offsets; null: hist still holds counts
 __global__ void __launch_bounds__(256)
 route_scatter_kernel(const int* __restrict__ top_experts, const float* __restrict__ top_gates, const int* __restrict__ hist,
@@ -707,6 +784,19 @@ route_scatter_kernel(const int* __restrict__ top_experts, const float* __restric
     }
 }
 
+// Tokens per CTA of the other forms: CTAs of 256 threads that are all resident at once (five per SM up to 256 experts, two beyond), so that none
+// waits for a second turn; full turns of them for more tokens.
+static inline int form_tokens_per_cta(int64_t T, int E) {
+    const int64_t slots = (E <= 256 ? 5 : 2) * (int64_t)sm_count();
+    const int64_t turns = (T + slots * ROUTE_MAX_TOKENS_PER_CTA - 1) / (slots * ROUTE_MAX_TOKENS_PER_CTA);
+    const int64_t ctas = slots * (turns < 1 ? 1 : turns), per = ((T + ctas - 1) / ctas + 7) / 8 * 8;
+    return (int)(per < 8 ? 8 : per);
+}
+int64_t moe_route_form_workspace_ints(int64_t T, int E) {
+    const int per = form_tokens_per_cta(T, E);
+    return ((T + per - 1) / per) * (int64_t)E + E;
+}
+
 int64_t moe_route_workspace_ints(int64_t T, int E) {
     const int per = route_tokens_per_cta(T, E);
     return ((T + per - 1) / per) * (int64_t)E + E;
@@ -784,7 +874,7 @@ static int moe_route(const void* logits, int logits_dtype, const float* bias, in
     }
     CINN_CHECK_ARG(logits && (bias || form) && workspace && top_experts && top_gates && token_indices && sorted_scores &&
                    sorted_experts && pair_pos && pair_gate, "moe_route: null pointer");
-    const int per = route_tokens_per_cta(T, E), n_ctas = (int)((T + per - 1) / per);
+    const int per = form ? form_tokens_per_cta(T, E) : route_tokens_per_cta(T, E), n_ctas = (int)((T + per - 1) / per);
     int* hist = workspace;
     int* totals = n_ctas > ROUTE_FEW_CTAS ? workspace + (int64_t)n_ctas * E : nullptr;
     if (form) {
@@ -796,7 +886,8 @@ static int moe_route(const void* logits, int logits_dtype, const float* bias, in
     else launch_topk((const __half*)logits, bias, (int)T, E, top_k, per, n_ctas, top_experts, top_gates, hist, st);
     CINN_CHECK_LAUNCH();
     if (totals) {
-        launch_dependent(route_scan_kernel, dim3((E + 7) / 8), dim3(256), 0, st, hist, n_ctas, E, totals);
+        if ((int64_t)n_ctas * E > 1 << 16) launch_dependent(route_scan_wide_kernel, dim3((E + 31) / 32), dim3(1024), 0, st, hist, n_ctas, E, totals);
+        else launch_dependent(route_scan_kernel, dim3((E + 7) / 8), dim3(256), 0, st, hist, n_ctas, E, totals);
         CINN_CHECK_LAUNCH();
     }
     launch_dependent(route_scatter_kernel, dim3(n_ctas), dim3(256), 0, st, top_experts, top_gates, hist, totals, (int)T, E, top_k, per, token_indices, sorted_scores,

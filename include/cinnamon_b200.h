@@ -526,9 +526,11 @@ int cinn_moe_route_ranges(const void* logits, int logits_dtype, const float* bia
  * 32) of equally many neighbours; those top_groups whose two largest scores + bias have the largest sums are open, and the top_k
  * experts with the largest score + bias are chosen out of them, by falling score + bias; ties go to the lower id, a NaN comes last, and no expert
  * is chosen twice.  The choice is that of 64-bit arithmetic.  Gates: scale * score / (sum of the chosen scores + 1e-9), or with
- * renormalise 0 scale * score.  bias: NULL = none.  No counterpart in the reference, whose router has one form.
+ * renormalise 0 scale * score.  bias: NULL = none.  workspace: cinn_moe_route_form_workspace_ints ints.
+ * No counterpart in the reference, whose router has one form.
  * cinn_moe_route_form_backward: d_logits (n_tokens, n_experts) of logits' type from the gradients of top_gates, pair_gate and
  * sorted_scores (NULL: none), for the experts that were chosen; sorted_experts and pair_pos are read for the last two only. */
+int64_t cinn_moe_route_form_workspace_ints(int64_t n_tokens, int n_experts);
 int cinn_moe_route_form(const void* logits, int logits_dtype, const float* bias, int64_t n_tokens, int n_experts, int top_k, int scores,
                         int n_groups, int top_groups, int renormalise, float scale, int* workspace, int* top_experts, float* top_gates,
                         int64_t* token_indices, float* sorted_scores, int64_t* sorted_experts, int64_t* counts, int64_t* starts, int64_t* ends,
