@@ -857,6 +857,8 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, target: torch.Te
     that count (NaN where there are none), "sum", or "none": the tokens' losses, of ``target``'s shape.  The loss is fp32; products
     are summed in fp32, and the logits' gradient is rounded to the operands' type before the two products that follow."""
     assert reduction in _REDUCTIONS, "reduction must be 'none', 'mean' or 'sum'"
+    if _ops is not None and torch.compiler.is_compiling():
+        return _ops.linear_cross_entropy(x, weight, target, int(ignore_index), _REDUCTIONS[reduction])
     return _host.linear_cross_entropy(x, weight, target, int(ignore_index), _REDUCTIONS[reduction])
 
 
@@ -903,6 +905,8 @@ def rotary(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, inv_freq: 
     inv_freq.numel()), and becomes ``magnitude`` (a cos t - b sin t, b cos t + a sin t) with t = position ``* inv_freq[i]``.
     ``positions`` (L,) or (batch, L), int64 or int32, any values; ``inv_freq`` as from ``rotary_frequencies``.  The angles of far positions
     are exact; products are fp32, rounded once."""
+    if _ops is not None and torch.compiler.is_compiling():
+        return _ops.rotary(q, k, positions, inv_freq, bool(interleaved), int(start), float(magnitude))
     return _host.rotary(q, k, positions, inv_freq, bool(interleaved), int(start), float(magnitude), False)
 
 

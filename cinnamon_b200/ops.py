@@ -3,16 +3,18 @@
 The reference compiles its model (``torch.compile(model)``, src/train.py:703) and its Triton kernels are traced as
 part of the graph.  This library's kernels are reached through ctypes, which a tracing compiler cannot look into: an
 ``autograd.Function`` whose forward calls ctypes makes dynamo break the graph at every FP8 layer.  The operators
-below wrap forward and backward of the three differentiable entry points as opaque nodes with shape functions
+below wrap forward and backward of the differentiable entry points as opaque nodes with shape functions
 (``register_fake``) and autograd formulas (``register_autograd``):
 
   cinnamon_b200::fp8_linear_fwd / fp8_linear_bwd      FP8MatmulFunction   (src/kernels.py:731-794)
   cinnamon_b200::grouped_gemm_fwd / grouped_gemm_bwd  moe_grouped_gemm    (src/kernels.py:526-581; differentiable here)
   cinnamon_b200::sparse_attn_fwd / sparse_attn_bwd    SparseAttentionFunction (src/kernels.py:1189-1289)
+  cinnamon_b200::linear_ce_fwd / linear_ce_bwd        linear_cross_entropy
+  cinnamon_b200::rotate                               rotary (its derivative is itself, the other way round)
 
 Each operator body runs the very code of the eager ``autograd.Function`` (its ``forward`` / ``backward`` static
 methods, handed a stand-in context), so compiled and eager results are the same bits.  ``FP8Linear.forward``,
-``moe_grouped_gemm`` and ``sparse_attention`` switch to the operators while ``torch.compiler.is_compiling()``; in
+``moe_grouped_gemm``, ``sparse_attention``, ``linear_cross_entropy`` and ``rotary`` switch to the operators while ``torch.compiler.is_compiling()``; in
 eager mode they keep calling the autograd functions directly, as the reference does.
 """
 from __future__ import annotations
@@ -246,3 +248,98 @@ sparse_attn_fwd.register_autograd(_attn_backward, setup_context=_attn_setup)
 def sparse_attention(q: Tensor, k: Tensor, v: Tensor, idx: Tensor, scale: float):
     out, attn, _, _ = torch.ops.cinnamon_b200.sparse_attn_fwd(q, k, v, idx, float(scale))
     return out, attn
+
+
+# ---------------------------------------------------------------------------------------------------------------
+# output projection + cross entropy
+# ---------------------------------------------------------------------------------------------------------------
+def _up(n, a: int):
+    return (n + a - 1) // a * a
+
+
+@torch.library.custom_op("cinnamon_b200::linear_ce_fwd", mutates_args=(), device_types="cuda")
+def linear_ce_fwd(x: Tensor, weight: Tensor, target: Tensor, ignore_index: int, reduction: int) -> Tuple[Tensor, Tensor]:
+    return K._host.linear_ce_forward(x, weight, target, ignore_index, reduction)
+
+
+@linear_ce_fwd.register_fake
+def _(x, weight, target, ignore_index, reduction):
+    T = x.shape[0]
+    state = 256 + 3 * _up(4 * T, 256) + _up(8 * T, 256) if T else 0                # cinn_linear_ce_state_bytes
+    return (torch.empty(() if reduction else (T,), dtype=torch.float32, device=x.device), torch.empty((state,), dtype=torch.uint8, device=x.device))
+
+
+@torch.library.custom_op("cinnamon_b200::linear_ce_bwd", mutates_args=(), device_types="cuda")
+def linear_ce_bwd(grad: Tensor, x: Tensor, weight: Tensor, state: Tensor, reduction: int) -> Tuple[Tensor, Tensor]:
+    return K._host.linear_ce_backward(grad, x, weight, state, reduction, True, True)
+
+
+@linear_ce_bwd.register_fake
+def _(grad, x, weight, state, reduction):
+    return (torch.empty(x.shape, dtype=x.dtype, device=x.device), torch.empty(weight.shape, dtype=weight.dtype, device=x.device))
+
+
+def _ce_setup(ctx, inputs, output):
+    x, weight, _, _, ctx.reduction = inputs
+    ctx.save_for_backward(x, weight, output[1])
+    ctx.set_materialize_grads(False)
+
+
+def _ce_backward(ctx, grad, *ignored):
+    if grad is None:
+        return None, None, None, None, None
+    gx, gw = torch.ops.cinnamon_b200.linear_ce_bwd(grad, *ctx.saved_tensors, ctx.reduction)
+    return gx, gw, None, None, None
+
+
+linear_ce_fwd.register_autograd(_ce_backward, setup_context=_ce_setup)
+
+
+def linear_cross_entropy(x: Tensor, weight: Tensor, target: Tensor, ignore_index: int, reduction: int) -> Tensor:
+    """The operands as the native call makes them (csrc/host/loss.cpp), in operations that can be traced; its checks of shapes and types are
+    the operators' own."""
+    flat = x.reshape(-1, x.shape[-1])
+    if torch.is_autocast_enabled("cuda"):
+        dtype = torch.get_autocast_dtype("cuda")
+        flat, weight = flat.to(dtype), weight.to(dtype)
+    odd = flat.shape[1] % 8
+    if odd:
+        flat, weight = (torch.nn.functional.pad(t, (0, 8 - odd)) for t in (flat, weight))
+    assert target.shape == x.shape[:-1] and weight.dim() == 2 and weight.shape[1] == flat.shape[1], "linear_cross_entropy: shapes"
+    assert flat.dtype == weight.dtype and flat.dtype in (torch.bfloat16, torch.float16), \
+        "linear_cross_entropy multiplies 16-bit operands: x and weight must both be bfloat16 or both float16 (or autocast must make them so)"
+    loss = torch.ops.cinnamon_b200.linear_ce_fwd(flat, weight, target.reshape(-1).long(), ignore_index, reduction)[0]
+    return loss if reduction else loss.view(target.shape)
+
+
+# ---------------------------------------------------------------------------------------------------------------
+# rotary positions
+# ---------------------------------------------------------------------------------------------------------------
+@torch.library.custom_op("cinnamon_b200::rotate", mutates_args=(), device_types="cuda")
+def rotate(tensors: List[Tensor], positions: Tensor, inv_freq: Tensor, interleaved: bool, start: int, magnitude: float, inverse: bool) -> List[Tensor]:
+    q, k = tensors if len(tensors) == 2 else (tensors[0], None)
+    out = K._host.rotary(q.detach(), None if k is None else k.detach(), positions, inv_freq, interleaved, start, magnitude, inverse)
+    return [t for t in out if t is not None]
+
+
+@rotate.register_fake
+def _(tensors, positions, inv_freq, interleaved, start, magnitude, inverse):
+    return [torch.empty_like(t if t.stride(-1) == 1 else t.contiguous()) for t in tensors]
+
+
+def _rotate_setup(ctx, inputs, output):
+    _, positions, inv_freq, ctx.interleaved, ctx.start, ctx.magnitude, ctx.inverse = inputs
+    ctx.save_for_backward(positions, inv_freq)
+
+
+def _rotate_backward(ctx, grads):
+    out = torch.ops.cinnamon_b200.rotate(list(grads), *ctx.saved_tensors, ctx.interleaved, ctx.start, ctx.magnitude, not ctx.inverse)
+    return out, None, None, None, None, None, None
+
+
+rotate.register_autograd(_rotate_backward, setup_context=_rotate_setup)
+
+
+def rotary(q, k, positions, inv_freq, interleaved, start, magnitude):
+    out = torch.ops.cinnamon_b200.rotate([q] if k is None else [q, k], positions, inv_freq, interleaved, start, magnitude, False)
+    return out[0], None if k is None else out[1]

@@ -1,0 +1,165 @@
+"""The operators around the framework's layers, together as a training step uses them: rotary positions in front of sparse attention, a
+router of groups in the MoE block, and the head's cross entropy; and the same under torch.compile.
+
+The step through autograd against the step taken apart, every operator called by itself with the gradient that comes back to it: the same bits,
+except behind sparse attention's keys and values, whose gradients are sums in no fixed order."""
+import pytest
+import torch
+import torch.nn as nn
+
+pytestmark = pytest.mark.gpu
+
+
+class Step(nn.Module):
+    def __init__(self, d=256, heads=4, d_head=96, rot=32, vocab=1000):
+        super().__init__()
+        from cinnamon_b200 import kernels as K, layers, moe
+        self.K, self.heads, self.rot = K, heads, rot
+        self.q = nn.Linear(d, heads * d_head, bias=False)
+        self.k = nn.Linear(d, heads * d_head, bias=False)
+        self.v = nn.Linear(d, heads * 64, bias=False)
+        self.o = nn.Linear(heads * 64, d, bias=False)
+        form = moe.RouterForm(scores="softmax", n_groups=4, top_groups=2, scale=2.0)
+        self.moe = layers.MoE(16, 1, 4, d, 512, 2, 0.001, router_form=form)
+        K.convert_to_fp8(self.moe)
+        self.head = nn.Linear(d, vocab, bias=False)
+        freq, self.magnitude = K.rotary_frequencies(rot, scaling="yarn", factor=4.0, original_len=512)
+        self.register_buffer("inv_freq", freq)
+
+    def split(self, t):
+        return t.unflatten(-1, (self.heads, -1)).transpose(1, 2)
+
+    def project(self, x):
+        return self.split(self.q(x)), self.split(self.k(x)), self.split(self.v(x))
+
+    def rotate(self, q, k, positions):
+        return self.K.rotary(q, k, positions, self.inv_freq, start=-self.rot, magnitude=self.magnitude)
+
+    def attend(self, q, k, v, idx):
+        return self.K.sparse_attention(q, k, v, idx)[0].transpose(1, 2).flatten(2)
+
+    def mix(self, x, a):
+        h = x + self.o(a)
+        return h + self.moe(h)[0]
+
+    def loss(self, h, target):
+        return self.K.linear_cross_entropy(h, self.head.weight, target)
+
+    def forward(self, x, positions, idx, target):
+        q, k, v = self.project(x)
+        q, k = self.rotate(q, k, positions)
+        return self.loss(self.mix(x, self.attend(q, k, v, idx)), target)
+
+
+def _data(d=256, vocab=1000, B=2, L=100, picks=24):
+    g = torch.Generator().manual_seed(4)
+    x = torch.randn(B, L, d, generator=g).cuda()
+    idx = (torch.rand(B, L, picks, generator=g) * (torch.arange(L).view(1, L, 1) + 1)).long().cuda()
+    target = torch.randint(0, vocab, (B, L), generator=g)
+    target[0, :30], target[1, -9:] = -100, -100                        # a prompt, and padding
+    positions = torch.arange(L) + torch.tensor([[0], [70000]])
+    return x, positions.cuda(), idx, target.cuda()
+
+
+def _close(a, b, what):
+    assert (a.float() - b.float()).norm() <= 2e-2 * b.float().norm(), what
+
+
+def test_step_is_its_operators():
+    torch.manual_seed(1)
+    step = Step().cuda().eval()
+    x, positions, idx, target = _data()
+    x.requires_grad_(True)
+    params = dict(step.named_parameters())
+    with torch.autocast("cuda", dtype=torch.bfloat16):
+        loss = step(x, positions, idx, target)
+    grads = dict(zip(["x", *params], torch.autograd.grad(loss, [x, *params.values()])))
+
+    leaf = lambda t: t.detach().requires_grad_(True)                    # noqa: E731
+    with torch.autocast("cuda", dtype=torch.bfloat16):
+        parts = [leaf(t) for t in step.project(x)]
+        turned = step.rotate(parts[0], parts[1], positions)
+        q, k, v = leaf(turned[0]), leaf(turned[1]), parts[2]
+        a = step.attend(q, k, v, idx)
+        la = leaf(a)
+        h = step.mix(x, la)
+        lh = leaf(h)
+        again = step.loss(lh, target)
+    assert torch.equal(again, loss)
+    gh, g_head = torch.autograd.grad(again, [lh, params["head.weight"]])
+    assert torch.equal(g_head, grads["head.weight"])
+    assert (gh[0, :30] == 0).all() and (gh[1, -9:] == 0).all() and (gh[0, 30:] != 0).any(-1).all()
+    inner = [n for n in params if n.startswith(("moe.", "o."))]
+    back = torch.autograd.grad(h, [la, *(params[n] for n in inner)], gh)
+    for n, g in zip(inner, back[1:]):
+        assert torch.equal(g, grads[n]), n
+    gq, gk, gv = torch.autograd.grad(a, [q, k, v], back[0])
+    dq, dk = torch.autograd.grad(turned, parts[:2], [gq, gk])
+    with torch.autocast("cuda", dtype=torch.bfloat16):
+        projected = step.project(x)
+    weights = torch.autograd.grad(projected, [params["q.weight"], params["k.weight"], params["v.weight"]], [dq, dk, gv])
+    for n, g in zip(("q.weight", "k.weight", "v.weight"), weights):
+        _close(g, grads[n], n)
+    assert all(torch.isfinite(g).all() and g.abs().sum() > 0 for g in grads.values())
+    assert step.K.device_status() == 0
+
+
+def test_step_captured_and_replayed():
+    torch.manual_seed(2)
+    step = Step().cuda().eval()
+    x, positions, idx, target = _data()
+    params = list(step.parameters())
+
+    def run():
+        with torch.autocast("cuda", dtype=torch.bfloat16, cache_enabled=False):
+            loss = step(x, positions, idx, target)
+        return [loss.detach(), *torch.autograd.grad(loss, params)]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            run()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            out = run()
+    torch.cuda.current_stream().wait_stream(side)
+    x2, _, _, target2 = _data()
+    with torch.no_grad():
+        x.copy_(x2.flip(0)), target.copy_(target2.flip(0)), positions.copy_(positions.flip(0))
+    graph.replay()
+    torch.cuda.synchronize()
+    want = run()
+    assert torch.equal(out[0], want[0])
+    for a, b, (name, _) in zip(out[1:], want[1:], step.named_parameters()):
+        _close(a, b, name)
+
+
+def test_cross_entropy_and_rotary_compile_as_one_graph():
+    from cinnamon_b200 import kernels as K
+    g = torch.Generator().manual_seed(3)
+    x, w = torch.randn(2, 40, 100, generator=g).cuda(), (torch.randn(300, 100, generator=g) * 0.1).cuda()
+    target = torch.randint(0, 300, (2, 40), generator=g).cuda()
+    target[0, :7] = -100
+    q, k = (torch.randn(2, h, 40, 64, generator=g).bfloat16().cuda() for h in (4, 1))
+    freq, _ = K.rotary_frequencies(32, device="cuda")
+    positions = torch.arange(40, device="cuda") + 1000
+
+    def head(x, w):
+        return K.linear_cross_entropy(x, w, target), K.linear_cross_entropy(x, w, target, reduction="none")
+
+    def turn(q, k):
+        return K.rotary(q, k, positions, freq, interleaved=True, start=16, magnitude=1.5)
+
+    results = []
+    for compiled in (False, True):
+        torch._dynamo.reset()
+        f, r = (torch.compile(head, fullgraph=True), torch.compile(turn, fullgraph=True)) if compiled else (head, turn)
+        leaves = [t.clone().requires_grad_(True) for t in (x, w, q, k)]
+        with torch.autocast("cuda", dtype=torch.bfloat16):
+            mean, each = f(*leaves[:2])
+        oq, ok = r(*leaves[2:])
+        grads = torch.autograd.grad([mean, each, oq, ok], leaves, [torch.ones_like(mean), each.detach(), q, k])
+        results.append([mean.detach(), each.detach(), oq.detach(), ok.detach(), *grads])
+    for a, b in zip(*results):
+        assert a.shape == b.shape and torch.equal(a, b)
