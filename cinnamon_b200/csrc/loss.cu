@@ -33,15 +33,17 @@ enum Mode { STATS = 0, SOFT = 1, DX = 2, DW = 3 };
 
 constexpr int M = 256, N = 256;            // the pair's tile
 constexpr int KE = 64;                     // elements of a K block: 128 bytes
-constexpr int STAGES = 4;
 constexpr int SIDE = 128 * 128;            // bytes of one operand's stage in one CTA: 128 rows (or columns) x 64 elements
 constexpr int EPI = 8, COLS = 128;         // epilogue warps: four lane quarters x two halves of the columns
 constexpr int W_TMA = EPI, W_MMA = EPI + 1;
 constexpr int THREADS = (EPI + 2) * 32;
-constexpr int BOX = 32 * 128;              // a TMA-store box: 32 rows of 128 bytes; two per epilogue warp, filled in turn
-constexpr int STAGE_BYTES = STAGES * 2 * SIDE;
-constexpr int C_BYTES = EPI * 2 * BOX;
-constexpr size_t SMEM_STATS = (size_t)STAGE_BYTES + 256 + 1024, SMEM = SMEM_STATS + C_BYTES;
+constexpr int BOX = 32 * 128;              // a TMA-store box: 32 rows of 128 bytes
+// The operands' ring takes what shared memory there is: with four stages the logits' product waited for operands 1800 of a tile's 4600 cycles, and
+// where dz is written to memory at the same time 3900 of 6100.
+constexpr int STAGES_Z = 7;                // product_kernel, which stores from registers
+constexpr int STAGES_G = 5, BOXES = 2;     // grads_kernel; boxes of an epilogue warp, filled in turn
+constexpr int C_BYTES = EPI * BOXES * BOX;
+constexpr size_t SMEM_Z = (size_t)STAGES_Z * 2 * SIDE + 256 + 1024, SMEM_G = (size_t)STAGES_G * 2 * SIDE + C_BYTES + 256 + 1024;
 constexpr int GROUP = 16;                  // tiles of tokens that meet a run of words before the next ones do (L2)
 constexpr int SCAN = 1024;                 // tokens per CTA of the passes that gather
 constexpr float LOG2E = 1.4426950408889634f;
@@ -65,6 +67,8 @@ struct Params {
     const float* grad;                     // the loss's gradient: one number, or one per token
     const unsigned* grad_max;              // the bits of the largest |gradient| (reduction "none")
     int mean;
+    uint16_t* dz;                          // the piece's, rows of dz_ld (a multiple of 64)
+    int dz_ld;
 };
 
 __device__ __forceinline__ bool wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, int code) {
@@ -187,8 +191,9 @@ __device__ __forceinline__ Unit unit_at(const Params& p, int valid, int u) {
     const int in = u - g * GROUP * across, n = in / size;
     r.m0 = (first + in - n * size) * M;
     if constexpr (MODE == STATS) {
-        r.n_first = (int)((int64_t)n_tiles * n / p.parts);
-        r.n_last = (int)((int64_t)n_tiles * (n + 1) / p.parts);
+        const int run = (n_tiles + p.parts - 1) / p.parts;             // (all of one length but the last)
+        r.n_first = n * run;
+        r.n_last = min(r.n_first + run, n_tiles);
     } else {
         r.n_first = n; r.n_last = n + 1;
     }
@@ -230,8 +235,13 @@ struct Schedule {
     }
 };
 
+__device__ __forceinline__ void store32(uint16_t* at, const uint32_t* v) {             // 32 bytes
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(at), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]),
+                 "r"(v[6]), "r"(v[7]) : "memory");
+}
+
 // What every product kernel sets up: barriers, tensor memory, the roles' view of both.
-template <int SMEM_C>
+template <int STAGES, int SMEM_C>
 struct Setup {
     uint8_t *smem_a, *smem_b, *c_stage;
     volatile int* abort_flag;
@@ -242,7 +252,7 @@ struct Setup {
         uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
         smem_a = smem;
         smem_b = smem + STAGES * SIDE;
-        c_stage = smem + STAGE_BYTES;
+        c_stage = smem + STAGES * 2 * SIDE;
         uint64_t* bars = reinterpret_cast<uint64_t*>(c_stage + SMEM_C);
         // [0, S) full (used in the leader), [S, 2S) empty, then: tensor memory full (2), empty (2, leader)
         uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * STAGES + 4);
@@ -301,22 +311,22 @@ struct Boxes {
     uint32_t slot, turn = 0;
     __device__ __forceinline__ Boxes(uint32_t s) : slot(s) {}
     __device__ __forceinline__ uint32_t open(int lane) {
-        if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
+        if (lane == 0) asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(BOXES - 1) : "memory");
         __syncwarp();
-        return slot + (turn & 1) * BOX;
+        return slot + turn * BOX;
     }
     __device__ __forceinline__ void send(int lane, const CUtensorMap* map, int col, int row, bool store, bool add) {
         fence_async_smem();
         __syncwarp();
         if (lane == 0) {
-            const uint32_t box = slot + (turn & 1) * BOX;
+            const uint32_t box = slot + turn * BOX;
             if (store) {
                 if (add) add_2d(map, box, col, row);
                 else tma_store_2d(map, box, col, row);
             }
             tma_store_commit();
         }
-        ++turn;
+        turn = turn + 1 == BOXES ? 0 : turn + 1;
     }
     __device__ __forceinline__ void drain(int lane) { if (lane == 0) tma_store_wait_all(); }
 };
@@ -331,9 +341,10 @@ __device__ __forceinline__ uint64_t pair2(float a, float b) {
 template <int MODE, bool BF16>
 __global__ void __launch_bounds__(THREADS, 1)
 product_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b, const __grid_constant__ CUtensorMap tm_xg,
-               const __grid_constant__ CUtensorMap tm_c, const Params p) {
+               const Params p) {
+    constexpr int STAGES = STAGES_Z;
     extern __shared__ uint8_t smem_raw[];
-    Setup<MODE == STATS ? 0 : C_BYTES> s(smem_raw);
+    Setup<STAGES, 0> s(smem_raw);
     const int warp = s.warp, lane = s.lane, rank = (int)s.rank;
     const int valid = *p.n_valid;
     const int n_units = unit_count<MODE>(p, valid);
@@ -393,7 +404,6 @@ product_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__
         // ------------------------------ epilogue (both CTAs) ------------------------------
         const int q = warp & 3, h = warp >> 2;
         const uint32_t tempty_leader = mapa(s.tempty0, 0);
-        Boxes boxes(smem_u32(s.c_stage) + warp * 2 * BOX);
         uint32_t tile = 0;
         bool alive = true;
         float most = 0.0f;                                 // SOFT, gradients per token: the largest
@@ -455,7 +465,6 @@ product_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__
                     __syncwarp();
                     if (lane == 0) arrive_remote(tempty_leader + 8 * b);
                 } else {
-                    uint32_t box = 0;
                     const uint64_t minus = pair2(-mx, -mx), scale = pair2(LOG2E, LOG2E), logs = pair2(-sum, -sum), rels = pair2(rel, rel);
                     uint32_t r[2][32];                     // a chunk of 32 words at work, the next one on its way
                     ld32(taddr, r[0]);
@@ -468,7 +477,6 @@ product_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__
                             __syncwarp();
                             if (lane == 0) arrive_remote(tempty_leader + 8 * b);       // all of the tile is in registers
                         }
-                        if ((c & 1) == 0) box = boxes.open(lane);
                         uint32_t(&z)[32] = r[c & 1];
                         const int hit = target - (col0 + c * 32), left = p.v0 + p.vc - (col0 + c * 32);      // words of the piece from here on
                         // two at a time: e^(z - lse), rounded once in the difference and once with the logarithm of the sum
@@ -499,16 +507,14 @@ product_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__
                             for (int j = 0; j < 32; ++j)
                                 if (!live || j >= left) z[j] = 0u;
                         }
+                        // A lane's 64 bytes as two whole sectors.  (dz has rows for whole tiles, and zeros in its last columns.)
+                        const int col = nt * N + h * COLS + c * 32;
+                        if (col < p.dz_ld) {
+                            uint32_t v[16];
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) {      // 16 bytes: 8 elements
-                            uint32_t v[4];
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) v[i] = pack2<BF16>(__uint_as_float(z[j * 8 + 2 * i]), __uint_as_float(z[j * 8 + 2 * i + 1]));
-                            stage16(box, lane, (c & 1) * 4 + j, v[0], v[1], v[2], v[3]);
-                        }
-                        if (c & 1) {
-                            const int col = nt * N + h * COLS + (c >> 1) * 64;
-                            boxes.send(lane, &tm_c, col, row - lane, col < p.vc, false);
+                            for (int j = 0; j < 16; ++j) v[j] = pack2<BF16>(__uint_as_float(z[2 * j]), __uint_as_float(z[2 * j + 1]));
+                            store32(p.dz + (int64_t)row * p.dz_ld + col, v);
+                            store32(p.dz + (int64_t)row * p.dz_ld + col + 16, v + 8);
                         }
                     }
                 }
@@ -521,7 +527,6 @@ product_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__
                 if (alive && live) p.part[(int64_t)(n * 2 + h) * p.part_ld + row] = make_float2(mx, sum);
             }
         }
-        if constexpr (MODE == SOFT) boxes.drain(lane);
     }
     s.finish();
 }
@@ -534,8 +539,9 @@ struct GradMaps { CUtensorMap z_rows, z_cols, w_cols, x_cols, xg_cols, c_dx, c_d
 template <bool BF16, bool DW_SUMS>
 __global__ void __launch_bounds__(THREADS, 1)
 grads_kernel(const __grid_constant__ GradMaps maps, const Params p) {
+    constexpr int STAGES = STAGES_G;
     extern __shared__ uint8_t smem_raw[];
-    Setup<C_BYTES> s(smem_raw);
+    Setup<STAGES, C_BYTES> s(smem_raw);
     const int warp = s.warp, lane = s.lane, rank = (int)s.rank;
     const int valid = *p.n_valid;
     const Schedule plan(p, valid, blockIdx.x >> 1, gridDim.x >> 1);
@@ -605,7 +611,7 @@ grads_kernel(const __grid_constant__ GradMaps maps, const Params p) {
         // ------------------------------ epilogue (both CTAs) ------------------------------
         const int q = warp & 3, h = warp >> 2;
         const uint32_t tempty_leader = mapa(s.tempty0, 0);
-        Boxes boxes(smem_u32(s.c_stage) + warp * 2 * BOX);
+        Boxes boxes(smem_u32(s.c_stage) + warp * BOXES * BOX);
         const float scale = DW_SUMS ? 1.0f : final_scale(p, BF16);
         for (int i = 0; plan.at(i, dx, u); ++i) {
             const Unit w = dx ? unit_at<DX>(p, valid, u) : unit_at<DW>(p, valid, u);
@@ -910,6 +916,7 @@ struct Plan {
     int64_t dz_ld;
 };
 
+constexpr int64_t PART_BYTES = 48LL << 20;
 constexpr int64_t DZ_BYTES = 512LL << 20;  // most of a piece of dz: smaller pieces cost passes over dx, larger ones only memory
 
 static Plan make_plan(int64_t T, int64_t V, int64_t d) {
@@ -917,8 +924,8 @@ static Plan make_plan(int64_t T, int64_t V, int64_t d) {
     r.T = T; r.V = V; r.d = d; r.Tp = up(T, M);
     r.clusters = std::max(1, sm_count() / 2);          // (not those under a cap: sizes must not change between two calls)
     const int64_t m_tiles = r.Tp / M, n_tiles = ceil_div(V, N), n_d = ceil_div(d, N);
-    // runs of words: as long as leaves every cluster some sixteen of them, for an even end
-    r.parts = (int)std::min<int64_t>(n_tiles, std::max<int64_t>(ceil_div(n_tiles, 16), ceil_div(16 * r.clusters, m_tiles)));
+    // runs of words: one tile each, for an even end, unless what they leave per token is more than PART_BYTES
+    r.parts = (int)ceil_div(n_tiles, ceil_div(16 * n_tiles * r.Tp, PART_BYTES));
     const int64_t fit = std::max<int64_t>(N, DZ_BYTES / (2 * r.Tp) / N * N);
     r.pieces = (int)ceil_div(V, fit);
     r.vc = up(ceil_div(V, r.pieces), N);   // equal pieces, in whole tiles
@@ -1043,7 +1050,7 @@ static int forward(const void* x, int64_t ldx, const void* w, int64_t ldw, const
     Params p{};
     p.n_valid = s.n_valid; p.T = (int)r.T; p.V = (int)r.V; p.d = (int)r.d; p.parts = r.parts;
     p.part = f.part; p.part_ld = r.Tp; p.target_logit = f.target_logit; p.target = s.target;
-    if ((rc = launch<product_kernel<STATS, BF16>, SMEM_STATS>(st, ta, tb, tx, ta, p))) return rc;
+    if ((rc = launch<product_kernel<STATS, BF16>, SMEM_Z>(st, ta, tb, tx, p))) return rc;
     launch_dependent(loss_kernel, dim3((unsigned)ceil_div(r.T, 32)), dim3(32 * JOIN), 0, st, f.part, r.Tp, 2 * r.parts, f.target_logit, s, (int)r.T,
                      reduction, f.block_sum, loss);
     CINN_CHECK_LAUNCH();
@@ -1082,18 +1089,17 @@ static int backward(const void* x, int64_t ldx, const void* w, int64_t ldw, cons
         else rc = map16(&g.c_dw, dw, r.d, r.V, r.d, 32, BF16);
         if (rc) return rc;
     }
+    p.dz = static_cast<uint16_t*>(b.dz); p.dz_ld = (int)r.dz_ld;
     p.dx_splits = dx ? r.dx_splits : 0; p.dx_rows = (int)r.Tp;
     p.dw_splits = dw ? r.dw_splits : 0; p.dw_rows = (int)up(r.V, M);
     for (int i = 0; i < r.pieces; ++i) {
         p.v0 = (int)(i * r.vc);
         p.vc = (int)std::min<int64_t>(r.vc, r.V - p.v0);
         p.add = i > 0;
-        CUtensorMap z_store;
-        if ((rc = map16(&z_store, b.dz, p.vc, r.Tp, r.dz_ld, 32, BF16))) return rc;
         if ((rc = map16(&g.z_rows, b.dz, p.vc, r.Tp, r.dz_ld, 128, BF16))) return rc;
         if ((rc = map16(&g.z_cols, b.dz, p.vc, r.Tp, r.dz_ld, 64, BF16))) return rc;
-        if ((rc = launch<product_kernel<SOFT, BF16>, SMEM>(st, x_rows, w_rows, xg_rows, z_store, p))) return rc;
-        rc = r.dw_splits > 1 ? launch<grads_kernel<BF16, true>, SMEM>(st, g, p) : launch<grads_kernel<BF16, false>, SMEM>(st, g, p);
+        if ((rc = launch<product_kernel<SOFT, BF16>, SMEM_Z>(st, x_rows, w_rows, xg_rows, p))) return rc;
+        rc = r.dw_splits > 1 ? launch<grads_kernel<BF16, true>, SMEM_G>(st, g, p) : launch<grads_kernel<BF16, false>, SMEM_G>(st, g, p);
         if (rc) return rc;
     }
     if (dx) {
