@@ -101,7 +101,9 @@ SIGNATURES = {
     "cinn_moe_sum_add": [_vp, _i32, _vp, _vp, _i32, _vp, _i64, _i64, _i32, _i64, _vp],
     "cinn_linear_ce_state_bytes": [_i64],
     "cinn_linear_ce_workspace_bytes": [_i64, _i64, _i64, _i32],
-    "cinn_linear_ce_forward": [_vp, _i64, _vp, _i64, _i32, _vp, _i64, _i64, _i64, _i64, _i32, _vp, _vp, _vp, _i64, _vp],
+    "cinn_linear_ce_early": [_i64, _i64, _i64, _i32, _i32],
+    "cinn_linear_ce_forward": [_vp, _i64, _vp, _i64, _i32, _vp, _i64, _i64, _i64, _i64, _i32, _vp, _vp, _vp, _vp, _vp, _i64, _vp],
+    "cinn_linear_ce_finish": [_i32, _vp, _i64, _i64, _i64, _i32, _vp, _vp, _vp, _vp, _vp, _vp],
     "cinn_linear_ce_backward": [_vp, _i64, _vp, _i64, _i32, _vp, _i64, _i64, _i64, _i32, _vp, _vp, _vp, _vp, _i64, _vp],
     "cinn_rotary": [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i32, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i32, _i32, ctypes.c_float, _vp],
     "cinn_moe_route_form_workspace_ints": [_i64, _i32],
@@ -133,7 +135,7 @@ def _load() -> ctypes.CDLL:
                                                  "cinn_sparse_attn_workspace_bytes", "cinn_launch_count",
                                                  "cinn_fp8_grouped_wgrad_scratch_bytes", "cinn_fp8_grouped_wgrad_fused_scratch_bytes",
                                                  "cinn_quant_segments_bytes", "cinn_fp8_grouped_wgrad_segments_scratch_bytes",
-                                                 "cinn_linear_ce_state_bytes", "cinn_linear_ce_workspace_bytes")
+                                                 "cinn_linear_ce_state_bytes", "cinn_linear_ce_workspace_bytes", "cinn_linear_ce_early")
                       else ctypes.c_int)
     return lib
 

@@ -149,7 +149,11 @@ int moe_route_form_backward(const void* logits, int logits_dtype, const int* top
 int64_t linear_ce_state_bytes(int64_t T);
 int64_t linear_ce_workspace_bytes(int64_t T, int64_t V, int64_t d, int pass);
 int linear_ce_forward(const void* x, int64_t ldx, const void* w, int64_t ldw, int dtype, const int64_t* target, int64_t ignore, int64_t T, int64_t V,
-                      int64_t d, int reduction, float* loss, void* state, void* workspace, int64_t workspace_bytes, cudaStream_t st);
+                      int64_t d, int reduction, float* loss, void* state, float* dx_sums, float* dw_sums, void* workspace, int64_t workspace_bytes,
+                      cudaStream_t st);
+int64_t linear_ce_early(int64_t T, int64_t V, int64_t d, int reduction, int which);
+int linear_ce_finish(int dtype, const float* grad, int64_t T, int64_t V, int64_t d, int reduction, const void* state, const float* dx_sums,
+                     const float* dw_sums, void* dx, void* dw, cudaStream_t st);
 int linear_ce_backward(const void* x, int64_t ldx, const void* w, int64_t ldw, int dtype, const float* grad, int64_t T, int64_t V, int64_t d,
                        int reduction, const void* state, void* dx, void* dw, void* workspace, int64_t workspace_bytes, cudaStream_t st);
 int update_bias(const int64_t* counts, float* bias, int E, float expected, float gamma, cudaStream_t st);
@@ -376,10 +380,15 @@ int cinn_lightning_indexer(const void* q, const void* k, const void* w, int dtyp
 int64_t cinn_linear_ce_state_bytes(int64_t T) { return cinn::linear_ce_state_bytes(T); }
 int64_t cinn_linear_ce_workspace_bytes(int64_t T, int64_t V, int64_t d, int pass) { return cinn::linear_ce_workspace_bytes(T, V, d, pass); }
 int cinn_linear_ce_forward(const void* x, int64_t ldx, const void* w, int64_t ldw, int dtype, const int64_t* target, int64_t ignore_index,
-                           int64_t T, int64_t V, int64_t d, int reduction, float* loss, void* state, void* workspace,
-                           int64_t workspace_bytes, void* stream) {
-    return cinn::linear_ce_forward(x, ldx, w, ldw, dtype, target, ignore_index, T, V, d, reduction, loss, state, workspace, workspace_bytes,
-                                   (cudaStream_t)stream);
+                           int64_t T, int64_t V, int64_t d, int reduction, float* loss, void* state, float* dx_sums, float* dw_sums,
+                           void* workspace, int64_t workspace_bytes, void* stream) {
+    return cinn::linear_ce_forward(x, ldx, w, ldw, dtype, target, ignore_index, T, V, d, reduction, loss, state, dx_sums, dw_sums, workspace,
+                                   workspace_bytes, (cudaStream_t)stream);
+}
+int64_t cinn_linear_ce_early(int64_t T, int64_t V, int64_t d, int reduction, int which) { return cinn::linear_ce_early(T, V, d, reduction, which); }
+int cinn_linear_ce_finish(int dtype, const float* grad, int64_t T, int64_t V, int64_t d, int reduction, const void* state,
+                          const float* dx_sums, const float* dw_sums, void* dx, void* dw, void* stream) {
+    return cinn::linear_ce_finish(dtype, grad, T, V, d, reduction, state, dx_sums, dw_sums, dx, dw, (cudaStream_t)stream);
 }
 int cinn_linear_ce_backward(const void* x, int64_t ldx, const void* w, int64_t ldw, int dtype, const float* grad, int64_t T, int64_t V,
                             int64_t d, int reduction, const void* state, void* dx, void* dw, void* workspace, int64_t workspace_bytes,

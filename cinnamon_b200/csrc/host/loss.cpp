@@ -12,18 +12,37 @@ Tensor rows_of(const Tensor& t) {
 }
 int64_t pitch(const Tensor& t) { return t.size(0) > 1 ? t.stride(0) : t.size(1); }
 
-// x (T, d), w (V, d) of one 16-bit type, d a multiple of 8; target (T,) int64; reduction 0 none, 1 mean, 2 sum.
-// -> loss (fp32, (T,) or ()), what the backward takes of the forward
-std::tuple<Tensor, Tensor> ce_forward(const Tensor& x, const Tensor& w, const Tensor& target, int64_t ignore, int64_t reduction) {
+struct CrossEntropy { Tensor loss, state, dx_sums, dw_sums; };            // the sums: of the early way, undefined where a gradient is not wanted
+
+// x (T, d), w (V, d) of one 16-bit type, d a multiple of 8; target (T,) int64; reduction 0 none, 1 mean, 2 sum.  early_x, early_w: the gradients whose
+// sums are made along the way.
+CrossEntropy ce_forward(const Tensor& x, const Tensor& w, const Tensor& target, int64_t ignore, int64_t reduction, bool early_x, bool early_w) {
     c10::cuda::CUDAGuard guard(x.device());
     const int64_t T = x.size(0), d = x.size(1), V = w.size(0);
-    Tensor loss = reduction ? empty({}, at::kFloat, x.device()) : empty({T}, at::kFloat, x.device());
-    Tensor state = empty({api.cinn_linear_ce_state_bytes(T)}, at::kByte, x.device());
-    const int64_t need = api.cinn_linear_ce_workspace_bytes(T, V, d, 0);
+    CrossEntropy r;
+    r.loss = reduction ? empty({}, at::kFloat, x.device()) : empty({T}, at::kFloat, x.device());
+    r.state = empty({api.cinn_linear_ce_state_bytes(T)}, at::kByte, x.device());
+    if (early_x) r.dx_sums = empty({api.cinn_linear_ce_early(T, V, d, (int)reduction, 1) / 4}, at::kFloat, x.device());
+    if (early_w) r.dw_sums = empty({api.cinn_linear_ce_early(T, V, d, (int)reduction, 2) / 4}, at::kFloat, x.device());
+    const int64_t need = api.cinn_linear_ce_workspace_bytes(T, V, d, early_x || early_w ? 1 : 0);
     Tensor ws = empty({need}, at::kByte, x.device());
     check(api.cinn_linear_ce_forward(x.data_ptr(), pitch(x), w.data_ptr(), pitch(w), tag_of(x.scalar_type()), target.data_ptr<int64_t>(), ignore, T, V, d,
-                                     (int)reduction, f32(loss), state.data_ptr(), ws.data_ptr(), need, stream()), "cinn_linear_ce_forward");
-    return {loss, state};
+                                     (int)reduction, f32(r.loss), r.state.data_ptr(), early_x ? f32(r.dx_sums) : nullptr, early_w ? f32(r.dw_sums) : nullptr,
+                                     ws.data_ptr(), need, stream()), "cinn_linear_ce_forward");
+    return r;
+}
+
+std::tuple<Tensor, Tensor> ce_finish(const Tensor& grad, const Tensor& state, const Tensor& dx_sums, const Tensor& dw_sums, int64_t T, int64_t V, int64_t d,
+                                     at::ScalarType type, int64_t reduction) {
+    c10::cuda::CUDAGuard guard(state.device());
+    const Tensor g = grad.to(at::kFloat).contiguous();
+    Tensor dx, dw;
+    if (dx_sums.defined()) dx = empty({T, d}, type, state.device());
+    if (dw_sums.defined()) dw = empty({V, d}, type, state.device());
+    check(api.cinn_linear_ce_finish(tag_of(type), f32(g), T, V, d, (int)reduction, state.data_ptr(), dx.defined() ? f32(dx_sums) : nullptr,
+                                    dw.defined() ? f32(dw_sums) : nullptr, dx.defined() ? dx.data_ptr() : nullptr, dw.defined() ? dw.data_ptr() : nullptr,
+                                    stream()), "cinn_linear_ce_finish");
+    return {dx, dw};
 }
 
 std::tuple<Tensor, Tensor> ce_backward(const Tensor& grad, const Tensor& x, const Tensor& w, const Tensor& state, int64_t reduction, bool want_x, bool want_w) {
@@ -44,18 +63,31 @@ struct CrossEntropyNode : public torch::autograd::Function<CrossEntropyNode> {
     static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& x_in, const Tensor& w_in, const Tensor& target, int64_t ignore,
                           int64_t reduction) {
         const Tensor x = rows_of(x_in), w = rows_of(w_in);
-        const auto [loss, state] = ce_forward(x, w, target, ignore, reduction);
-        ctx->save_for_backward({x, w, state});
+        const bool early = api.cinn_linear_ce_early(x.size(0), w.size(0), x.size(1), (int)reduction, 0);
+        const CrossEntropy r = ce_forward(x, w, target, ignore, reduction, early && x_in.requires_grad(), early && w_in.requires_grad());
+        if (early) {
+            ctx->save_for_backward({r.state, r.dx_sums, r.dw_sums});
+            ctx->saved_data["shape"] = std::vector<int64_t>{x.size(0), w.size(0), x.size(1), (int64_t)x.scalar_type()};
+        } else {
+            ctx->save_for_backward({x, w, r.state});
+        }
+        ctx->saved_data["early"] = early;
         ctx->saved_data["reduction"] = reduction;
-        return loss;
+        return r.loss;
     }
     static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
         auto s = ctx->get_saved_variables();
         Tensor dx, dw;
         as_python_error([&] {
             require(!at::GradMode::is_enabled(), "linear_cross_entropy has no second derivative (create_graph=True)");
-            std::tie(dx, dw) = ce_backward(grads[0], s[0], s[1], s[2], ctx->saved_data["reduction"].toInt(), ctx->needs_input_grad(0),
-                                           ctx->needs_input_grad(1));
+            const int64_t reduction = ctx->saved_data["reduction"].toInt();
+            const bool want_x = ctx->needs_input_grad(0), want_w = ctx->needs_input_grad(1);
+            if (ctx->saved_data["early"].toBool()) {
+                const auto n = ctx->saved_data["shape"].toIntVector();
+                std::tie(dx, dw) = ce_finish(grads[0], s[0], want_x ? s[1] : Tensor(), want_w ? s[2] : Tensor(), n[0], n[1], n[2], (at::ScalarType)n[3], reduction);
+            } else {
+                std::tie(dx, dw) = ce_backward(grads[0], s[0], s[1], s[2], reduction, want_x, want_w);
+            }
         });
         return {dx, dw, Tensor(), Tensor(), Tensor()};
     }
@@ -90,8 +122,19 @@ std::tuple<Tensor, Tensor, Tensor> ce_operands(const Tensor& x_in, const Tensor&
 
 void bind_loss(pybind11::module_& m) {
     m.def("linear_ce_operands", &ce_operands);
-    m.def("linear_ce_forward", [](const Tensor& x, const Tensor& w, const Tensor& target, int64_t ignore, int64_t reduction) {
-        return ce_forward(rows_of(x), rows_of(w), target, ignore, reduction);
+    m.def("linear_ce_early", [](int64_t T, int64_t V, int64_t d, int64_t reduction, int which) { return api.cinn_linear_ce_early(T, V, d, (int)reduction, which); });
+    // (loss, state, sums of dx, sums of dw); the sums are empty in the late way
+    m.def("linear_ce_forward", [](const Tensor& x, const Tensor& w, const Tensor& target, int64_t ignore, int64_t reduction, bool early) {
+        CrossEntropy r = ce_forward(rows_of(x), rows_of(w), target, ignore, reduction, early, early);
+        if (!early) {
+            r.dx_sums = empty({0}, at::kFloat, x.device());
+            r.dw_sums = empty({0}, at::kFloat, x.device());
+        }
+        return std::make_tuple(r.loss, r.state, r.dx_sums, r.dw_sums);
+    });
+    m.def("linear_ce_finish", [](const Tensor& grad, const Tensor& state, const Tensor& dx_sums, const Tensor& dw_sums, const Tensor& x, const Tensor& w,
+                                 int64_t reduction) {
+        return ce_finish(grad, state, dx_sums, dw_sums, x.size(0), w.size(0), x.size(1), x.scalar_type(), reduction);
     });
     m.def("linear_ce_backward", [](const Tensor& grad, const Tensor& x, const Tensor& w, const Tensor& state, int64_t reduction, bool want_x, bool want_w) {
         return ce_backward(grad, rows_of(x), rows_of(w), state, reduction, want_x, want_w);
@@ -99,7 +142,7 @@ void bind_loss(pybind11::module_& m) {
     m.def("linear_cross_entropy", [](const Tensor& x_in, const Tensor& w_in, const Tensor& target_in, int64_t ignore, int64_t reduction) {
         const auto [x, w, target] = ce_operands(x_in, w_in, target_in);
         const Tensor loss = takes_node(x, w) ? CrossEntropyNode::apply(x, w, target, ignore, reduction)
-                                             : std::get<0>(ce_forward(rows_of(x), rows_of(w), target, ignore, reduction));
+                                             : ce_forward(rows_of(x), rows_of(w), target, ignore, reduction, false, false).loss;
         return reduction ? loss : loss.view(target_in.sizes());
     });
 }

@@ -6,10 +6,16 @@
 //
 // Forward: a tile of 256 tokens x 256 words is multiplied by a pair of SMs and read out of tensor memory once, into a running
 // maximum and sum per token (two fp32 numbers); tiles of one run of words are joined in registers, runs by a small pass
-// at the end.  Backward: the words in pieces; a piece's product is made again, turned into dz in the epilogue and rounded to
-// the operands' type (bf16, or fp16 times 2^14, so that small probabilities keep their bits), and two products over the
-// piece add up dx (fp32, in L2) and write the piece's rows of dW.  So the work is 2 T V d forward and 6 T V d backward, one T V d more than
-// with kept logits, and the memory is that of one piece.
+// at the end.  Backward, one of two ways:
+//   late    The words in pieces; a piece's product is made again, turned into dz in the epilogue and rounded to the operands' type
+//           (bf16, or fp16 times 2^14, so that small probabilities keep their bits), and two products over the piece add up dx
+//           (fp32, in L2) and write the piece's rows of dW.  2 T V d forward and 6 T V d backward, one 2 T V d more than with kept logits.
+//   early   The tokens in pieces; a piece's e^(z - maximum of its 128 words) is written in fp16 by the forward's product, turned into dz by one
+//           pass over it once the sums are known, and the two products add up dx and dW in fp32, all in the forward.  What is left for the
+//           backward is the loss's gradient, one number, and the one rounding.  6 T V d in all: what bounds these products is the power of
+//           the matrix units, so the fourth product is a fifth of the time; but the sums of dW stay until the backward, and a
+//           loss whose gradient is never asked for has cost three times as much.  For sums and means over many tokens (early_pays).
+// The memory is that of one piece, and early that of the gradients' sums.
 //
 // Tokens whose target is ignored take part in nothing: the others' rows are gathered first (where none is ignored, x is read
 // as it is), so that what stands in ignored rows, infinities and NaN as well, reaches neither gradient, and half a batch of
@@ -29,7 +35,7 @@ namespace ce {
 
 __device__ int g_status = 0;               // 0, or (role << 8) | reason of a bounded wait that ran out
 
-enum Mode { STATS = 0, SOFT = 1, DX = 2, DW = 3 };
+enum Mode { STATS = 0, SOFT = 1, KEEP = 2, DX = 3, DW = 4 };
 
 constexpr int M = 256, N = 256;            // the pair's tile
 constexpr int KE = 64;                     // elements of a K block: 128 bytes
@@ -52,14 +58,16 @@ constexpr float FP16_SCALE = 16384.0f;     // of dz in fp16: the smallest probab
 struct Params {
     const int* n_valid;                    // rows in use (device)
     int T, V, d;
-    int v0, vc;                            // the piece: its first word, how many
-    int parts;                             // STATS: runs of words per tile of tokens
+    int v0, vc;                            // a piece of the words: its first, how many
+    int t0, tc;                            // a piece of the rows in use
+    int parts;                             // STATS, KEEP: runs of words per tile of tokens
     int dx_splits, dw_splits;              // pieces that the reductions are cut into, each with sums of its own; 0: not wanted
     int dx_rows, dw_rows;                  // rows of one such piece's sums
-    int add;                               // dx: add to the sums of earlier pieces
+    int add_dx, add_dw;                    // add to the sums of earlier pieces
     int per_row;                           // SOFT: gradients per token (reduction "none")
     int64_t part_ld;
-    float2* part;                          // STATS: (parts * 2, part_ld) maximum and sum
+    float2* part;                          // STATS, KEEP: (parts * 2, part_ld) maximum and sum, a row for every one of the piece
+    float* tile_max;                       // KEEP: (two for each tile of words, part_ld) maximum of 128 words
     float* target_logit;
     const int* target;                     // per row in use
     const int* rows;                       // the token of every row in use
@@ -67,7 +75,7 @@ struct Params {
     const float* grad;                     // the loss's gradient: one number, or one per token
     const unsigned* grad_max;              // the bits of the largest |gradient| (reduction "none")
     int mean;
-    uint16_t* dz;                          // the piece's, rows of dz_ld (a multiple of 64)
+    uint16_t* dz;                          // the piece's (KEEP: what it will be made of), rows of dz_ld (a multiple of 64)
     int dz_ld;
 };
 
@@ -160,23 +168,27 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
 // What the gradients are multiplied by once their sums are complete: the loss's gradient (over the number of targets for a
 // mean), or the largest of the tokens' gradients, to which SOFT has related each.
 __device__ __forceinline__ float final_scale(const Params& p, bool bf16) {
-    const float s = p.per_row ? __uint_as_float(*p.grad_max) : p.mean ? *p.grad / (float)*p.n_valid : *p.grad;
+    // (a mean over nothing: no gradient, not 0 times infinity)
+    const float s = p.per_row ? __uint_as_float(*p.grad_max) : !p.mean ? *p.grad : *p.n_valid ? *p.grad / (float)*p.n_valid : 0.0f;
     return bf16 ? s : s * (1.0f / FP16_SCALE);
 }
 
+// rows in use of the piece
+__device__ __forceinline__ int rows_of(const Params& p) { return min(max(*p.n_valid - p.t0, 0), p.tc); }
+
 struct Unit { int m0, n_first, n_last, kb0, KB, split; };
 
-// Work of one cluster at a time: a tile (a run of them along the words for STATS).  Groups of GROUP row tiles, rows fastest inside.
+// Work of one cluster at a time: a tile (a run of them along the words for STATS and KEEP).  Groups of GROUP row tiles, rows fastest inside.
 template <int MODE>
 __device__ __forceinline__ int unit_count(const Params& p, int valid) {
-    const int rows = MODE == DW ? p.vc : valid, cols = MODE == STATS ? p.V : MODE == SOFT ? p.vc : p.d;
-    const int tiles = ((rows + M - 1) / M) * (MODE == STATS ? p.parts : (cols + N - 1) / N);
+    const int rows = MODE == DW ? p.vc : valid, cols = MODE == SOFT ? p.vc : MODE <= KEEP ? p.V : p.d;
+    const int tiles = ((rows + M - 1) / M) * (MODE == STATS || MODE == KEEP ? p.parts : (cols + N - 1) / N);
     return MODE == DX ? tiles * p.dx_splits : MODE == DW ? tiles * p.dw_splits : tiles;
 }
 template <int MODE>
 __device__ __forceinline__ Unit unit_at(const Params& p, int valid, int u) {
-    const int rows = MODE == DW ? p.vc : valid, cols = MODE == STATS ? p.V : MODE == SOFT ? p.vc : p.d;
-    const int m_tiles = (rows + M - 1) / M, n_tiles = (cols + N - 1) / N, across = MODE == STATS ? p.parts : n_tiles;
+    const int rows = MODE == DW ? p.vc : valid, cols = MODE == SOFT ? p.vc : MODE <= KEEP ? p.V : p.d;
+    const int m_tiles = (rows + M - 1) / M, n_tiles = (cols + N - 1) / N, across = MODE == STATS || MODE == KEEP ? p.parts : n_tiles;
     const int red = MODE == DX ? p.vc : MODE == DW ? valid : p.d, blocks = (red + KE - 1) / KE;
     Unit r;
     r.split = 0; r.kb0 = 0; r.KB = blocks;
@@ -190,7 +202,7 @@ __device__ __forceinline__ Unit unit_at(const Params& p, int valid, int u) {
     const int g = u / (GROUP * across), first = g * GROUP, size = min(GROUP, m_tiles - first);
     const int in = u - g * GROUP * across, n = in / size;
     r.m0 = (first + in - n * size) * M;
-    if constexpr (MODE == STATS) {
+    if constexpr (MODE == STATS || MODE == KEEP) {
         const int run = (n_tiles + p.parts - 1) / p.parts;             // (all of one length but the last)
         r.n_first = n * run;
         r.n_last = min(r.n_first + run, n_tiles);
@@ -336,7 +348,8 @@ __device__ __forceinline__ uint64_t pair2(float a, float b) {
     return r;
 }
 
-// The logits' product: A = x, B = W, both K-major.  STATS leaves maxima and sums of its runs, SOFT dz of the piece.  xg: x's rows in use,
+// The logits' product: A = x, B = W, both K-major.  STATS leaves maxima and sums of its runs, SOFT dz of the piece, KEEP both maxima and sums, and
+// e^(z - maximum) in fp16, of each half tile.  xg: x's rows in use,
 // gathered; read in x's place where some token is ignored.
 template <int MODE, bool BF16>
 __global__ void __launch_bounds__(THREADS, 1)
@@ -346,7 +359,7 @@ product_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__
     extern __shared__ uint8_t smem_raw[];
     Setup<STAGES, 0> s(smem_raw);
     const int warp = s.warp, lane = s.lane, rank = (int)s.rank;
-    const int valid = *p.n_valid;
+    const int valid = rows_of(p);
     const int n_units = unit_count<MODE>(p, valid);
     const int cluster = blockIdx.x >> 1, n_clusters = gridDim.x >> 1;
 
@@ -354,13 +367,13 @@ product_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__
         // ------------------------------ TMA producer (both CTAs) ------------------------------
         if (lane == 0) {
             const uint32_t full_leader = mapa(s.full0, 0);
-            const CUtensorMap* map_a = valid != p.T ? &tm_xg : &tm_a;
+            const CUtensorMap* map_a = *p.n_valid != p.T ? &tm_xg : &tm_a;
             uint32_t it = 0;
             bool alive = true;
             for (int u = cluster; u < n_units && alive; u += n_clusters) {
                 const Unit w = unit_at<MODE>(p, valid, u);
                 for (int nt = w.n_first; nt < w.n_last && alive; ++nt) {
-                    const int ma = w.m0 + 128 * rank, nb = p.v0 + nt * N + 128 * rank;
+                    const int ma = p.t0 + w.m0 + 128 * rank, nb = p.v0 + nt * N + 128 * rank;
                     for (int kb = 0; kb < w.KB; ++kb, ++it) {
                         const int st = it % STAGES;
                         if (!wait(s.empty0 + 8 * st, (it / STAGES & 1) ^ 1, s.abort_flag, (11 << 8) | 1)) { alive = false; break; }
@@ -417,7 +430,7 @@ product_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__
             float mx = -INFINITY, sum = 0.0f, rel = 0.0f;
             int target = -1;
             if (live) {
-                target = p.target[row];
+                target = p.target[p.t0 + row];
                 if constexpr (MODE == SOFT) {
                     const float2 st = p.stat[row];
                     mx = st.x; sum = st.y;
@@ -444,7 +457,7 @@ product_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__
                             float z = 0.0f;
 #pragma unroll
                             for (int j = 0; j < 32; ++j) z = j == hit ? __uint_as_float(r[j]) : z;
-                            p.target_logit[row] = z;
+                            p.target_logit[p.t0 + row] = z;
                         }
                         if (at + 32 > p.V) {               // words past the last one
 #pragma unroll
@@ -464,6 +477,72 @@ product_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__
                     tc_fence_before();
                     __syncwarp();
                     if (lane == 0) arrive_remote(tempty_leader + 8 * b);
+                } else if constexpr (MODE == KEEP) {
+                    uint32_t r[2][32];                     // 32 words at work, the next ones on their way
+                    float top = -INFINITY;
+                    ld32(taddr, r[0]);
+#pragma unroll
+                    for (int c = 0; c < COLS / 32; ++c) {
+                        ld_wait();
+                        ld32(taddr + (c + 1) % (COLS / 32) * 32, r[(c + 1) & 1]);      // (after the last: the first again)
+                        const uint32_t(&z)[32] = r[c & 1];
+                        const int at = col0 + c * 32, hit = target - at, left = p.V - at;
+                        if ((unsigned)hit < 32u) {
+                            float v = 0.0f;
+#pragma unroll
+                            for (int j = 0; j < 32; ++j) v = j == hit ? __uint_as_float(z[j]) : v;
+                            p.target_logit[p.t0 + row] = v;
+                        }
+                        if (left >= 32) {
+#pragma unroll
+                            for (int j = 0; j < 32; ++j) top = fmaxf(top, __uint_as_float(z[j]));
+                        } else {
+#pragma unroll
+                            for (int j = 0; j < 32; ++j) top = j < left ? fmaxf(top, __uint_as_float(z[j])) : top;
+                        }
+                    }
+                    const float base = top == -INFINITY ? 0.0f : top;
+                    const uint64_t minus = pair2(-base, -base), scale = pair2(LOG2E, LOG2E);
+                    float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                    for (int c = 0; c < COLS / 32; ++c) {
+                        ld_wait();
+                        if (c + 1 < COLS / 32) ld32(taddr + (c + 1) * 32, r[(c + 1) & 1]);
+                        else {
+                            tc_fence_before();
+                            __syncwarp();
+                            if (lane == 0) arrive_remote(tempty_leader + 8 * b);       // all of the tile is in registers
+                        }
+                        uint32_t(&z)[32] = r[c & 1];
+                        const int left = p.V - (col0 + c * 32);
+#pragma unroll
+                        for (int j = 0; j < 32; j += 2)
+                            asm("{\n\t.reg .b64 a;\n\t"
+                                "mov.b64 a, {%0, %1};\n\t"
+                                "add.rn.f32x2 a, a, %2;\n\t"
+                                "mul.rn.f32x2 a, a, %3;\n\t"
+                                "mov.b64 {%0, %1}, a;\n\t"
+                                "ex2.approx.ftz.f32 %0, %0;\n\tex2.approx.ftz.f32 %1, %1;\n\t}" : "+r"(z[j]), "+r"(z[j + 1]) : "l"(minus), "l"(scale));
+                        if (!live || left < 32) {
+#pragma unroll
+                            for (int j = 0; j < 32; ++j)
+                                if (!live || j >= left) z[j] = 0u;
+                        }
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) part[j & 3] += __uint_as_float(z[j]);
+                        const int col = nt * N + h * COLS + c * 32;
+                        if (col < p.dz_ld) {
+                            uint32_t v[16];
+#pragma unroll
+                            for (int j = 0; j < 16; ++j) v[j] = pack2<false>(__uint_as_float(z[2 * j]), __uint_as_float(z[2 * j + 1]));
+                            store32(p.dz + (int64_t)row * p.dz_ld + col, v);
+                            store32(p.dz + (int64_t)row * p.dz_ld + col + 16, v + 8);
+                        }
+                    }
+                    if (live) p.tile_max[(int64_t)(nt * 2 + h) * p.part_ld + row] = base;
+                    const float best = fmaxf(mx, top), from = best == -INFINITY ? 0.0f : best;
+                    sum = sum * exp2_approx((mx - from) * LOG2E) + ((part[0] + part[1]) + (part[2] + part[3])) * exp2_approx((top - from) * LOG2E);
+                    mx = best;
                 } else {
                     const uint64_t minus = pair2(-mx, -mx), scale = pair2(LOG2E, LOG2E), logs = pair2(-sum, -sum), rels = pair2(rel, rel);
                     uint32_t r[2][32];                     // a chunk of 32 words at work, the next one on its way
@@ -519,7 +598,7 @@ product_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__
                     }
                 }
             }
-            if constexpr (MODE == STATS) {
+            if constexpr (MODE == STATS || MODE == KEEP) {
                 // (a part holds two halves of the columns, each a warp's)
                 const int across = p.parts, m_tiles = (valid + M - 1) / M;
                 const int g = u / (GROUP * across), size = min(GROUP, m_tiles - g * GROUP);
@@ -543,7 +622,7 @@ grads_kernel(const __grid_constant__ GradMaps maps, const Params p) {
     extern __shared__ uint8_t smem_raw[];
     Setup<STAGES, C_BYTES> s(smem_raw);
     const int warp = s.warp, lane = s.lane, rank = (int)s.rank;
-    const int valid = *p.n_valid;
+    const int valid = rows_of(p);
     const Schedule plan(p, valid, blockIdx.x >> 1, gridDim.x >> 1);
     bool dx;
     int u;
@@ -552,7 +631,7 @@ grads_kernel(const __grid_constant__ GradMaps maps, const Params p) {
         // ------------------------------ TMA producer (both CTAs) ------------------------------
         if (lane == 0) {
             const uint32_t full_leader = mapa(s.full0, 0);
-            const CUtensorMap* map_x = valid != p.T ? &maps.xg_cols : &maps.x_cols;
+            const CUtensorMap* map_x = *p.n_valid != p.T ? &maps.xg_cols : &maps.x_cols;
             uint32_t it = 0;
             bool alive = true;
             for (int i = 0; alive && plan.at(i, dx, u); ++i) {
@@ -564,7 +643,7 @@ grads_kernel(const __grid_constant__ GradMaps maps, const Params p) {
                     if (!wait(s.empty0 + 8 * st, (it / STAGES & 1) ^ 1, s.abort_flag, (11 << 8) | 2)) { alive = false; break; }
                     if (rank == 0) mbar_expect_tx(s.full0 + 8 * st, 4 * SIDE);
                     const uint32_t bar = full_leader + 8 * st, da = smem_u32(s.smem_a + st * SIDE), db = smem_u32(s.smem_b + st * SIDE);
-                    const int k = (w.kb0 + kb) * KE, y = dx ? p.v0 + k : k;
+                    const int k = (w.kb0 + kb) * KE, y = dx ? p.v0 + k : p.t0 + k;
                     if (dx) {
                         load_2d(&maps.z_rows, bar, da, k, ma);
                     } else {
@@ -642,8 +721,8 @@ grads_kernel(const __grid_constant__ GradMaps maps, const Params p) {
 #pragma unroll
                     for (int j = 0; j < 8; ++j) stage16(box, lane, j, v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
                     const int col = col0 + c * 32;
-                    if (dx) boxes.send(lane, &maps.c_dx, col, w.split * p.dx_rows + row, col < p.d, p.add);
-                    else boxes.send(lane, &maps.c_dw, col, w.split * p.dw_rows + row, col < p.d, false);
+                    if (dx) boxes.send(lane, &maps.c_dx, col, w.split * p.dx_rows + p.t0 + row, col < p.d, p.add_dx);
+                    else boxes.send(lane, &maps.c_dw, col, w.split * p.dw_rows + row, col < p.d, p.add_dw);
                 } else {                                   // 64 columns
                     if ((c & 1) == 0) box = boxes.open(lane);
 #pragma unroll
@@ -799,14 +878,14 @@ constexpr int JOIN = 16;                   // warps of a block: each joins every
 // read one after the other.)
 __global__ void __launch_bounds__(32 * JOIN)
 loss_kernel(const float2* __restrict__ part, int64_t part_ld, int parts, const float* __restrict__ target_logit, State s, int T, int reduction,
-            double* __restrict__ block_sum, float* __restrict__ loss) {
+            double* __restrict__ block_sum, float* __restrict__ loss, int t0, int tc, int last) {
     pdl_wait();
     pdl_trigger();
     __shared__ float2 s_part[JOIN][32];
     __shared__ double s_sum[JOIN];
     __shared__ bool s_last;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, t = blockIdx.x * 32 + lane;
-    const int row = t < T ? s.slot[t] : -1;
+    const int slot = t < T ? s.slot[t] : -1, row = slot >= t0 && slot - t0 < tc ? slot : -1;       // (of this piece)
     float mx = -INFINITY, sum = 0.0f;
     auto join = [&](float2 v) {
         const float top = fmaxf(mx, v.x), base = top == -INFINITY ? 0.0f : top;
@@ -815,13 +894,13 @@ loss_kernel(const float2* __restrict__ part, int64_t part_ld, int parts, const f
     };
     if (row >= 0) {
 #pragma unroll 4
-        for (int i = warp; i < parts; i += JOIN) join(part[(int64_t)i * part_ld + row]);
+        for (int i = warp; i < parts; i += JOIN) join(part[(int64_t)i * part_ld + row - t0]);
     }
     s_part[warp][lane] = make_float2(mx, sum);
     __syncthreads();
     double mine = 0.0;
     if (warp == 0 && t < T) {
-        float l = row == -2 ? NAN : 0.0f;
+        float l = slot == -2 && t0 == 0 ? NAN : 0.0f;
         if (row >= 0) {
 #pragma unroll
             for (int w = 1; w < JOIN; ++w) join(s_part[w][lane]);
@@ -840,9 +919,10 @@ loss_kernel(const float2* __restrict__ part, int64_t part_ld, int parts, const f
     if (warp == 0) {
         mine = warp_total(mine);
         if (lane == 0) {
+            if (t0) mine += block_sum[blockIdx.x];           // of earlier pieces
             block_sum[blockIdx.x] = mine;
             __threadfence();
-            s_last = atomicAdd(&s.n_valid[1], 1) == (int)gridDim.x - 1;
+            s_last = last && atomicAdd(&s.n_valid[1], 1) == (int)gridDim.x - 1;
         }
     }
     __syncthreads();
@@ -861,8 +941,37 @@ loss_kernel(const float2* __restrict__ part, int64_t part_ld, int parts, const f
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
-// gradients: what is left when the products are done
+// gradients: what is left around the products
 // ---------------------------------------------------------------------------------------------------------------------
+// What KEEP left, turned into dz in its place: e^(z - m) e^(m - lse) - [the target], m the maximum of the 128 words.  A warp a row, 256 words at a time; bound by
+// reading and writing them.  Where the target is the likeliest word, its e^0 is exact, and so 1 - p keeps the bits of p's fp32.
+template <bool BF16>
+__global__ void __launch_bounds__(256)
+soften_kernel(const Params p) {
+    pdl_wait();
+    pdl_trigger();
+    const int lane = threadIdx.x & 31, valid = rows_of(p), vecs = p.dz_ld / 8;
+    const int per = (vecs + 31) / 32;                      // turns of a row
+    for (int64_t i = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); i < (int64_t)valid * per; i += (int64_t)gridDim.x * 8) {
+        const int row = (int)(i / per), at = (int)(i - (int64_t)row * per) * 32 + lane;
+        if (at >= vecs) continue;
+        const float2 st = p.stat[p.t0 + row];
+        const float f = exp2_approx((p.tile_max[(int64_t)(at / 16) * p.part_ld + row] - st.x) * LOG2E - st.y);
+        uint4* q = reinterpret_cast<uint4*>(p.dz + (int64_t)row * p.dz_ld) + at;
+        uint4 v = *q;
+        uint32_t* h = &v.x;
+        const int hit = p.target[p.t0 + row] - at * 8;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            float2 e = __half22float2(*reinterpret_cast<const __half2*>(&h[j]));
+            e.x = e.x * f - (hit == 2 * j ? 1.0f : 0.0f);
+            e.y = e.y * f - (hit == 2 * j + 1 ? 1.0f : 0.0f);
+            h[j] = BF16 ? pack2<true>(e.x, e.y) : pack2<false>(e.x * FP16_SCALE, e.y * FP16_SCALE);
+        }
+        *q = v;
+    }
+}
+
 // the largest |gradient| among the tokens in use, as bits (a NaN is larger than any number); *out starts at 0
 __global__ void __launch_bounds__(256)
 grad_max_kernel(const float* __restrict__ grad, const int* __restrict__ slot, int T, unsigned* __restrict__ out) {
@@ -914,30 +1023,58 @@ struct Plan {
     int64_t vc;                            // words of a piece
     int pieces, dx_splits, dw_splits;
     int64_t dz_ld;
+    bool early;
+    int64_t tc;                            // early: tokens of a piece
 };
 
 constexpr int64_t PART_BYTES = 48LL << 20;
 constexpr int64_t DZ_BYTES = 512LL << 20;  // most of a piece of dz: smaller pieces cost passes over dx, larger ones only memory
 
-static Plan make_plan(int64_t T, int64_t V, int64_t d) {
+constexpr int64_t EARLY_BYTES = 5LL << 28; // the same of a piece of tokens: beyond the first one dW is added to, in memory
+constexpr int64_t EARLY_TOKENS = 2048;     // from here on the early way saves more than the sums of dW cost
+constexpr int64_t EARLY_KEPT = 8LL << 30;  // most of what it leaves for the backward
+
+static Plan make_plan(int64_t T, int64_t V, int64_t d, bool early) {
     Plan r{};
-    r.T = T; r.V = V; r.d = d; r.Tp = up(T, M);
+    r.T = T; r.V = V; r.d = d; r.Tp = up(T, M); r.early = early;
     r.clusters = std::max(1, sm_count() / 2);          // (not those under a cap: sizes must not change between two calls)
-    const int64_t m_tiles = r.Tp / M, n_tiles = ceil_div(V, N), n_d = ceil_div(d, N);
-    // runs of words: one tile each, for an even end, unless what they leave per token is more than PART_BYTES
-    r.parts = (int)ceil_div(n_tiles, ceil_div(16 * n_tiles * r.Tp, PART_BYTES));
-    const int64_t fit = std::max<int64_t>(N, DZ_BYTES / (2 * r.Tp) / N * N);
-    r.pieces = (int)ceil_div(V, fit);
-    r.vc = up(ceil_div(V, r.pieces), N);   // equal pieces, in whole tiles
-    r.pieces = (int)ceil_div(V, r.vc);
-    r.dz_ld = up(std::min(r.vc, V), KE);
+    const int64_t n_tiles = ceil_div(V, N), n_d = ceil_div(d, N);
     // reductions cut where their tiles would leave SMs idle, down to 16 K blocks a piece
     auto cut = [&](int64_t tiles, int64_t blocks) {
         return (int)std::max<int64_t>(1, std::min<int64_t>({(int64_t)r.clusters / std::max<int64_t>(1, tiles), blocks / 16, (int64_t)16}));
     };
-    r.dx_splits = cut(m_tiles * n_d, ceil_div(std::min(r.vc, V), KE));
-    r.dw_splits = r.pieces > 1 ? 1 : cut(n_tiles * n_d, ceil_div(T, KE));
+    if (early) {
+        r.dz_ld = up(V, KE);
+        const int64_t fit = std::max<int64_t>(M, EARLY_BYTES / (2 * r.dz_ld) / M * M);
+        r.pieces = (int)ceil_div(r.Tp, fit);
+        r.tc = up(ceil_div(r.Tp, r.pieces), M);        // equal pieces, in whole tiles
+        r.pieces = (int)ceil_div(r.Tp, r.tc);
+        r.vc = V;
+        r.dx_splits = cut(r.tc / M * n_d, ceil_div(V, KE));
+        r.dw_splits = r.pieces > 1 ? 1 : cut(n_tiles * n_d, ceil_div(T, KE));
+    } else {
+        const int64_t fit = std::max<int64_t>(N, DZ_BYTES / (2 * r.Tp) / N * N);
+        r.pieces = (int)ceil_div(V, fit);
+        r.vc = up(ceil_div(V, r.pieces), N);
+        r.pieces = (int)ceil_div(V, r.vc);
+        r.dz_ld = up(std::min(r.vc, V), KE);
+        r.tc = r.Tp;
+        r.dx_splits = cut(r.Tp / M * n_d, ceil_div(std::min(r.vc, V), KE));
+        r.dw_splits = r.pieces > 1 ? 1 : cut(n_tiles * n_d, ceil_div(T, KE));
+    }
+    // runs of words: one tile each, for an even end, unless what they leave per token is more than PART_BYTES
+    r.parts = (int)ceil_div(n_tiles, ceil_div(16 * n_tiles * r.tc, PART_BYTES));
     return r;
+}
+
+static int64_t dx_sums_bytes(const Plan& r) { return 4 * r.dx_splits * r.Tp * r.d; }
+static int64_t dw_sums_bytes(const Plan& r) { return 4 * r.dw_splits * up(r.V, M) * r.d; }
+// Whether both gradients of a sum or mean are made in the forward.  What it saves, a product of 2 T V d at 1.3e15 a second, is more than what it
+// costs, 10 V d bytes of sums at 6e12, from some 1100 tokens on.
+static bool early_pays(int64_t T, int64_t V, int64_t d, int reduction) {
+    if (reduction == 0 || T < EARLY_TOKENS) return false;
+    const Plan r = make_plan(T, V, d, true);
+    return dx_sums_bytes(r) + dw_sums_bytes(r) <= EARLY_KEPT;
 }
 
 struct Carver {                            // sub-allocations of one workspace, 256 bytes apart
@@ -958,15 +1095,17 @@ static State carve_state(void* mem, int64_t T, int64_t* bytes) {
     return s;
 }
 
-struct Forward { int* counts; void* xg; float2* part; float* target_logit; double* block_sum; };
+struct Forward { int* counts; void* xg; float2* part; float* target_logit; double* block_sum; void* dz; float* tile_max; };
 static Forward carve_forward(void* mem, const Plan& r, int64_t* bytes) {
     Carver c{static_cast<uint8_t*>(mem)};
     Forward f;
     f.counts = static_cast<int*>(c.take(4 * ceil_div(r.T, SCAN)));
     f.xg = c.take(up(r.T, KE) * r.d * 2);
-    f.part = static_cast<float2*>(c.take(8LL * 2 * r.parts * r.Tp));
+    f.part = static_cast<float2*>(c.take(8LL * 2 * r.parts * r.tc));
     f.target_logit = static_cast<float*>(c.take(4 * r.T));
     f.block_sum = static_cast<double*>(c.take(8 * ceil_div(r.T, 32)));
+    f.dz = c.take(r.early ? r.tc * r.dz_ld * 2 : 0);
+    f.tile_max = static_cast<float*>(c.take(r.early ? 4 * 2 * ceil_div(r.V, N) * r.tc : 0));
     if (bytes) *bytes = c.used;
     return f;
 }
@@ -977,8 +1116,8 @@ static Backward carve_backward(void* mem, const Plan& r, bool want_dx, bool want
     b.grad_max = static_cast<unsigned*>(c.take(4));
     b.xg = c.take(up(r.T, KE) * r.d * 2);
     b.dz = c.take(r.Tp * r.dz_ld * 2);
-    b.dx = static_cast<float*>(c.take(want_dx ? 4 * r.dx_splits * r.Tp * r.d : 0));
-    b.dw = static_cast<float*>(c.take(want_dw && r.dw_splits > 1 ? 4 * r.dw_splits * up(r.V, M) * r.d : 0));
+    b.dx = static_cast<float*>(c.take(want_dx ? dx_sums_bytes(r) : 0));
+    b.dw = static_cast<float*>(c.take(want_dw && r.dw_splits > 1 ? dw_sums_bytes(r) : 0));
     if (bytes) *bytes = c.used;
     return b;
 }
@@ -1005,6 +1144,10 @@ static int map16(CUtensorMap* m, const void* base, int64_t inner, int64_t rows, 
                          bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
+static int map_sums(CUtensorMap* m, float* base, int64_t rows, int64_t d) {
+    return encode_map_2d(m, base, (uint64_t)d, (uint64_t)rows, (uint64_t)d * 4, 32, 32, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
 static unsigned grid_for(int64_t items, int64_t per_block) { return (unsigned)std::max<int64_t>(1, std::min<int64_t>(ceil_div(items, per_block), 8LL * sm_count())); }
 
 static int check_shapes(const void* x, int64_t ldx, const void* w, int64_t ldw, int dtype, int64_t T, int64_t V, int64_t d, int reduction) {
@@ -1029,7 +1172,7 @@ static int gather(const void* x, int64_t ldx, const Plan& r, const State& s, voi
 
 template <bool BF16>
 static int forward(const void* x, int64_t ldx, const void* w, int64_t ldw, const int64_t* target, int64_t ignore, const Plan& r, int reduction,
-                   float* loss, const State& s, const Forward& f, cudaStream_t st) {
+                   float* loss, const State& s, const Forward& f, float* dx_sums, float* dw_sums, cudaStream_t st) {
     const int blocks = (int)ceil_div(r.T, SCAN);
     int rc = CINN_OK;
     if (r.T <= SMALL) {
@@ -1048,11 +1191,46 @@ static int forward(const void* x, int64_t ldx, const void* w, int64_t ldw, const
     if ((rc = map16(&tx, f.xg, r.d, up(r.T, KE), r.d, 128, BF16))) return rc;
     if ((rc = map16(&tb, w, r.d, r.V, ldw, 128, BF16))) return rc;
     Params p{};
-    p.n_valid = s.n_valid; p.T = (int)r.T; p.V = (int)r.V; p.d = (int)r.d; p.parts = r.parts;
-    p.part = f.part; p.part_ld = r.Tp; p.target_logit = f.target_logit; p.target = s.target;
-    if ((rc = launch<product_kernel<STATS, BF16>, SMEM_Z>(st, ta, tb, tx, p))) return rc;
-    launch_dependent(loss_kernel, dim3((unsigned)ceil_div(r.T, 32)), dim3(32 * JOIN), 0, st, f.part, r.Tp, 2 * r.parts, f.target_logit, s, (int)r.T,
-                     reduction, f.block_sum, loss);
+    p.n_valid = s.n_valid; p.T = (int)r.T; p.V = (int)r.V; p.d = (int)r.d; p.vc = (int)r.V; p.tc = (int)r.tc; p.parts = r.parts;
+    p.part = f.part; p.part_ld = r.tc; p.target_logit = f.target_logit; p.target = s.target; p.stat = s.stat;
+    auto join = [&](int last) {
+        launch_dependent(loss_kernel, dim3((unsigned)ceil_div(r.T, 32)), dim3(32 * JOIN), 0, st, f.part, r.tc, 2 * r.parts, f.target_logit, s, (int)r.T,
+                         reduction, f.block_sum, loss, p.t0, p.tc, last);
+        CINN_CHECK_LAUNCH();
+        return (int)CINN_OK;
+    };
+    if (!r.early) {
+        if ((rc = launch<product_kernel<STATS, BF16>, SMEM_Z>(st, ta, tb, tx, p))) return rc;
+        return join(1);
+    }
+    GradMaps g;
+    if ((rc = map16(&g.x_cols, x, r.d, r.T, ldx, 64, BF16))) return rc;
+    if ((rc = map16(&g.xg_cols, f.xg, r.d, up(r.T, KE), r.d, 64, BF16))) return rc;
+    if ((rc = map16(&g.w_cols, w, r.d, r.V, ldw, 64, BF16))) return rc;
+    if ((rc = map16(&g.z_rows, f.dz, r.V, r.tc, r.dz_ld, 128, BF16))) return rc;
+    if ((rc = map16(&g.z_cols, f.dz, r.V, r.tc, r.dz_ld, 64, BF16))) return rc;
+    g.c_dx = g.c_dw = g.x_cols;            // (one that is not wanted is not used)
+    if (dx_sums && (rc = map_sums(&g.c_dx, dx_sums, r.dx_splits * r.Tp, r.d))) return rc;
+    if (dw_sums && (rc = map_sums(&g.c_dw, dw_sums, r.dw_splits * up(r.V, M), r.d))) return rc;
+    p.dz = static_cast<uint16_t*>(f.dz); p.dz_ld = (int)r.dz_ld; p.tile_max = f.tile_max;
+    p.dx_splits = dx_sums ? r.dx_splits : 0; p.dx_rows = (int)r.Tp;
+    p.dw_splits = dw_sums ? r.dw_splits : 0; p.dw_rows = (int)up(r.V, M);
+    for (int i = 0; i < r.pieces; ++i) {
+        p.t0 = (int)(i * r.tc);
+        p.add_dw = i > 0;
+        if ((rc = launch<product_kernel<KEEP, BF16>, SMEM_Z>(st, ta, tb, tx, p))) return rc;
+        if ((rc = join(i + 1 == r.pieces))) return rc;
+        launch_dependent(soften_kernel<BF16>, dim3((unsigned)(8 * sm_count())), dim3(256), 0, st, p);
+        CINN_CHECK_LAUNCH();
+        if ((rc = launch<grads_kernel<BF16, true>, SMEM_G>(st, g, p))) return rc;
+    }
+    return CINN_OK;
+}
+
+template <bool BF16>
+static int finish(const float* sums, int splits, int64_t split_rows, int64_t rows, int64_t d, const int* slot, const Params& p, void* out, cudaStream_t st) {
+    launch_dependent(finish_kernel<BF16>, dim3(grid_for(rows * (d / 4), 256)), dim3(256), 0, st, sums, splits, split_rows * d, (int)rows, (int)d, slot, p,
+                     static_cast<uint2*>(out));
     CINN_CHECK_LAUNCH();
     return CINN_OK;
 }
@@ -1063,7 +1241,7 @@ static int backward(const void* x, int64_t ldx, const void* w, int64_t ldw, cons
     int rc = gather(x, ldx, r, s, b.xg, st);
     if (rc) return rc;
     Params p{};
-    p.n_valid = s.n_valid; p.T = (int)r.T; p.V = (int)r.V; p.d = (int)r.d;
+    p.n_valid = s.n_valid; p.T = (int)r.T; p.V = (int)r.V; p.d = (int)r.d; p.tc = (int)r.Tp;
     p.target = s.target; p.rows = s.rows; p.stat = s.stat; p.grad = grad; p.grad_max = b.grad_max;
     p.per_row = reduction == 0; p.mean = reduction == 1;
     if (p.per_row) {
@@ -1079,13 +1257,10 @@ static int backward(const void* x, int64_t ldx, const void* w, int64_t ldw, cons
     if ((rc = map16(&g.x_cols, x, r.d, r.T, ldx, 64, BF16))) return rc;
     if ((rc = map16(&g.xg_cols, b.xg, r.d, up(r.T, KE), r.d, 64, BF16))) return rc;
     if ((rc = map16(&g.w_cols, w, r.d, r.V, ldw, 64, BF16))) return rc;
-    auto sums = [&](CUtensorMap* m, float* base, int64_t rows) {
-        return encode_map_2d(m, base, (uint64_t)r.d, (uint64_t)rows, (uint64_t)r.d * 4, 32, 32, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, CU_TENSOR_MAP_SWIZZLE_128B);
-    };
     g.c_dx = g.c_dw = g.x_cols;            // (one that is not wanted is not used)
-    if (dx && (rc = sums(&g.c_dx, b.dx, r.dx_splits * r.Tp))) return rc;
+    if (dx && (rc = map_sums(&g.c_dx, b.dx, r.dx_splits * r.Tp, r.d))) return rc;
     if (dw) {
-        if (r.dw_splits > 1) rc = sums(&g.c_dw, b.dw, r.dw_splits * up(r.V, M));
+        if (r.dw_splits > 1) rc = map_sums(&g.c_dw, b.dw, r.dw_splits * up(r.V, M), r.d);
         else rc = map16(&g.c_dw, dw, r.d, r.V, r.d, 32, BF16);
         if (rc) return rc;
     }
@@ -1095,23 +1270,15 @@ static int backward(const void* x, int64_t ldx, const void* w, int64_t ldw, cons
     for (int i = 0; i < r.pieces; ++i) {
         p.v0 = (int)(i * r.vc);
         p.vc = (int)std::min<int64_t>(r.vc, r.V - p.v0);
-        p.add = i > 0;
+        p.add_dx = i > 0;
         if ((rc = map16(&g.z_rows, b.dz, p.vc, r.Tp, r.dz_ld, 128, BF16))) return rc;
         if ((rc = map16(&g.z_cols, b.dz, p.vc, r.Tp, r.dz_ld, 64, BF16))) return rc;
         if ((rc = launch<product_kernel<SOFT, BF16>, SMEM_Z>(st, x_rows, w_rows, xg_rows, p))) return rc;
         rc = r.dw_splits > 1 ? launch<grads_kernel<BF16, true>, SMEM_G>(st, g, p) : launch<grads_kernel<BF16, false>, SMEM_G>(st, g, p);
         if (rc) return rc;
     }
-    if (dx) {
-        launch_dependent(finish_kernel<BF16>, dim3(grid_for(r.T * (r.d / 4), 256)), dim3(256), 0, st, b.dx, r.dx_splits, r.Tp * r.d, (int)r.T, (int)r.d,
-                         s.slot, p, static_cast<uint2*>(dx));
-        CINN_CHECK_LAUNCH();
-    }
-    if (dw && r.dw_splits > 1) {
-        launch_dependent(finish_kernel<BF16>, dim3(grid_for(r.V * (r.d / 4), 256)), dim3(256), 0, st, b.dw, r.dw_splits, up(r.V, M) * r.d, (int)r.V,
-                         (int)r.d, nullptr, p, static_cast<uint2*>(dw));
-        CINN_CHECK_LAUNCH();
-    }
+    if (dx && (rc = finish<BF16>(b.dx, r.dx_splits, r.Tp, r.T, r.d, s.slot, p, dx, st))) return rc;
+    if (dw && r.dw_splits > 1) return finish<BF16>(b.dw, r.dw_splits, up(r.V, M), r.V, r.d, nullptr, p, dw, st);
     return CINN_OK;
 }
 
@@ -1122,33 +1289,64 @@ int64_t linear_ce_state_bytes(int64_t T) {
     if (T > 0) ce::carve_state(nullptr, T, &n);
     return n;
 }
+// pass: 0 = forward, 1 = forward with early gradients, 4 = (late) backward, + 1 with dx, + 2 with dw
 int64_t linear_ce_workspace_bytes(int64_t T, int64_t V, int64_t d, int pass) {
     if (T <= 0 || V <= 0 || d <= 0) return 0;
     int64_t n = 0;
-    const ce::Plan r = ce::make_plan(T, V, d);
-    if (pass == 0) ce::carve_forward(nullptr, r, &n);
+    const ce::Plan r = ce::make_plan(T, V, d, pass == 1);
+    if (pass < 4) ce::carve_forward(nullptr, r, &n);
     else ce::carve_backward(nullptr, r, pass & 1, pass & 2, &n);
     return n;
 }
+// which: 0 = whether the early way is taken, 1, 2 = bytes of the sums of dx, dw
+int64_t linear_ce_early(int64_t T, int64_t V, int64_t d, int reduction, int which) {
+    if (T <= 0 || V <= 0 || d <= 0) return 0;
+    if (which == 0) return ce::early_pays(T, V, d, reduction);
+    const ce::Plan r = ce::make_plan(T, V, d, true);
+    return which == 1 ? ce::dx_sums_bytes(r) : ce::dw_sums_bytes(r);
+}
 
 int linear_ce_forward(const void* x, int64_t ldx, const void* w, int64_t ldw, int dtype, const int64_t* target, int64_t ignore, int64_t T, int64_t V,
-                      int64_t d, int reduction, float* loss, void* state, void* workspace, int64_t workspace_bytes, cudaStream_t st) {
+                      int64_t d, int reduction, float* loss, void* state, float* dx_sums, float* dw_sums, void* workspace, int64_t workspace_bytes,
+                      cudaStream_t st) {
     int rc = ce::check_shapes(x, ldx, w, ldw, dtype, T, V, d, reduction);
     if (rc) return rc;
     CINN_CHECK_ARG(loss || (T == 0 && reduction == 0), "linear_ce: null pointer");
+    const bool early = dx_sums || dw_sums;
+    CINN_CHECK_ARG(!early || (reduction != 0 && T > 0), "linear_ce: early gradients are those of a sum or mean over some tokens");
+    CINN_CHECK_ARG(((reinterpret_cast<uintptr_t>(dx_sums) | reinterpret_cast<uintptr_t>(dw_sums)) & 15) == 0, "linear_ce: sums must be 16-byte aligned");
     if (T == 0) {
         // a mean of nothing is NaN (all bits set), a sum 0
         if (reduction) CINN_CHECK_CUDA(cudaMemsetAsync(loss, reduction == 1 ? 0xff : 0, 4, st));
         return CINN_OK;
     }
     CINN_CHECK_ARG(target && state && workspace, "linear_ce: null pointer");
-    const ce::Plan r = ce::make_plan(T, V, d);
+    const ce::Plan r = ce::make_plan(T, V, d, early);
     int64_t need = 0;
     const ce::Forward f = ce::carve_forward(workspace, r, &need);
     CINN_CHECK_ARG(workspace_bytes >= need, "linear_ce: workspace of %lld bytes, %lld are needed", (long long)workspace_bytes, (long long)need);
     const ce::State s = ce::carve_state(state, T, nullptr);
-    return dtype == CINN_BF16 ? ce::forward<true>(x, ldx, w, ldw, target, ignore, r, reduction, loss, s, f, st)
-                              : ce::forward<false>(x, ldx, w, ldw, target, ignore, r, reduction, loss, s, f, st);
+    return dtype == CINN_BF16 ? ce::forward<true>(x, ldx, w, ldw, target, ignore, r, reduction, loss, s, f, dx_sums, dw_sums, st)
+                              : ce::forward<false>(x, ldx, w, ldw, target, ignore, r, reduction, loss, s, f, dx_sums, dw_sums, st);
+}
+
+// what is left of the early way's backward: the loss's gradient, and one rounding
+int linear_ce_finish(int dtype, const float* grad, int64_t T, int64_t V, int64_t d, int reduction, const void* state, const float* dx_sums,
+                     const float* dw_sums, void* dx, void* dw, cudaStream_t st) {
+    CINN_CHECK_ARG((dtype == CINN_BF16 || dtype == CINN_F16) && T > 0 && V > 0 && d > 0 && d % 8 == 0 && (reduction == 1 || reduction == 2), "linear_ce finish: bad arguments");
+    CINN_CHECK_ARG(grad && state && (!dx || dx_sums) && (!dw || dw_sums), "linear_ce finish: null pointer");
+    CINN_CHECK_ARG(((reinterpret_cast<uintptr_t>(dx) | reinterpret_cast<uintptr_t>(dw) | reinterpret_cast<uintptr_t>(dx_sums) |
+                     reinterpret_cast<uintptr_t>(dw_sums)) & 15) == 0, "linear_ce finish: pointers must be 16-byte aligned");
+    const ce::Plan r = ce::make_plan(T, V, d, true);
+    const ce::State s = ce::carve_state(const_cast<void*>(state), T, nullptr);
+    ce::Params p{};
+    p.n_valid = s.n_valid; p.grad = grad; p.mean = reduction == 1;
+    const bool bf16 = dtype == CINN_BF16;
+    int rc = CINN_OK;
+    if (dx) rc = bf16 ? ce::finish<true>(dx_sums, r.dx_splits, r.Tp, T, d, s.slot, p, dx, st) : ce::finish<false>(dx_sums, r.dx_splits, r.Tp, T, d, s.slot, p, dx, st);
+    if (rc || !dw) return rc;
+    return bf16 ? ce::finish<true>(dw_sums, r.dw_splits, ce::up(V, ce::M), V, d, nullptr, p, dw, st)
+                : ce::finish<false>(dw_sums, r.dw_splits, ce::up(V, ce::M), V, d, nullptr, p, dw, st);
 }
 
 int linear_ce_backward(const void* x, int64_t ldx, const void* w, int64_t ldw, int dtype, const float* grad, int64_t T, int64_t V, int64_t d,
@@ -1162,7 +1360,7 @@ int linear_ce_backward(const void* x, int64_t ldx, const void* w, int64_t ldw, i
     }
     CINN_CHECK_ARG(grad && state && workspace, "linear_ce: null pointer");
     CINN_CHECK_ARG(((reinterpret_cast<uintptr_t>(dx) | reinterpret_cast<uintptr_t>(dw)) & 15) == 0, "linear_ce: gradients must be 16-byte aligned");
-    const ce::Plan r = ce::make_plan(T, V, d);
+    const ce::Plan r = ce::make_plan(T, V, d, false);
     int64_t need = 0;
     const ce::Backward b = ce::carve_backward(workspace, r, dx != nullptr, dw != nullptr, &need);
     CINN_CHECK_ARG(workspace_bytes >= need, "linear_ce: workspace of %lld bytes, %lld are needed", (long long)workspace_bytes, (long long)need);

@@ -258,41 +258,51 @@ def _up(n, a: int):
 
 
 @torch.library.custom_op("cinnamon_b200::linear_ce_fwd", mutates_args=(), device_types="cuda")
-def linear_ce_fwd(x: Tensor, weight: Tensor, target: Tensor, ignore_index: int, reduction: int) -> Tuple[Tensor, Tensor]:
-    return K._host.linear_ce_forward(x, weight, target, ignore_index, reduction)
+def linear_ce_fwd(x: Tensor, weight: Tensor, target: Tensor, ignore_index: int, reduction: int, early: bool) -> Tuple[Tensor, Tensor, Tensor, Tensor]:
+    return K._host.linear_ce_forward(x, weight, target, ignore_index, reduction, early)
 
 
 @linear_ce_fwd.register_fake
-def _(x, weight, target, ignore_index, reduction):
-    T = x.shape[0]
+def _(x, weight, target, ignore_index, reduction, early):
+    T, d = x.shape
     state = 256 + 3 * _up(4 * T, 256) + _up(8 * T, 256) if T else 0                # cinn_linear_ce_state_bytes
-    return (torch.empty(() if reduction else (T,), dtype=torch.float32, device=x.device), torch.empty((state,), dtype=torch.uint8, device=x.device))
+    sums = [K._host.linear_ce_early(int(T), weight.shape[0], int(d), reduction, i) // 4 if early else 0 for i in (1, 2)]
+    e = lambda shape, dt: torch.empty(shape, dtype=dt, device=x.device)                         # noqa: E731
+    return e(() if reduction else (T,), torch.float32), e((state,), torch.uint8), e((sums[0],), torch.float32), e((sums[1],), torch.float32)
 
 
 @torch.library.custom_op("cinnamon_b200::linear_ce_bwd", mutates_args=(), device_types="cuda")
-def linear_ce_bwd(grad: Tensor, x: Tensor, weight: Tensor, state: Tensor, reduction: int) -> Tuple[Tensor, Tensor]:
+def linear_ce_bwd(grad: Tensor, x: Tensor, weight: Tensor, state: Tensor, dx_sums: Tensor, dw_sums: Tensor, reduction: int,
+                  early: bool) -> Tuple[Tensor, Tensor]:
+    if early:
+        return K._host.linear_ce_finish(grad, state, dx_sums, dw_sums, x, weight, reduction)
     return K._host.linear_ce_backward(grad, x, weight, state, reduction, True, True)
 
 
 @linear_ce_bwd.register_fake
-def _(grad, x, weight, state, reduction):
+def _(grad, x, weight, state, dx_sums, dw_sums, reduction, early):
     return (torch.empty(x.shape, dtype=x.dtype, device=x.device), torch.empty(weight.shape, dtype=weight.dtype, device=x.device))
 
 
 def _ce_setup(ctx, inputs, output):
-    x, weight, _, _, ctx.reduction = inputs
-    ctx.save_for_backward(x, weight, output[1])
+    x, weight, _, _, ctx.reduction, ctx.early = inputs
+    ctx.save_for_backward(x, weight, *output[1:])
     ctx.set_materialize_grads(False)
 
 
 def _ce_backward(ctx, grad, *ignored):
     if grad is None:
-        return None, None, None, None, None
-    gx, gw = torch.ops.cinnamon_b200.linear_ce_bwd(grad, *ctx.saved_tensors, ctx.reduction)
-    return gx, gw, None, None, None
+        return None, None, None, None, None, None
+    gx, gw = torch.ops.cinnamon_b200.linear_ce_bwd(grad, *ctx.saved_tensors, ctx.reduction, ctx.early)
+    return gx, gw, None, None, None, None
 
 
 linear_ce_fwd.register_autograd(_ce_backward, setup_context=_ce_setup)
+
+
+@torch.compiler.assume_constant_result
+def _ce_early(tokens: int, words: int, d: int, reduction: int) -> bool:
+    return bool(K._host.linear_ce_early(tokens, words, d, reduction, 0))
 
 
 def linear_cross_entropy(x: Tensor, weight: Tensor, target: Tensor, ignore_index: int, reduction: int) -> Tensor:
@@ -308,7 +318,8 @@ def linear_cross_entropy(x: Tensor, weight: Tensor, target: Tensor, ignore_index
     assert target.shape == x.shape[:-1] and weight.dim() == 2 and weight.shape[1] == flat.shape[1], "linear_cross_entropy: shapes"
     assert flat.dtype == weight.dtype and flat.dtype in (torch.bfloat16, torch.float16), \
         "linear_cross_entropy multiplies 16-bit operands: x and weight must both be bfloat16 or both float16 (or autocast must make them so)"
-    loss = torch.ops.cinnamon_b200.linear_ce_fwd(flat, weight, target.reshape(-1).long(), ignore_index, reduction)[0]
+    early = flat.requires_grad and weight.requires_grad and torch.is_grad_enabled() and _ce_early(flat.shape[0], weight.shape[0], flat.shape[1], reduction)
+    loss = torch.ops.cinnamon_b200.linear_ce_fwd(flat, weight, target.reshape(-1).long(), ignore_index, reduction, early)[0]
     return loss if reduction else loss.view(target.shape)
 
 

@@ -567,12 +567,20 @@ int cinn_moe_route_static(const float* logits, const float* bias, int64_t n_toke
  * reduction 0: loss (T,), one per token; 1: the mean over the tokens with a target (NaN where there is none), 2: the sum.
  * grad: (T,) or one number, fp32.  dx (T, d) and dw (V, d), contiguous, of the operands' type; either may be NULL.
  * state: cinn_linear_ce_state_bytes(T), written by the forward for the backward.  workspace: scratch of
- * cinn_linear_ce_workspace_bytes(T, V, d, pass): pass 0 = forward, 4 = backward, + 1 with dx, + 2 with dw. */
+ * cinn_linear_ce_workspace_bytes(T, V, d, pass) bytes.  Two ways to the gradients:
+ *   late   the forward with dx_sums and dw_sums NULL (pass 0); cinn_linear_ce_backward multiplies the logits once more, a piece of
+ *          the words at a time (pass 4, + 1 with dx, + 2 with dw);
+ *   early  reduction 1 or 2: the forward leaves the fp32 sums of one or both gradients (pass 1); cinn_linear_ce_finish multiplies
+ *          them by grad and rounds.  Three products instead of four, in all.  cinn_linear_ce_early(..., 0): 1 where that is
+ *          the faster way and the sums take 8 GiB at most; (..., 1) and (..., 2): the bytes of dx_sums and dw_sums. */
 int64_t cinn_linear_ce_state_bytes(int64_t T);
 int64_t cinn_linear_ce_workspace_bytes(int64_t T, int64_t V, int64_t d, int pass);
+int64_t cinn_linear_ce_early(int64_t T, int64_t V, int64_t d, int reduction, int which);
 int cinn_linear_ce_forward(const void* x, int64_t ldx, const void* w, int64_t ldw, int dtype, const int64_t* target,
                            int64_t ignore_index, int64_t T, int64_t V, int64_t d, int reduction, float* loss, void* state,
-                           void* workspace, int64_t workspace_bytes, void* stream);
+                           float* dx_sums, float* dw_sums, void* workspace, int64_t workspace_bytes, void* stream);
+int cinn_linear_ce_finish(int dtype, const float* grad, int64_t T, int64_t V, int64_t d, int reduction, const void* state,
+                          const float* dx_sums, const float* dw_sums, void* dx, void* dw, void* stream);
 int cinn_linear_ce_backward(const void* x, int64_t ldx, const void* w, int64_t ldw, int dtype, const float* grad, int64_t T,
                             int64_t V, int64_t d, int reduction, const void* state, void* dx, void* dw, void* workspace,
                             int64_t workspace_bytes, void* stream);

@@ -3,7 +3,8 @@
 Tolerances, per element, from the arithmetic (u: half a step of the operands' type, 2^-8 for bf16 and 2^-11 for fp16):
   logits   fp32 sums of exact products: ez = (d / 16 + 8) 2^-22 max_v sum_k |x_k w_vk| (sixteen products a step; a step may truncate)
   loss     2 ez, the exponentials' and the sum's 2^-20, and 2^-22 of the loss and of the maximum
-  dz       rounded once to the operands' type: u |dz|, and the probabilities' own 2 ez + 2^-20
+  dz       rounded once to the operands' type: u |dz|, and the probabilities' own 2 ez + 2^-20; made early (sums and means over 2048
+           tokens or more) from exponentials in fp16: 2^-11 of the probability more, and 2^-25 of the largest one beside it
   dx, dW   the errors of dz through the product, fp32 sums (their number of terms / 16 + 8) 2^-22 of the sum of absolute terms, and one
            rounding of the result, u |dx| (in fp16 at least half the smallest step, 2^-25)
 """
@@ -28,7 +29,7 @@ def _inputs(T, V, d, dtype, seed=0, ignored=0.0, lift=6.0):
     return x.to(dtype).cuda(), w.cuda(), target.cuda()
 
 
-def _oracle(x, w, target, grad, ignore=-100):
+def _oracle(x, w, target, grad, ignore=-100, early=False):
     """Losses, gradients and the tolerances of all three, in 64 bits.  ``grad``: the gradient of every token's loss."""
     u = HALF_STEP[x.dtype]
     tiny = 2.0 ** -25 if x.dtype == torch.float16 else 0.0
@@ -52,6 +53,8 @@ def _oracle(x, w, target, grad, ignore=-100):
     # dz is held relative to the largest gradient, in fp16 times 2^14
     held = (2.0 ** -39 if x.dtype == torch.float16 else 0.0) * (gr.abs().amax() if len(rows) else 0.0)
     e_dz = (u * dz.abs() + (1 + u) * p * (2 * ez + 2.0 ** -20)) * gr.abs() + held + 2.0 ** -22 * (dz * gr).abs()
+    if early:
+        e_dz = e_dz + (1 + u) * (2.0 ** -11 * p + 2.0 ** -25) * gr.abs()
     dz = dz * gr
     dx, dx_tol = torch.zeros(len(x), d, dtype=torch.float64, device=x.device), torch.zeros(len(x), d, dtype=torch.float64, device=x.device)
     dx[rows] = dz @ wd
@@ -94,7 +97,7 @@ def test_mean_loss_and_gradients(T, V, d, ignored, dtype):
     target[0] = V - 1                                                  # (some token counts, and the last word is hit)
     n = int((target != -100).sum())
     up = 64.0
-    want = _oracle(x, w, target, torch.full((T,), up / n, device="cuda"))
+    want = _oracle(x, w, target, torch.full((T,), up / n, device="cuda"), early=T >= 2048)
     loss, gx, gw = _run(x, w, target, torch.tensor(up, device="cuda"))
     _within(loss, want[0].sum() / n, want[1].sum() / n + 2.0 ** -23 * want[0].sum() / n, "loss")
     _within(gx, want[2], want[3], "grad_x")
@@ -121,38 +124,81 @@ def test_losses_of_tokens_with_a_gradient_each(T, V, d, ignored, dtype):
     _within(sw, want[4], want[5], "grad_w of the sum")
 
 
-def test_vocabulary_in_pieces():
-    """More than one piece of the vocabulary (a piece's gradient of the logits holds 512 MiB at most): dx is added up over them."""
-    T, V, d = 65536 + 130, 8192 + 70, 64
+@pytest.mark.parametrize("early", [False, True])
+def test_in_pieces(early):
+    """More than one piece: of the vocabulary (512 MiB of the logits' gradient), where dx is added up over them, or early of the
+    tokens (1.25 GiB), where dW is."""
+    T, V, d = (90000 if early else 65536) + 130, 8192 + 70, 64
     x, w, target = _inputs(T, V, d, torch.bfloat16, seed=5, ignored=0.01)
-    n = int((target != -100).sum())
-    loss, gx, gw = _run(x, w, target)
-    want = _oracle(x[:2048], w, target[:2048], torch.full((2048,), 1.0 / n, device="cuda"))
-    _within(gx[:2048], want[2], want[3], "grad_x")
-    # the weight's gradient, from the whole batch in pieces of rows
-    dw, tol = 0.0, 0.0
+    grad = torch.full((T,), 1.0, device="cuda")
+    n = int((target != -100).sum()) if early else 1.0
+    loss, gx, gw = _run(x, w, target) if early else _run(x, w, target, grad, reduction="none")
+    for at in (0, T - 2048):
+        want = _oracle(x[at:at + 2048], w, target[at:at + 2048], grad[:2048] / n, early=early)
+        _within(gx[at:at + 2048], want[2], want[3], "grad_x")
+        if not early:
+            _within(loss[at:at + 2048], want[0], want[1], "loss")
+    # the weight's gradient and the mean, from the whole batch in pieces of rows
+    dw, tol, total, total_tol = 0.0, 0.0, 0.0, 0.0
     for at in range(0, T, 8192):
-        part = _oracle(x[at:at + 8192], w, target[at:at + 8192], torch.full((min(8192, T - at),), 1.0 / n, device="cuda"))
-        dw, tol = dw + part[4], tol + part[5]
+        part = _oracle(x[at:at + 8192], w, target[at:at + 8192], grad[at:at + 8192] / n, early=early)
+        dw, tol, total, total_tol = dw + part[4], tol + part[5], total + part[0].sum(), total_tol + part[1].sum()
     _within(gw, dw, tol + (T / 16) * 2.0 ** -22 * tol / HALF_STEP[torch.bfloat16], "grad_w")
+    if early:
+        _within(loss, total / n, total_tol / n + 2.0 ** -23 * total / n, "loss")
 
 
-def test_well_predicted_tokens_keep_their_gradient():
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_early_gradients_alone_twice_and_late(dtype):
+    """Sums over many tokens: each gradient by itself, a backward that is run again, another scale of the loss, and the late way's result."""
+    from cinnamon_b200 import kernels as K
+    T, V, d = 2300, 1030, 136
+    x, w, target = _inputs(T, V, d, dtype, seed=T, ignored=0.25)
+    assert K._host.linear_ce_early(T, V, d, 2, 0) == 1 and K._host.linear_ce_early(T, V, d, 0, 0) == 0
+    want = _oracle(x, w, target, torch.full((T,), 3.0, device="cuda"), early=True)
+    a, b = x.clone().requires_grad_(True), w.clone().requires_grad_(True)
+    loss = K.linear_cross_entropy(a, b, target, reduction="sum")
+    three = torch.tensor(3.0, device="cuda")
+    first = torch.autograd.grad(loss, [a, b], three, retain_graph=True)
+    _within(loss.detach(), want[0].sum(), want[1].sum() + 2.0 ** -23 * want[0].sum(), "sum")
+    _within(first[0], want[2], want[3], "grad_x")
+    _within(first[1], want[4], want[5], "grad_w")
+    first[0].zero_()                                                   # (what was returned is the caller's)
+    again = torch.autograd.grad(loss, [a, b], three, retain_graph=True)
+    _within(again[0], want[2], want[3], "grad_x again")
+    assert torch.equal(again[1], first[1])
+    assert torch.equal(torch.autograd.grad(K.linear_cross_entropy(a, w, target, reduction="sum"), a, three)[0], again[0])
+    assert torch.equal(torch.autograd.grad(K.linear_cross_entropy(x, b, target, reduction="sum"), b, three)[0], again[1])
+    late = _run(x, w, target, torch.full((T,), 3.0, device="cuda"), reduction="none")
+    u = HALF_STEP[dtype]
+    for e, l in zip(again, late[1:]):
+        assert (e.float() - l.float()).norm() <= 4 * u * l.float().norm()
+    # in place after the forward: the gradients are those of the values it was called with
+    loss = K.linear_cross_entropy(a, b, target, reduction="sum")
+    with torch.no_grad():
+        assert K.linear_cross_entropy(a, b, target, reduction="sum") == loss
+
+
+@pytest.mark.parametrize("T", [256, 2304])
+def test_well_predicted_tokens_keep_their_gradient(T):
     """Targets with probabilities up to 1 - 1e-5: what is left of 1 - p has to come through."""
-    T, V, d = 256, 500, 64
+    V, d = 500, 64
     g = torch.Generator().manual_seed(1)
     w = torch.randn(V, d, generator=g).bfloat16().cuda()
     target = torch.randint(0, V, (T,), generator=g).cuda()
     x = (w[target].float() * torch.linspace(0.05, 0.6, T, device="cuda")[:, None]).bfloat16()
-    want = _oracle(x, w, target, torch.full((T,), 1.0, device="cuda"))
-    loss, gx, gw = _run(x, w, target, torch.ones(T, device="cuda"), reduction="none")
-    _within(loss, want[0], want[1], "loss")
+    early = T >= 2048
+    want = _oracle(x, w, target, torch.full((T,), 1.0, device="cuda"), early=early)
+    loss, gx, gw = _run(x, w, target, reduction="sum") if early else _run(x, w, target, torch.ones(T, device="cuda"), reduction="none")
+    if not early:
+        _within(loss, want[0], want[1], "loss")
     _within(gx, want[2], want[3], "grad_x")
 
 
+@pytest.mark.parametrize("T", [700, 2500, 5000])
 @pytest.mark.parametrize("reduction", ["mean", "sum", "none"])
-def test_ignored_rows_reach_nothing(reduction):
-    T, V, d = 700, 999, 96
+def test_ignored_rows_reach_nothing(reduction, T):
+    V, d = 999, 96
     x, w, target = _inputs(T, V, d, torch.bfloat16, seed=11, ignored=0.4)
     grad = torch.randn(T, device="cuda") if reduction == "none" else torch.tensor(1.0, device="cuda")
     clean = _run(x, w, target, grad, reduction=reduction)
@@ -168,9 +214,10 @@ def test_ignored_rows_reach_nothing(reduction):
     assert (dirty[1][bad] == 0).all()
 
 
-def test_nothing_but_ignored_rows():
-    x, w, _ = _inputs(300, 400, 64, torch.bfloat16)
-    target = torch.full((300,), -100, device="cuda")
+@pytest.mark.parametrize("T", [300, 2500])
+def test_nothing_but_ignored_rows(T):
+    x, w, _ = _inputs(T, 400, 64, torch.bfloat16)
+    target = torch.full((T,), -100, device="cuda")
     loss, gx, gw = _run(x, w, target)
     assert torch.isnan(loss) and (gx == 0).all() and (gw == 0).all()
     loss, gx, gw = _run(x, w, target, reduction="sum")
@@ -189,8 +236,9 @@ def test_no_rows():
     assert K.linear_cross_entropy(x, w, target, reduction="none").shape == (0,)
 
 
-def test_targets_that_are_no_words():
-    T, V, d = 200, 300, 64
+@pytest.mark.parametrize("T", [200, 4500])
+def test_targets_that_are_no_words(T):
+    V, d = 300, 64
     x, w, target = _inputs(T, V, d, torch.bfloat16, seed=2)
     bad = target.clone()
     bad[3], bad[77], bad[150] = V, -1, 1 << 40
@@ -299,9 +347,10 @@ def test_gradient_against_differences():
         assert slack < 0.2 * abs(diff) or abs(diff) < 1.0
 
 
-def test_other_streams_and_a_captured_step():
+@pytest.mark.parametrize("T", [400, 2400])
+def test_other_streams_and_a_captured_step(T):
     from cinnamon_b200 import kernels as K
-    x, w, target = _inputs(400, 1500, 128, torch.bfloat16, seed=21, ignored=0.2)
+    x, w, target = _inputs(T, 1500, 128, torch.bfloat16, seed=21, ignored=0.2)
     ref = _run(x, w, target)
     side = torch.cuda.Stream()
     side.wait_stream(torch.cuda.current_stream())
@@ -320,7 +369,7 @@ def test_other_streams_and_a_captured_step():
                 loss = K.linear_cross_entropy(xs, ws, ts)
                 gx, gw = torch.autograd.grad(loss, [xs, ws])
         graphs.append((graph, loss, gx, gw))
-    x2, w2, t2 = _inputs(400, 1500, 128, torch.bfloat16, seed=22, ignored=0.6)
+    x2, w2, t2 = _inputs(T, 1500, 128, torch.bfloat16, seed=22, ignored=0.6)
     want = _run(x2, w2, t2)
     with torch.no_grad():
         xs.copy_(x2), ws.copy_(w2), ts.copy_(t2)
@@ -332,9 +381,10 @@ def test_other_streams_and_a_captured_step():
             assert torch.equal(a, b)
 
 
-def test_a_cap_on_the_sms_changes_no_bits():
+@pytest.mark.parametrize("T", [600, 2600])
+def test_a_cap_on_the_sms_changes_no_bits(T):
     from cinnamon_b200 import kernels as K
-    x, w, target = _inputs(600, 2000, 128, torch.bfloat16, seed=31)
+    x, w, target = _inputs(T, 2000, 128, torch.bfloat16, seed=31)
     ref = _run(x, w, target)
     try:
         for cap in (1, 2, 37):

@@ -135,15 +135,16 @@ def test_step_captured_and_replayed():
         _close(a, b, name)
 
 
-def test_cross_entropy_and_rotary_compile_as_one_graph():
+@pytest.mark.parametrize("L", [40, 1200])                              # (the second: gradients made early)
+def test_cross_entropy_and_rotary_compile_as_one_graph(L):
     from cinnamon_b200 import kernels as K
     g = torch.Generator().manual_seed(3)
-    x, w = torch.randn(2, 40, 100, generator=g).cuda(), (torch.randn(300, 100, generator=g) * 0.1).cuda()
-    target = torch.randint(0, 300, (2, 40), generator=g).cuda()
+    x, w = torch.randn(2, L, 100, generator=g).cuda(), (torch.randn(300, 100, generator=g) * 0.1).cuda()
+    target = torch.randint(0, 300, (2, L), generator=g).cuda()
     target[0, :7] = -100
-    q, k = (torch.randn(2, h, 40, 64, generator=g).bfloat16().cuda() for h in (4, 1))
+    q, k = (torch.randn(2, h, L, 64, generator=g).bfloat16().cuda() for h in (4, 1))
     freq, _ = K.rotary_frequencies(32, device="cuda")
-    positions = torch.arange(40, device="cuda") + 1000
+    positions = torch.arange(L, device="cuda") + 1000
 
     def head(x, w):
         return K.linear_cross_entropy(x, w, target), K.linear_cross_entropy(x, w, target, reduction="none")
