@@ -21,6 +21,7 @@ void check_rotary(const Tensor& q, const Tensor& k, const Tensor& positions, con
             "rotary: positions are (positions,) or (batch, positions)");
     require(freq.dim() == 1 && freq.numel() >= 1 && (freq.scalar_type() == at::kDouble || freq.scalar_type() == at::kFloat),
             "rotary: inv_freq is one number for every pair, float64 (or float32)");
+    require(!(at::GradMode::is_enabled() && freq.requires_grad()), "rotary: inv_freq takes no gradient");
 }
 
 Tensor heads_of(const Tensor& t) { return t.stride(-1) == 1 || t.numel() == 0 || t.size(-1) == 1 ? t : t.contiguous(); }

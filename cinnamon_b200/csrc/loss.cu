@@ -12,9 +12,8 @@
 //           (fp32, in L2) and write the piece's rows of dW.  2 T V d forward and 6 T V d backward, one 2 T V d more than with kept logits.
 //   early   The tokens in pieces; a piece's e^(z - maximum of its 128 words) is written in fp16 by the forward's product, turned into dz by one
 //           pass over it once the sums are known, and the two products add up dx and dW in fp32, all in the forward.  What is left for the
-//           backward is the loss's gradient, one number, and the one rounding.  6 T V d in all: what bounds these products is the power of
-//           the matrix units, so the fourth product is a fifth of the time; but the sums of dW stay until the backward, and a
-//           loss whose gradient is never asked for has cost three times as much.  For sums and means over many tokens (early_pays).
+//           backward is the loss's gradient, one number, and the one rounding.  6 T V d in all.  The sums stay until the backward, and a
+//           loss whose gradient is never asked for has cost three times as much.  For sums and means over many and wide rows (early_pays).
 // The memory is that of one piece, and early that of the gradients' sums.
 //
 // Tokens whose target is ignored take part in nothing: the others' rows are gathered first (where none is ignored, x is read
@@ -984,30 +983,31 @@ grad_max_kernel(const float* __restrict__ grad, const int* __restrict__ slot, in
     if ((threadIdx.x & 31) == 0 && most) atomicMax(out, most);
 }
 
-// out[r] = scale * sum of the splits' sums of r's row, rounded once; slot (null: every row its own) -1 or -2: zeros
+// out[r] = scale * sum of the splits' sums of r's row, rounded once; slot (null: every row its own) -1 or -2: zeros.  Eight columns a thread.
 template <bool BF16>
 __global__ void __launch_bounds__(256)
 finish_kernel(const float* __restrict__ sums, int splits, int64_t split_elems, int rows, int d, const int* __restrict__ slot, const Params p,
-              uint2* __restrict__ out) {
+              uint4* __restrict__ out) {
     pdl_wait();
     pdl_trigger();
-    const int vecs = d / 4;
+    const int vecs = d / 8;
     const int64_t n = (int64_t)rows * vecs;
     const float scale = final_scale(p, BF16);
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
         const int r = (int)(i / vecs), c = (int)(i - (int64_t)r * vecs);
         const int from = slot ? slot[r] : r;
-        float4 a = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        float a[8] = {};
         if (from >= 0) {
-            const float* at = sums + (int64_t)from * d + c * 4;
-            a = *reinterpret_cast<const float4*>(at);
-            for (int s = 1; s < splits; ++s) {
-                const float4 b = *reinterpret_cast<const float4*>(at + s * split_elems);
-                a.x += b.x; a.y += b.y; a.z += b.z; a.w += b.w;
+            const float* at = sums + (int64_t)from * d + c * 8;
+            for (int s = 0; s < splits; ++s, at += split_elems) {
+                const float4 u = __ldcs(reinterpret_cast<const float4*>(at)), v = __ldcs(reinterpret_cast<const float4*>(at) + 1);
+                a[0] += u.x; a[1] += u.y; a[2] += u.z; a[3] += u.w;
+                a[4] += v.x; a[5] += v.y; a[6] += v.z; a[7] += v.w;
             }
-            a.x *= scale; a.y *= scale; a.z *= scale; a.w *= scale;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) a[j] *= scale;
         }
-        out[i] = make_uint2(pack2<BF16>(a.x, a.y), pack2<BF16>(a.z, a.w));
+        out[i] = make_uint4(pack2<BF16>(a[0], a[1]), pack2<BF16>(a[2], a[3]), pack2<BF16>(a[4], a[5]), pack2<BF16>(a[6], a[7]));
     }
 }
 
@@ -1031,8 +1031,8 @@ constexpr int64_t PART_BYTES = 48LL << 20;
 constexpr int64_t DZ_BYTES = 512LL << 20;  // most of a piece of dz: smaller pieces cost passes over dx, larger ones only memory
 
 constexpr int64_t EARLY_BYTES = 5LL << 28; // the same of a piece of tokens: beyond the first one dW is added to, in memory
-constexpr int64_t EARLY_TOKENS = 2048;     // from here on the early way saves more than the sums of dW cost
-constexpr int64_t EARLY_KEPT = 8LL << 30;  // most of what it leaves for the backward
+constexpr int64_t EARLY_TOKENS = 2048, EARLY_WIDTH = 1024;               // see early_pays
+constexpr int64_t EARLY_KEPT = 8LL << 30;  // most of what the early way leaves for the backward
 
 static Plan make_plan(int64_t T, int64_t V, int64_t d, bool early) {
     Plan r{};
@@ -1069,10 +1069,12 @@ static Plan make_plan(int64_t T, int64_t V, int64_t d, bool early) {
 
 static int64_t dx_sums_bytes(const Plan& r) { return 4 * r.dx_splits * r.Tp * r.d; }
 static int64_t dw_sums_bytes(const Plan& r) { return 4 * r.dw_splits * up(r.V, M) * r.d; }
-// Whether both gradients of a sum or mean are made in the forward.  What it saves, a product of 2 T V d at 1.3e15 a second, is more than what it
-// costs, 10 V d bytes of sums at 6e12, from some 1100 tokens on.
+// Whether both gradients of a sum or mean are made in the forward.  That saves a product, which goes with d, and costs a pass over the piece and
+// an epilogue that reads its tile twice, which do not, and 10 bytes of sums for each element of dW, which does not go with the tokens.  us
+// late and early, in bf16: 8192 tokens x 512 to 32000 words 970 and 1060, 768 1400 and 1370, 1024 1810 and 1700, 2048 3440 and 3050; 1024 tokens x 2048
+// 490 and 513, 1536 697 and 676, 2048 891 and 847; 2048 x 4096 to 128000 6870 and 6490, 16384 x 2048 to 128000 27.5 and 24.7 ms.
 static bool early_pays(int64_t T, int64_t V, int64_t d, int reduction) {
-    if (reduction == 0 || T < EARLY_TOKENS) return false;
+    if (reduction == 0 || T < EARLY_TOKENS || d < EARLY_WIDTH) return false;
     const Plan r = make_plan(T, V, d, true);
     return dx_sums_bytes(r) + dw_sums_bytes(r) <= EARLY_KEPT;
 }
@@ -1229,8 +1231,8 @@ static int forward(const void* x, int64_t ldx, const void* w, int64_t ldw, const
 
 template <bool BF16>
 static int finish(const float* sums, int splits, int64_t split_rows, int64_t rows, int64_t d, const int* slot, const Params& p, void* out, cudaStream_t st) {
-    launch_dependent(finish_kernel<BF16>, dim3(grid_for(rows * (d / 4), 256)), dim3(256), 0, st, sums, splits, split_rows * d, (int)rows, (int)d, slot, p,
-                     static_cast<uint2*>(out));
+    launch_dependent(finish_kernel<BF16>, dim3(grid_for(rows * (d / 8), 256)), dim3(256), 0, st, sums, splits, split_rows * d, (int)rows, (int)d, slot, p,
+                     static_cast<uint4*>(out));
     CINN_CHECK_LAUNCH();
     return CINN_OK;
 }

@@ -848,7 +848,7 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, target: torch.Te
     """``F.cross_entropy(F.linear(x, weight).float(), target, ...)`` of an output projection (the reference's ``lm_head`` and
     loss, src/train.py:338-376) without the logits in memory: forward and both gradients are made from ``x`` and ``weight``
     tile by tile.  Beside inputs and gradients a call holds a piece of the logits' gradient at a time: 512 MiB, or 256 words for more than a
-    million tokens.  A mean or sum over 2048 tokens or more whose gradients are wanted makes them in the forward, in three products in
+    million tokens.  A mean or sum over 2048 rows or more of 1024 or more whose gradients are wanted makes them in the forward, in three products in
     place of four: it holds 1.25 GiB meanwhile and the gradients' fp32 sums until its backward (where these are 8 GiB at most), and under
     ``torch.no_grad()`` none of it.
 

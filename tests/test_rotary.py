@@ -219,6 +219,8 @@ def test_refusals():
                        ((q.double(), None, p, freq), "bfloat16"), ((q, k, p.cpu(), freq), "CUDA"), ((q, k, p, freq.repeat(3)), "do not fit")]:
         with pytest.raises(AssertionError, match=what):
             K.rotary(*args)
+    with pytest.raises(AssertionError, match="no gradient"):
+        K.rotary(q, k, p, freq.clone().requires_grad_(True))
     for start in (17, -15, -33):
         with pytest.raises(AssertionError, match="do not fit"):
             K.rotary(q, k, p, freq, start=start)

@@ -175,6 +175,20 @@ def test_groups_whose_experts_are_banned(low):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("E,n_groups,top_groups,k", [(1, 1, 1, 1), (32, 32, 5, 5), (8, 8, 3, 3), (64, 32, 16, 32), (1024, 32, 1, 32), (96, 3, 1, 32), (512, 4, 1, 32),
+                                                     (1024, 8, 8, 32)])
+def test_groups_of_one_and_all_of_a_lane(E, n_groups, top_groups, k):
+    """Groups of a single expert, every expert of the open groups, and more of the best in one lane than it keeps."""
+    from cinnamon_b200 import kernels as K
+    g = torch.Generator().manual_seed(E)
+    for scores in ("sigmoid", "softmax"):
+        logits = torch.randn(70, E, generator=g)
+        logits[:, :k] += 3.0
+        r = K.moe_route(logits.cuda(), None, k, scores=scores, n_groups=n_groups, top_groups=top_groups)
+        assert torch.equal(r["top_experts"].cpu(), _choose(logits, None, k, scores, n_groups, top_groups)[1].int())
+
+
+@pytest.mark.gpu
 def test_the_references_form_keeps_its_bits_and_gains_a_gradient():
     from cinnamon_b200 import kernels as K
     g = torch.Generator().manual_seed(1)

@@ -135,11 +135,11 @@ def test_step_captured_and_replayed():
         _close(a, b, name)
 
 
-@pytest.mark.parametrize("L", [40, 1200])                              # (the second: gradients made early)
-def test_cross_entropy_and_rotary_compile_as_one_graph(L):
+@pytest.mark.parametrize("L,d", [(40, 100), (1200, 1025)])               # (the second: gradients made early)
+def test_cross_entropy_and_rotary_compile_as_one_graph(L, d):
     from cinnamon_b200 import kernels as K
     g = torch.Generator().manual_seed(3)
-    x, w = torch.randn(2, L, 100, generator=g).cuda(), (torch.randn(300, 100, generator=g) * 0.1).cuda()
+    x, w = torch.randn(2, L, d, generator=g).cuda(), (torch.randn(300, d, generator=g) * 0.1).cuda()
     target = torch.randint(0, 300, (2, L), generator=g).cuda()
     target[0, :7] = -100
     q, k = (torch.randn(2, h, L, 64, generator=g).bfloat16().cuda() for h in (4, 1))
