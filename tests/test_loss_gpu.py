@@ -4,7 +4,8 @@ Tolerances, per element, from the arithmetic (u: half a step of the operands' ty
   logits   fp32 sums of exact products: ez = (d / 16 + 8) 2^-22 max_v sum_k |x_k w_vk| (sixteen products a step; a step may truncate)
   loss     2 ez, the exponentials' and the sum's 2^-20, and 2^-22 of the loss and of the maximum
   dz       rounded once to the operands' type: u |dz|, and the probabilities' own 2 ez + 2^-20; made early (sums and means over 2048
-           rows or more of 1024 or more) from exponentials in fp16: 2^-11 of the probability more, and 2^-25 of the largest one beside it
+           rows or more of 1024 or more) from exponentials in fp16: 2^-11 of the probability more, and 2^-25 of the largest one beside it;
+           for up to 128 rows held in two parts: u^2 |dz| in place of u |dz|
   dx, dW   the errors of dz through the product, fp32 sums (their number of terms / 16 + 8) 2^-22 of the sum of absolute terms, and one
            rounding of the result, u |dx| (in fp16 at least half the smallest step, 2^-25)
 """
@@ -29,7 +30,7 @@ def _inputs(T, V, d, dtype, seed=0, ignored=0.0, lift=6.0):
     return x.to(dtype).cuda(), w.cuda(), target.cuda()
 
 
-def _oracle(x, w, target, grad, ignore=-100, early=False):
+def _oracle(x, w, target, grad, ignore=-100, early=False, few=False):
     """Losses, gradients and the tolerances of all three, in 64 bits.  ``grad``: the gradient of every token's loss."""
     u = HALF_STEP[x.dtype]
     tiny = 2.0 ** -25 if x.dtype == torch.float16 else 0.0
@@ -52,7 +53,7 @@ def _oracle(x, w, target, grad, ignore=-100, early=False):
     gr = grad[rows].double()[:, None]
     # dz is held relative to the largest gradient, in fp16 times 2^14
     held = (2.0 ** -39 if x.dtype == torch.float16 else 0.0) * (gr.abs().amax() if len(rows) else 0.0)
-    e_dz = (u * dz.abs() + (1 + u) * p * (2 * ez + 2.0 ** -20)) * gr.abs() + held + 2.0 ** -22 * (dz * gr).abs()
+    e_dz = ((u * u if few else u) * dz.abs() + (1 + u) * p * (2 * ez + 2.0 ** -20)) * gr.abs() + held + 2.0 ** -22 * (dz * gr).abs()
     if early:
         e_dz = e_dz + (1 + u) * (2.0 ** -11 * p + 2.0 ** -25) * gr.abs()
     dz = dz * gr
@@ -410,3 +411,20 @@ def test_refusals():
     a = x.detach().requires_grad_(True)
     with pytest.raises(AssertionError, match="second derivative"):
         torch.autograd.grad(call(a, w, target), a, create_graph=True)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("reduction", ["mean", "none"])
+@pytest.mark.parametrize("T,V,d,ignored", [(1, 700, 64, 0.0), (2, 33, 200, 0.0), (3, 1000, 512, 0.3), (31, 300, 72, 0.0), (32, 300, 72, 0.5), (33, 2000, 256, 0.0),
+                                           (64, 513, 128, 0.0), (65, 513, 128, 0.4), (127, 4000, 64, 0.2), (128, 260, 1032, 0.0), (128, 32000, 512, 0.9)])
+def test_a_few_tokens_lose_nothing_to_dz(T, V, d, ignored, reduction, dtype):
+    """One token's dz is a factor of all that it adds: its rounding would not average out."""
+    x, w, target = _inputs(T, V, d, dtype, seed=T + V, ignored=ignored, lift=14.0)
+    target[0] = V // 2
+    n = int((target >= 0).sum())
+    grad = torch.randn(T, generator=torch.Generator().manual_seed(5)).cuda() if reduction == "none" else None
+    loss, gx, gw = _run(x, w, target, grad, reduction)
+    per = grad if reduction == "none" else torch.full((T,), 1.0 / n, device="cuda")
+    _, _, dx, dx_tol, dw, dw_tol = _oracle(x, w, target, per, few=True)
+    _within(gx, dx, dx_tol, "dx")
+    _within(gw, dw, dw_tol, "dw")
