@@ -326,8 +326,8 @@ __device__ __forceinline__ void stage16(uint32_t box, int row, int piece, uint32
     asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(box + row * 128 + ((piece ^ (row & 7)) << 4)), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
 // An epilogue warp's two boxes, in turn: `open` waits until the one to be filled has been read by its last store (the one after may still
-// be on its way), `send` hands it over.  (All boxes of a tile by a warp of their own, behind a barrier of all warps: dz of 32768 x 8192 words took
-// 227 us, the tile's conversion and its stores one after the other.)
+// be on its way), `send` hands it over: a tile's conversion and its stores run beside one another, where one warp for all of a tile's stores, behind a
+// barrier of all warps, put them one after the other.
 struct Boxes {
     uint32_t slot, turn = 0;
     __device__ __forceinline__ Boxes(uint32_t s) : slot(s) {}
@@ -358,8 +358,8 @@ __device__ __forceinline__ uint64_t pair2(float a, float b) {
 }
 
 // The logits' product: A = x, B = W, both K-major.  STATS leaves maxima and sums of its runs, SOFT dz of the piece, KEEP both maxima and sums, and
-// e^(z - maximum) in fp16, of each half tile.  xg: x's rows in use,
-// gathered; read in x's place where some token is ignored.
+// e^(z - maximum) in fp16, of each half tile.  xg: x's rows in use, gathered; read in x's place where some token is ignored.  Bound by the tensor cores
+// (active 87.6 % of STATS at 8192 x 32000 x 512, 74 % of SOFT, which also writes dz) and, in long calls, by the power that they draw.
 template <int MODE, bool BF16>
 __global__ void __launch_bounds__(THREADS, 1)
 product_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b, const __grid_constant__ CUtensorMap tm_xg,
@@ -630,7 +630,7 @@ product_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__
 
 // Both gradients of a piece.  dx tiles: A = dz as stored, B = W, MN-major; fp32 sums, stored or added (the pieces run one after the other, so
 // the order of a sum is always the same).  dW tiles: A = dz's transpose, B = x, both MN-major; the piece's rows of dW, complete, scaled and
-// rounded, or with DW_SUMS the fp32 sums of a cut reduction.
+// rounded, or with DW_SUMS the fp32 sums of a cut reduction.  Bound as the logits' product is (tensor cores active 84.5 % at 8192 x 32000 x 512).
 struct GradMaps { CUtensorMap z_rows, z_cols, w_cols, x_cols, xg_cols, c_dx, c_dw; };
 
 template <bool BF16, bool DW_SUMS>

@@ -18,6 +18,7 @@
 // heads.  What TMA cannot read goes through a kernel of plain loads and stores.
 #include "tma.cuh"
 #include <algorithm>
+#include <cmath>
 
 namespace cinn {
 namespace rope {
@@ -70,6 +71,7 @@ template <typename T, int VEC> struct alignas(sizeof(T) * VEC) Piece { T v[VEC];
 __device__ __forceinline__ float2 turn_of(int64_t position, double freq) {
     double turns = freq * 0.15915494309189533577;
     turns -= floor(turns);
+    if (!(turns >= 0.0)) return make_float2(NAN, NAN);                               // (a frequency that is no number, or infinite)
     const uint64_t unit = __double2ull_rn(turns * 18446744073709551616.0);           // 2^64 (a whole turn saturates: off by 2^-64)
     const uint64_t at = unit * (uint64_t)position;
     const uint64_t quadrant = (at + (1ull << 61)) >> 62;

@@ -148,7 +148,8 @@ class MoE(nn.Module):
         if self.balance_alpha > 0 and shared_out.requires_grad:
             plain = plain and all(type(e) is SwiGLU and not K.has_hooks(e) and K.swiglu_block_ready(x, e.w1, e.w2, e.w3)
                                   for e in self.shared_experts)
-        return (plain and (reference or self.balance_alpha <= 0) and not self.sharded and flat.shape[0] > 0 and not torch.compiler.is_compiling() and K.gemm_events is None
+        return (plain and (reference or self.balance_alpha <= 0) and not self.sharded and flat.shape[0] > 0
+                and not torch.compiler.is_compiling() and K.gemm_events is None
                 and K._MOE_GROUPED_PRECISION == "fp8" and ex.d_model % 256 == 0 and ex.hidden_dim % 256 == 0
                 and all(w.dtype in (torch.float32, torch.bfloat16) and w.is_contiguous() for w in (ex.w12, ex.w3))
                 and flat.dtype in K._DTYPE_TAG and shared_out.dtype in K._DTYPE_TAG and self.expert_bias.dtype == torch.float32

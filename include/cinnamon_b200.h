@@ -537,7 +537,8 @@ int cinn_moe_route_form(const void* logits, int logits_dtype, const float* bias,
                         int64_t* pair_pos, float* pair_gate, void* stream);
 int cinn_moe_route_form_backward(const void* logits, int logits_dtype, const int* top_experts, const int64_t* sorted_experts,
                                  const int64_t* pair_pos, const float* d_top_gates, const float* d_pair_gate,
-                                 const float* d_sorted_scores, int64_t n_tokens, int n_experts, int top_k, int scores, int renormalise, float scale, void* d_logits, void* stream);
+                                 const float* d_sorted_scores, int64_t n_tokens, int n_experts, int top_k, int scores, int renormalise,
+                                 float scale, void* d_logits, void* stream);
 
 /* cinn_moe_route for callers that have no device memory to give as a workspace and may not allocate any: a
  * serving process that handed all of HBM to its own arena at start-up, a job running at the memory limit, a

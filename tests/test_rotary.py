@@ -49,6 +49,18 @@ def _heads(B, H, L, d, dtype, seed, first=False):
     return x.transpose(1, 2) if first else x.transpose(1, 2).contiguous()
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_a_frequency_that_is_no_number_reaches_its_pair_alone(dtype):
+    from cinnamon_b200 import kernels as K
+    q = _heads(1, 2, 3, 72, dtype, 5)
+    freq, _ = K.rotary_frequencies(32, device="cuda")
+    freq[3], freq[7] = float("nan"), float("inf")
+    out, _ = K.rotary(q, None, torch.arange(3, device="cuda"), freq, interleaved=True, start=8)
+    nan = torch.isnan(out)[0].all(0).all(0).cpu()
+    assert nan.tolist() == [i in (14, 15, 22, 23) for i in range(72)] and torch.isnan(out).sum() == 2 * 3 * 4
+
+
 # batch, heads of q and k, positions, elements of q and k, rotated, start
 SHAPES = [
     (1, 1, 1, 1, 2, 2, 2, 0), (2, 3, 1, 5, 64, 64, 64, 0), (1, 8, 8, 130, 192, 192, 64, -64), (3, 7, 2, 33, 96, 40, 32, 8),
