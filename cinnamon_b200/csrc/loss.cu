@@ -1051,7 +1051,8 @@ struct Plan {
 };
 
 constexpr int64_t PART_BYTES = 48LL << 20;
-constexpr int64_t DZ_BYTES = 512LL << 20;  // most of a piece of dz: smaller pieces cost passes over dx, larger ones only memory
+constexpr int64_t DZ_BYTES = 512LL << 20;  // most of a piece of dz: smaller pieces cost passes over dx, larger ones only memory (32768 tokens x 512 to 32000 words
+                                           // with 128 MiB 5.0 ms, 256 3.92, 512 3.89, 1024 3.85, 2048 3.87)
 
 // Up to FEW tokens, dz stands in two parts, rounded and what the rounding left, in rows of their own: a tile has 256 anyway, x's rows stand twice behind
 // one another, and dW sums over twice as many.  Where a gradient is made of a few tokens, each one's dz is a factor of all that it adds and its rounding
