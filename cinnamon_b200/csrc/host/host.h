@@ -117,6 +117,21 @@ inline void* stream() { return at::cuda::getCurrentCUDAStream().stream(); }
 inline bool capturing() {
     return stream() != nullptr && c10::cuda::currentStreamCaptureStatusMayInitCtx() != c10::cuda::CaptureStatus::None;
 }
+// Whether the input's own step of a backward pass belongs to the null stream: an earlier graph of a leaf that still lives, or one that `t` comes
+// from, was recorded on it.  A captured backward pass would wait for that stream, which breaks the capture in a thread of autograd's.
+inline bool differentiates_on_null_stream(const Tensor& t) {
+    if (!t.defined() || !t.requires_grad()) return false;
+    const auto node = t.grad_fn() ? t.grad_fn() : torch::autograd::impl::try_get_grad_accumulator(t);
+    if (!node) return false;
+    const auto s = node->stream();
+    return s.has_value() && c10::cuda::CUDAStream(*s).stream() == nullptr;
+}
+template <typename... T>
+void check_capture(const char* who, const T&... t) {
+    if (at::GradMode::is_enabled() && capturing() && (differentiates_on_null_stream(t) || ...))
+        throw CinnError(std::string(who) + ": a step that is captured with its gradients must not share its inputs with a graph recorded on the "
+                        "default stream that still lives (drop that loss, or record it on a stream of its own)", true);
+}
 inline float* f32(const Tensor& t);
 Tensor gemm(const Tensor& a, const Tensor& sa, const Tensor& b, int layout, const Tensor& sb, int64_t sbk, int64_t sbn, int64_t M,
             int64_t N, int64_t K, at::ScalarType type, int tag);               // linear.cpp

@@ -194,6 +194,7 @@ void bind_moe(pybind11::module_& m) {
         RouteCall c{bias.has_value() ? bias->detach() : Tensor(), top_k, route_form(form), {}};
         const int64_t T = logits.size(0), E = logits.size(1), pairs = T * top_k;
         Tensor top, pair, sorted;
+        check_capture("moe_route", logits);
         if (takes_node(logits)) {
             const auto v = RouteNode::apply(logits, &c);
             top = v[0]; pair = v[1]; sorted = v[2];

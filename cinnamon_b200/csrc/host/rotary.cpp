@@ -96,6 +96,7 @@ void bind_rotary(pybind11::module_& m) {
         const Tensor positions = positions_in.to(at::kLong), freq = freq_in.detach().to(at::kDouble).contiguous();
         const Form f{start, magnitude, interleaved};
         std::array<Tensor, 2> r;
+        check_capture("rotary", q, k);
         if (!inverse && (k.defined() ? takes_node(q, k) : takes_node(q))) {
             const auto v = RotaryNode::apply(q, k.defined() ? c10::optional<Tensor>(k) : c10::nullopt, positions, freq, &f);
             r = {v[0], v.size() > 1 ? v[1] : Tensor()};

@@ -135,6 +135,45 @@ def test_step_captured_and_replayed():
         _close(a, b, name)
 
 
+@pytest.mark.parametrize("op", ["loss", "loss_padded", "rotary", "route", "route_reference"])
+def test_capture_beside_a_living_graph_of_the_default_stream_is_refused(op):
+    """Its backward pass would wait for the default stream, which no capture may."""
+    from cinnamon_b200 import kernels as K
+    g = torch.Generator().manual_seed(4)
+    d = 70 if op == "loss_padded" else 64
+    x, w = (torch.randn(40, d, generator=g).cuda().bfloat16().requires_grad_(True) for _ in range(2))
+    q = torch.randn(1, 2, 40, 64, generator=g).cuda().requires_grad_(True)
+    target, positions, bias = torch.arange(40, device="cuda"), torch.arange(40, device="cuda"), torch.zeros(d, device="cuda")
+    freq, _ = K.rotary_frequencies(32, device="cuda")
+    calls = {"loss": lambda: K.linear_cross_entropy(x, w, target), "loss_padded": lambda: K.linear_cross_entropy(x, w, target),
+             "rotary": lambda: K.rotary(q, q.detach(), positions, freq)[0].sum(),
+             "route": lambda: K.moe_route(x, bias, 2, scores="softmax")["top_gates"].sum(),
+             "route_reference": lambda: K.moe_route(x, bias, 2)["top_gates"].sum()}
+    leaves = [q] if op == "rotary" else [x] if op.startswith("route") else [x, w]
+    call = calls[op]
+    earlier = call()
+    want = torch.autograd.grad(earlier, leaves, retain_graph=True)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        with pytest.raises(AssertionError, match="default stream"):
+            with torch.cuda.graph(torch.cuda.CUDAGraph(), stream=side):
+                call()
+        with torch.no_grad(), torch.cuda.graph(torch.cuda.CUDAGraph(), stream=side):    # (without gradients there is nothing to refuse)
+            call()
+        del earlier
+        call()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            got = torch.autograd.grad(call(), leaves)
+    torch.cuda.current_stream().wait_stream(side)
+    graph.replay()
+    torch.cuda.synchronize()
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
+    assert K.device_status() == 0
+
+
 @pytest.mark.parametrize("L,d", [(40, 100), (1200, 1025)])               # (the second: gradients made early)
 def test_cross_entropy_and_rotary_compile_as_one_graph(L, d):
     from cinnamon_b200 import kernels as K
