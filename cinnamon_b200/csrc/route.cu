@@ -538,7 +538,9 @@ route_form_kernel(const L* __restrict__ logits, const float* __restrict__ bias, 
 
 // d logits of the gates, from their gradients by slot (d_top), in the order of pair_pos (d_pair) and by sorted pair (d_sorted); null: none.  One warp per
 // token; d score of a chosen expert is scale * d gate, or with renormalised gates scale * (d gate - sum_j d gate_j s_j / S) / S, S = sum of
-// the chosen s + 1e-9; then s (1 - s) d, or for a softmax s_e (d_e - sum_j d_j s_j).  Bound by reading and writing the logits.
+// the chosen s + 1e-9; then s (1 - s) d, or for a softmax s_e (d_e - sum_j d_j s_j).  Two of these differences cancel, wholly so for a single
+// chosen expert, whose gate is 1 - 1e-9 / S whatever its score; they are taken as what is left: (sum_j s_j (d gate - d gate_j) + 1e-9 d gate) / S^2,
+// and 1e-9 sum_j d gate_j s_j / S^2.  Bound by reading and writing the logits.
 template <int VPL, typename L, bool SOFTMAX>
 __global__ void __launch_bounds__(256)
 route_form_backward_kernel(const L* __restrict__ logits, const int* __restrict__ top_experts, const int64_t* __restrict__ sorted_experts,
@@ -591,12 +593,17 @@ route_form_backward_kernel(const L* __restrict__ logits, const int* __restrict__
             }
         }
         g *= form.scale;
+        float common = 0.0f;
         if (form.renormalise) {
-            const float total = warp_sum(s) + 1e-9f, dot = warp_sum(g * s);
-            g = lane < top_k ? (g - dot / total) / total : 0.0f;
+            const float total = warp_sum(s) + 1e-9f;
+            if (SOFTMAX) common = 1e-9f * warp_sum(g * s) / total / total;
+            float d = 1e-9f * g;
+            for (int j = 0; j < top_k; ++j) d = fmaf(__shfl_sync(0xffffffffu, s, j), g - __shfl_sync(0xffffffffu, g, j), d);
+            g = lane < top_k ? d / total / total : 0.0f;
+        } else if (SOFTMAX) {
+            common = warp_sum(g * s);
         }
-        float d = SOFTMAX ? s * g : s * (1.0f - s) * g;                        // of the chosen expert (softmax: before the sum's part)
-        const float common = SOFTMAX ? warp_sum(d) : 0.0f;
+        float d = s * (1.0f - s) * g;
         float out[VPL];
 #pragma unroll
         for (int i = 0; i < VPL; ++i) out[i] = SOFTMAX ? -(x[i] * inv) * common : 0.0f;

@@ -332,3 +332,24 @@ def test_block_on_the_cpu_and_refusals():
     for bad in (dict(n_groups=3), dict(n_groups=8, top_groups=1), dict(scores="max"), dict(n_groups=2, top_groups=3)):
         with pytest.raises(AssertionError):
             _block(moe.RouterForm(**bad))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("scores", ["sigmoid", "softmax"])
+@pytest.mark.parametrize("E", [16, 60, 257])
+def test_the_gradient_of_a_single_renormalised_gate_is_what_is_left(E, scores, dtype):
+    """The gate is s / (s + 1e-9): its derivative 1e-9 / (s + 1e-9)^2 is far below the rounding of what cancels.  Three quotients and sums in fp32 of
+    relative error 2^-23 each, the score's own 2^-21 three times over, 1 - s from a score near 1: 2^-23 / (1 - s)."""
+    from cinnamon_b200 import kernels as K
+    g = torch.Generator().manual_seed(E)
+    logits = torch.randn(300, E, generator=g).to(dtype).cuda().requires_grad_(True)
+    d = torch.randn(300, 1, generator=g).cuda()
+    r = K.moe_route(logits, None, 1, scores=scores, n_groups=1 if scores == "softmax" or E == 257 else 2, scale=2.0)
+    got, = torch.autograd.grad(r["top_gates"], logits, d)
+    x = logits.detach().double().requires_grad_(True)
+    s = (torch.sigmoid(x) if scores == "sigmoid" else torch.softmax(x, -1)).gather(-1, r["top_experts"].long())
+    want, = torch.autograd.grad(2.0 * s / (s + 1e-9), x, d.double())
+    half = 2.0 ** -8 if dtype == torch.bfloat16 else 0.0
+    tol = want.abs() * (half + 2.0 ** -18 + 2.0 ** -22 / (1 - s.detach()).clamp(min=1e-6)) + 2.0 ** -133
+    assert ((got.double() - want).abs() <= tol).all()
