@@ -75,6 +75,7 @@ struct Params {
     const float* grad;                     // the loss's gradient: one number, or one per token
     const unsigned* grad_max;              // the bits of the largest |gradient| (reduction "none")
     int mean;
+    float log2e;                           // of one unit of the logits as they stand in tensor memory (see growth)
     uint16_t* dz;                          // the piece's (KEEP: what it will be made of), rows of dz_ld (a multiple of 64)
     int dz_ld;
 };
@@ -479,9 +480,9 @@ product_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__
 #pragma unroll
                         for (int j = 0; j < 32; ++j) top = fmaxf(top, __uint_as_float(r[j]));
                         const float base = top == -INFINITY ? 0.0f : top;
-                        float part[4] = {sum * exp2_approx((mx - base) * LOG2E), 0.0f, 0.0f, 0.0f};
+                        float part[4] = {sum * exp2_approx((mx - base) * p.log2e), 0.0f, 0.0f, 0.0f};
 #pragma unroll
-                        for (int j = 0; j < 32; ++j) part[j & 3] += exp2_approx((__uint_as_float(r[j]) - base) * LOG2E);
+                        for (int j = 0; j < 32; ++j) part[j & 3] += exp2_approx((__uint_as_float(r[j]) - base) * p.log2e);
                         sum = (part[0] + part[1]) + (part[2] + part[3]);
                         mx = top;
                     }
@@ -513,7 +514,7 @@ product_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__
                         }
                     }
                     const float base = top == -INFINITY ? 0.0f : top;
-                    const uint64_t minus = pair2(-base, -base), scale = pair2(LOG2E, LOG2E);
+                    const uint64_t minus = pair2(-base, -base), scale = pair2(p.log2e, p.log2e);
                     float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
                     for (int c = 0; c < COLS / 32; ++c) {
@@ -552,10 +553,10 @@ product_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__
                     }
                     if (live) p.tile_max[(int64_t)(nt * 2 + h) * p.part_ld + row] = base;
                     const float best = fmaxf(mx, top), from = best == -INFINITY ? 0.0f : best;
-                    sum = sum * exp2_approx((mx - from) * LOG2E) + ((part[0] + part[1]) + (part[2] + part[3])) * exp2_approx((top - from) * LOG2E);
+                    sum = sum * exp2_approx((mx - from) * p.log2e) + ((part[0] + part[1]) + (part[2] + part[3])) * exp2_approx((top - from) * p.log2e);
                     mx = best;
                 } else {
-                    const uint64_t minus = pair2(-mx, -mx), scale = pair2(LOG2E, LOG2E), logs = pair2(-sum, -sum), rels = pair2(rel, rel);
+                    const uint64_t minus = pair2(-mx, -mx), scale = pair2(p.log2e, p.log2e), logs = pair2(-sum, -sum), rels = pair2(rel, rel);
                     uint32_t r[2][32];                     // a chunk of 32 words at work, the next one on its way
                     ld32(taddr, r[0]);
 #pragma unroll
@@ -899,12 +900,13 @@ constexpr int JOIN = 16;                   // warps of a block: each joins every
 // The tensor cores cut off what a step of 16 products leaves below the running sum's last bit, which puts a logit off by up to d / 16 such bits, towards zero.
 // Among the other words most of that averages out; the target's logit is the one that a loss hangs on.  So it is multiplied once more in plain fp32, and its
 // term in the sum exchanged for that: loss = log(1 + sum of the others e^(z - z_target)).  Relative errors for 5000 words: one token of 512 up to
-// 1.2e-5 -> 3.1e-7, 200 of 2048 8e-7 -> 2.2e-7, of 7168 2.8e-6 -> 2.4e-6; 1531 tokens of 512 to 32000 words scored 53.5 -> 54.6 us.
+// 1.2e-5 -> 3.1e-7, 200 of 2048 8e-7 -> 2.2e-7, and with growth 7e-8; of 7168 2.8e-6 -> 2.4e-6, and with growth 3e-7; 1531 tokens of 512 to 32000 words scored 53.5 -> 54.6 us.
 template <bool BF16>
 __global__ void __launch_bounds__(32 * JOIN)
 loss_kernel(const float2* __restrict__ part, int64_t part_ld, int parts, const float* __restrict__ target_logit, State s, int T, int reduction,
             double* __restrict__ block_sum, float* __restrict__ loss, int t0, int tc, int last, const uint4* __restrict__ x, int64_t ldx,
-            const uint4* __restrict__ w, int64_t ldw, int vecs) {
+            const uint4* __restrict__ w, int64_t ldw, int vecs, float grown) {
+    const float log2e = LOG2E * grown;
     pdl_wait();
     pdl_trigger();
     __shared__ float2 s_part[JOIN][32];
@@ -916,7 +918,7 @@ loss_kernel(const float2* __restrict__ part, int64_t part_ld, int parts, const f
     float mx = -INFINITY, sum = 0.0f;
     auto join = [&](float2 v) {
         const float top = fmaxf(mx, v.x), base = top == -INFINITY ? 0.0f : top;
-        sum = sum * exp2f((mx - base) * LOG2E) + v.y * exp2f((v.x - base) * LOG2E);
+        sum = sum * exp2f((mx - base) * log2e) + v.y * exp2f((v.x - base) * log2e);
         mx = top;
     };
     if (row >= 0) {
@@ -952,9 +954,9 @@ loss_kernel(const float2* __restrict__ part, int64_t part_ld, int parts, const f
 #pragma unroll
             for (int w = 1; w < JOIN; ++w) join(s_part[w][lane]);
             s.stat[row] = make_float2(mx, log2f(sum));
-            float others = sum - exp2f((target_logit[row] - mx) * LOG2E);      // (the term as it was added: exact where it is the largest)
+            float others = sum - exp2f((target_logit[row] - mx) * log2e);      // (the term as it was added: exact where it is the largest)
             others = others < 0.0f ? 0.0f : others;
-            const float over = mx - s_logit[lane];
+            const float over = mx * grown - s_logit[lane];
             l = over > 0.0f ? over + logf(others + exp2f(-over * LOG2E)) : log1pf(others * exp2f(over * LOG2E));
         }
         if (reduction == 0) loss[t] = l;
@@ -1006,7 +1008,7 @@ soften_kernel(const Params p) {
         const int row = (int)(i / per), at = (int)(i - (int64_t)row * per) * 32 + lane;
         if (at >= vecs) continue;
         const float2 st = p.stat[p.t0 + row];
-        const float f = exp2_approx((p.tile_max[(int64_t)(at / 16) * p.part_ld + row] - st.x) * LOG2E - st.y);
+        const float f = exp2_approx((p.tile_max[(int64_t)(at / 16) * p.part_ld + row] - st.x) * p.log2e - st.y);
         uint4* q = reinterpret_cast<uint4*>(p.dz + (int64_t)row * p.dz_ld) + at;
         uint4 v = *q;
         uint32_t* h = &v.x;
@@ -1186,6 +1188,12 @@ static Backward carve_backward(void* mem, const Plan& r, bool want_dx, bool want
     return b;
 }
 
+// What a logit z = x w has lost on its way through tensor memory is made good for by as much as it loses on average.  A step of 16 products cuts the running
+// sum off below its last bit: half such a bit, about 0.36 2^-23 of the sum (mantissas spread as logarithms are); and after k of K steps the sum is z k / K
+// on average, whatever the order.  That makes 0.36 K 2^-24 of z.  Measured, in units of K 2^-24, d from 256 to 7168: bf16 0.25 to 0.28 for the words that a
+// softmax is made of, 0.29 to 0.42 for z of 12 to 30, scattered by a tenth of that; fp16 0.3 and, its products having more bits to lose, 0.5 to 1.1.
+static float growth(int64_t d) { return 1.0f + 0.3f * (float)(d / 16) * 0x1p-24f; }
+
 template <auto KERN, size_t SMEM_BYTES, typename... A>
 static int launch(cudaStream_t st, A&&... args) {
     int rc = allow_smem_once<KERN>(SMEM_BYTES);
@@ -1256,11 +1264,12 @@ static int forward(const void* x, int64_t ldx, const void* w, int64_t ldw, const
     if ((rc = map16(&tb, w, r.d, r.V, ldw, 128, BF16))) return rc;
     Params p{};
     p.n_valid = s.n_valid; p.T = (int)r.T; p.V = (int)r.V; p.d = (int)r.d; p.vc = (int)r.V; p.tc = (int)r.tc; p.parts = r.parts;
+    p.log2e = LOG2E * growth(r.d);
     p.part = f.part; p.part_ld = r.tc; p.target_logit = f.target_logit; p.target = s.target; p.stat = s.stat;
     auto join = [&](int last) {
         launch_dependent(loss_kernel<BF16>, dim3((unsigned)ceil_div(r.T, 32)), dim3(32 * JOIN), 0, st, f.part, r.tc, 2 * r.parts, f.target_logit, s, (int)r.T,
                          reduction, f.block_sum, loss, p.t0, p.tc, last, static_cast<const uint4*>(x), ldx / 8, static_cast<const uint4*>(w), ldw / 8,
-                         (int)(r.d / 8));
+                         (int)(r.d / 8), growth(r.d));
         CINN_CHECK_LAUNCH();
         return (int)CINN_OK;
     };
@@ -1308,7 +1317,7 @@ static int backward(const void* x, int64_t ldx, const void* w, int64_t ldw, cons
     Params p{};
     p.n_valid = s.n_valid; p.T = r.half ? -1 : (int)r.T; p.V = (int)r.V; p.d = (int)r.d; p.tc = (int)r.Tp; p.half = (int)r.half;
     p.target = s.target; p.rows = s.rows; p.stat = s.stat; p.grad = grad; p.grad_max = b.grad_max;
-    p.per_row = reduction == 0; p.mean = reduction == 1;
+    p.per_row = reduction == 0; p.mean = reduction == 1; p.log2e = LOG2E * growth(r.d);
     if (p.per_row) {
         CINN_CHECK_CUDA(cudaMemsetAsync(b.grad_max, 0, 4, st));
         launch_dependent(grad_max_kernel, dim3(grid_for(r.T, 1024)), dim3(256), 0, st, grad, s.slot, (int)r.T, b.grad_max);
