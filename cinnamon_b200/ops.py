@@ -23,6 +23,7 @@ from typing import List, Tuple
 
 import torch
 from torch import Tensor
+from torch.fx.experimental.symbolic_shapes import has_static_value
 
 from . import kernels as K
 from . import sparse_attention as SA
@@ -318,7 +319,10 @@ def linear_cross_entropy(x: Tensor, weight: Tensor, target: Tensor, ignore_index
     assert target.shape == x.shape[:-1] and weight.dim() == 2 and weight.shape[1] == flat.shape[1], "linear_cross_entropy: shapes"
     assert flat.dtype == weight.dtype and flat.dtype in (torch.bfloat16, torch.float16), \
         "linear_cross_entropy multiplies 16-bit operands: x and weight must both be bfloat16 or both float16 (or autocast must make them so)"
-    early = flat.requires_grad and weight.requires_grad and torch.is_grad_enabled() and _ce_early(flat.shape[0], weight.shape[0], flat.shape[1], reduction)
+    # the gradients' sums have sizes that only known ones give: a call that is traced for any number of tokens makes them in its backward
+    known = has_static_value(flat.shape[0]) and has_static_value(weight.shape[0]) and has_static_value(flat.shape[1])
+    early = (known and flat.requires_grad and weight.requires_grad and torch.is_grad_enabled()
+             and _ce_early(flat.shape[0], weight.shape[0], flat.shape[1], reduction))
     loss = torch.ops.cinnamon_b200.linear_ce_fwd(flat, weight, target.reshape(-1).long(), ignore_index, reduction, early)[0]
     return loss if reduction else loss.view(target.shape)
 

@@ -203,3 +203,34 @@ def test_cross_entropy_and_rotary_compile_as_one_graph(L, d):
         results.append([mean.detach(), each.detach(), oq.detach(), ok.detach(), *grads])
     for a, b in zip(*results):
         assert a.shape == b.shape and torch.equal(a, b)
+
+
+@pytest.mark.parametrize("dynamic", [True, None])
+def test_compiled_loss_over_many_token_counts(dynamic):
+    """One function traced for any number of tokens, through the border of the gradients that are made in the forward (at a width they are made
+    for), against 64 bits; with and without a frozen weight, and the tokens' losses to the bit."""
+    from cinnamon_b200 import kernels as K
+    from test_loss_gpu import _inputs, _oracle, _within
+
+    def mean(x, w, t):
+        return K.linear_cross_entropy(x, w, t)
+
+    def each(x, w, t):
+        return K.linear_cross_entropy(x, w, t, reduction="none")
+
+    torch._dynamo.reset()
+    f, e = torch.compile(mean, fullgraph=True, dynamic=dynamic), torch.compile(each, fullgraph=True, dynamic=dynamic)
+    for T in (130, 257, 2300, 150, 1, 2049):
+        x, w, target = _inputs(T, 300, 1024, torch.bfloat16, seed=T)
+        x.requires_grad_(True)
+        assert torch.equal(e(x.detach(), w, target), each(x.detach(), w, target))
+        want = _oracle(x.detach(), w, target, torch.full((T,), 1 / T, device="cuda"), early=T >= 2048)
+        for frozen in (False, True):
+            w = w.detach().requires_grad_(not frozen)
+            loss = f(x, w, target)
+            grads = torch.autograd.grad(loss, [x] if frozen else [x, w])
+            _within(loss.detach(), want[0].sum() / T, want[1].sum() / T + 2.0 ** -23 * want[0].sum() / T, "loss")
+            _within(grads[0], want[2], want[3], "grad_x")
+            if not frozen:
+                _within(grads[1], want[4], want[5], "grad_w")
+    assert K.device_status() == 0
