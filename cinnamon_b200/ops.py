@@ -317,6 +317,7 @@ def linear_cross_entropy(x: Tensor, weight: Tensor, target: Tensor, ignore_index
     if odd:
         flat, weight = (torch.nn.functional.pad(t, (0, 8 - odd)) for t in (flat, weight))
     assert target.shape == x.shape[:-1] and weight.dim() == 2 and weight.shape[1] == flat.shape[1], "linear_cross_entropy: shapes"
+    assert target.dtype in (torch.int64, torch.int32), "linear_cross_entropy: targets are int64 or int32"
     assert flat.dtype == weight.dtype and flat.dtype in (torch.bfloat16, torch.float16), \
         "linear_cross_entropy multiplies 16-bit operands: x and weight must both be bfloat16 or both float16 (or autocast must make them so)"
     # the gradients' sums have sizes that only known ones give: a call that is traced for any number of tokens makes them in its backward

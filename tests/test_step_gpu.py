@@ -234,3 +234,16 @@ def test_compiled_loss_over_many_token_counts(dynamic):
             if not frozen:
                 _within(grads[1], want[4], want[5], "grad_w")
     assert K.device_status() == 0
+
+
+def test_compiled_refusals():
+    """What the eager call refuses is refused under torch.compile too."""
+    from cinnamon_b200 import kernels as K
+    x, w = torch.zeros(5, 64, device="cuda", dtype=torch.bfloat16), torch.zeros(7, 64, device="cuda", dtype=torch.bfloat16)
+    t = torch.zeros(5, device="cuda", dtype=torch.int64)
+    f = torch.compile(lambda x, w, t: K.linear_cross_entropy(x, w, t))
+    for args in ((x, w, t.float()), (x, w, t[:4]), (x.float(), w, t), (x, w[:, :56], t)):
+        torch._dynamo.reset()
+        with pytest.raises(Exception, match="linear_cross_entropy"):
+            f(*args)
+    assert torch.isfinite(f(x, w, t.int()))
