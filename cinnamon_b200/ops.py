@@ -357,5 +357,6 @@ rotate.register_autograd(_rotate_backward, setup_context=_rotate_setup)
 
 
 def rotary(q, k, positions, inv_freq, interleaved, start, magnitude):
+    assert not (torch.is_grad_enabled() and inv_freq.requires_grad), "rotary: inv_freq takes no gradient"
     out = torch.ops.cinnamon_b200.rotate([q] if k is None else [q, k], positions, inv_freq, interleaved, start, magnitude, False)
     return out[0], None if k is None else out[1]

@@ -247,3 +247,15 @@ def test_compiled_refusals():
         with pytest.raises(Exception, match="linear_cross_entropy"):
             f(*args)
     assert torch.isfinite(f(x, w, t.int()))
+
+
+def test_compiled_rotary_refuses_a_gradient_of_the_frequencies():
+    from cinnamon_b200 import kernels as K
+    q, p = torch.zeros(1, 2, 5, 64, device="cuda"), torch.arange(5, device="cuda")
+    freq = K.rotary_frequencies(32, device="cuda")[0].requires_grad_(True)
+    torch._dynamo.reset()
+    f = torch.compile(lambda q, freq: K.rotary(q, None, p, freq)[0])
+    with pytest.raises(Exception, match="takes no gradient"):
+        f(q, freq)
+    with torch.no_grad():
+        assert torch.equal(f(q, freq), q)
