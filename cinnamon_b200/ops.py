@@ -13,7 +13,8 @@ below wrap forward and backward of the differentiable entry points as opaque nod
   cinnamon_b200::rotate                               rotary (its derivative is itself, the other way round)
 
 Each operator body runs the very code of the eager ``autograd.Function`` (its ``forward`` / ``backward`` static
-methods, handed a stand-in context), so compiled and eager results are the same bits.  ``FP8Linear.forward``,
+methods, handed a stand-in context), so compiled and eager results are the same bits (but for ``linear_cross_entropy`` traced for
+any number of tokens, whose gradients are never made in the forward).  ``FP8Linear.forward``,
 ``moe_grouped_gemm``, ``sparse_attention``, ``linear_cross_entropy`` and ``rotary`` switch to the operators while ``torch.compiler.is_compiling()``; in
 eager mode they keep calling the autograd functions directly, as the reference does.
 """
