@@ -137,6 +137,12 @@ struct RouteCall {
     int64_t top_k;
     RouteForm form;
     Routes out;
+    Tensor experts, sorted_experts, pos;                     // as the caller gets them
+    void parts(int64_t T) {
+        experts = part_of(out.top, 0, {T, top_k});
+        sorted_experts = part_of(out.longs, out.pairs, {out.pairs});
+        pos = part_of(out.longs, 2 * out.pairs, {T, top_k});
+    }
 };
 
 // gates by slot, in the order of pair_pos and by sorted pair, from the logits
@@ -148,11 +154,13 @@ struct RouteNode : public torch::autograd::Function<RouteNode> {
         Tensor top;
         c->out = route(logits, c->bias, c->top_k, c->form, &top);
         const Routes& r = c->out;
-        ctx->save_for_backward({logits, r.top, r.longs});
+        const int64_t T = logits.size(0);
+        // the caller's own tensors: what they are changed to in place is not what was chosen, and their versions tell
+        c->parts(T);
+        ctx->save_for_backward({logits, c->experts, c->sorted_experts, c->pos});
         ctx->saved_data["n"] = std::vector<int64_t>{c->top_k, c->form.scores, c->form.renormalise, (int64_t)logits_in.scalar_type()};
         ctx->saved_data["scale"] = c->form.scale;
         ctx->set_materialize_grads(false);
-        const int64_t T = logits.size(0);
         return {part_of(top, 0, {T, c->top_k}), part_of(r.floats, r.pairs, {T, c->top_k}), part_of(r.floats, 0, {r.pairs})};
     }
     static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
@@ -164,15 +172,13 @@ struct RouteNode : public torch::autograd::Function<RouteNode> {
             const Tensor& logits = s[0];
             c10::cuda::CUDAGuard guard(logits.device());
             const int64_t T = logits.size(0), E = logits.size(1);
-            Routes r;
-            r.longs = s[2]; r.pairs = T * n[0]; r.E = E;
             Tensor g[3];
             for (int i = 0; i < 3; ++i)
                 if (grads[i].defined()) g[i] = grads[i].to(at::kFloat).contiguous();
             auto at = [&](int i) { return g[i].defined() ? f32(g[i]) : nullptr; };
             d = empty({T, E}, logits.scalar_type(), logits.device());
-            check(api.cinn_moe_route_form_backward(logits.data_ptr(), tag_of(logits.scalar_type()), s[1].data_ptr<int>(), r.sorted_experts(), r.pos(), at(0), at(1),
-                                                   at(2), T, (int)E, (int)n[0], (int)n[1], (int)n[2], (float)ctx->saved_data["scale"].toDouble(), d.data_ptr(),
+            check(api.cinn_moe_route_form_backward(logits.data_ptr(), tag_of(logits.scalar_type()), s[1].data_ptr<int>(), s[2].data_ptr<int64_t>(),
+                                                   s[3].data_ptr<int64_t>(), at(0), at(1), at(2), T, (int)E, (int)n[0], (int)n[1], (int)n[2], (float)ctx->saved_data["scale"].toDouble(), d.data_ptr(),
                                                    stream()), "cinn_moe_route backward");
             d = d.to((at::ScalarType)n[3]);
         });
@@ -200,21 +206,22 @@ void bind_moe(pybind11::module_& m) {
             top = v[0]; pair = v[1]; sorted = v[2];
         } else {
             c.out = route(logits, c.bias, top_k, c.form, &top);
+            c.parts(T);
             top = part_of(top, 0, {T, top_k});
             pair = part_of(c.out.floats, pairs, {T, top_k});
             sorted = part_of(c.out.floats, 0, {pairs});
         }
         const Routes& r = c.out;
         pybind11::dict out;
-        out["top_experts"] = part_of(r.top, 0, {T, top_k});
+        out["top_experts"] = c.experts;
         out["top_gates"] = top;
         out["token_indices"] = part_of(r.longs, 0, {pairs});
         out["sorted_scores"] = sorted;
-        out["sorted_experts"] = part_of(r.longs, pairs, {pairs});
+        out["sorted_experts"] = c.sorted_experts;
         out["counts"] = r.counts();
         out["starts"] = r.starts();
         out["ends"] = r.ends();
-        out["pair_pos"] = part_of(r.longs, 2 * pairs, {T, top_k});
+        out["pair_pos"] = c.pos;
         out["pair_gate"] = pair;
         return out;
     });

@@ -573,18 +573,25 @@ route_form_backward_kernel(const L* __restrict__ logits, const int* __restrict__
         float s = 0.0f, g = 0.0f;
         if (lane < top_k) {
             mine = top_experts[t * top_k + lane];
-            const float v = logit<L>(row[mine]);
-            s = SOFTMAX ? expf(v - m) * inv : __fdiv_rn(1.0f, 1.0f + expf(-v));
-            if (d_top) g = d_top[t * top_k + lane];
+            if ((unsigned)mine < (unsigned)E) {
+                const float v = logit<L>(row[mine]);
+                s = SOFTMAX ? expf(v - m) * inv : __fdiv_rn(1.0f, 1.0f + expf(-v));
+                if (d_top) g = d_top[t * top_k + lane];
+            } else {
+                mine = -1;                                                     // (not what the forward wrote: no part in anything)
+            }
         }
         if (d_pair || d_sorted) {                                              // lane j: the token's j-th pair, its expert and its gradient
             int e = -2;
             float h = 0.0f;
             if (lane < top_k) {
                 const int64_t at = pair_pos[t * top_k + lane];
-                e = (int)sorted_experts[at];
-                if (d_pair) h = d_pair[t * top_k + lane];
-                if (d_sorted) h += d_sorted[at];
+                if (at >= 0 && at < T * top_k) {
+                    const int64_t chosen = sorted_experts[at];
+                    if (chosen >= 0 && chosen < E) e = (int)chosen;
+                    if (d_pair) h = d_pair[t * top_k + lane];
+                    if (d_sorted) h += d_sorted[at];
+                }
             }
             for (int j = 0; j < top_k; ++j) {
                 const int ej = __shfl_sync(0xffffffffu, e, j);

@@ -1041,7 +1041,7 @@ def moe_route(logits: torch.Tensor, bias: torch.Tensor, top_k: int, scores: str 
     ``top_experts`` (T, k) int32, ``top_gates`` (T, k), ``token_indices`` / ``sorted_scores`` /
     ``sorted_experts`` (T*k), ``counts`` and the row ranges ``starts`` / ``ends`` (E) int64, ``pair_pos`` / ``pair_gate`` (T, k).
     Where ``logits`` requires a gradient, it reaches them through ``top_gates``, ``pair_gate`` and ``sorted_scores`` (the gates by
-    slot, by rising position, by expert).
+    slot, by rising position, by expert); the backward reads ``top_experts``, ``sorted_experts`` and ``pair_pos``, and refuses them changed in place.
 
     The router's other forms: ``scores`` "softmax" over the experts; ``n_groups`` (1 to 32) groups of equally many neighbouring experts, of which
     the ``top_groups`` whose two best scores + bias add up to the most are open to a token; gates without ``renormalise``, the scores as

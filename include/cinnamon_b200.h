@@ -529,7 +529,8 @@ int cinn_moe_route_ranges(const void* logits, int logits_dtype, const float* bia
  * renormalise 0 scale * score.  bias: NULL = none.  workspace: cinn_moe_route_form_workspace_ints ints.
  * No counterpart in the reference, whose router has one form.
  * cinn_moe_route_form_backward: d_logits (n_tokens, n_experts) of logits' type from the gradients of top_gates, pair_gate and
- * sorted_scores (NULL: none), for the experts that were chosen; sorted_experts and pair_pos are read for the last two only. */
+ * sorted_scores (NULL: none), for the experts that were chosen; sorted_experts and pair_pos are read for the last two only.  An expert or a
+ * pair of theirs that there is not has no part in it. */
 int64_t cinn_moe_route_form_workspace_ints(int64_t n_tokens, int n_experts);
 int cinn_moe_route_form(const void* logits, int logits_dtype, const float* bias, int64_t n_tokens, int n_experts, int top_k, int scores,
                         int n_groups, int top_groups, int renormalise, float scale, int* workspace, int* top_experts, float* top_gates,

@@ -353,3 +353,41 @@ def test_the_gradient_of_a_single_renormalised_gate_is_what_is_left(E, scores, d
     half = 2.0 ** -8 if dtype == torch.bfloat16 else 0.0
     tol = want.abs() * (half + 2.0 ** -18 + 2.0 ** -22 / (1 - s.detach()).clamp(min=1e-6)) + 2.0 ** -133
     assert ((got.double() - want).abs() <= tol).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("scores,renormalise", [("softmax", True), ("sigmoid", False), ("sigmoid", True)])
+@pytest.mark.parametrize("gates", ["top_gates", "pair_gate", "sorted_scores"])
+def test_outputs_changed_in_place_before_the_backward(gates, scores, renormalise):
+    """What the backward reads cannot be changed unnoticed (a sharded caller that makes expert ids local does it); what it does not read can."""
+    from cinnamon_b200 import kernels as K
+    x = torch.randn(70, 32, device="cuda").requires_grad_(True)
+    form = dict(scores=scores, renormalise=renormalise, scale=2.0)
+    up = torch.randn(70, 4, device="cuda")
+
+    def call():
+        r = K.moe_route(x, None, 4, **form)
+        return r, lambda: torch.autograd.grad(r[gates], x, up.view(r[gates].shape))[0]
+    want = call()[1]()
+    for name in ("top_experts", "sorted_experts", "pair_pos"):
+        r, back = call()
+        r[name] -= 16
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            back()
+    r, back = call()
+    for name in ("token_indices", "counts", "starts", "ends"):
+        r[name].fill_(-7)
+    with torch.no_grad():
+        r["top_gates" if gates != "top_gates" else "pair_gate"].zero_()
+    assert torch.equal(back(), want)
+    # past the versions, ids that there are none of have no part in it
+    r, back = call()
+    r["top_experts"].data.fill_(1 << 30)
+    assert (back() == 0).all()
+    for bad in (-1, 70 * 4, 1 << 40):
+        r, back = call()
+        r["pair_pos"].data.fill_(bad)
+        r["sorted_experts"].data.fill_(bad)
+        got = back()
+        assert torch.equal(got, want) if gates == "top_gates" else (got == 0).all()
+    assert K.device_status() == 0
