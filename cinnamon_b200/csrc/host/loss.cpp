@@ -125,7 +125,7 @@ void bind_loss(pybind11::module_& m) {
     m.def("linear_ce_early", [](int64_t T, int64_t V, int64_t d, int64_t reduction, int which) { return api.cinn_linear_ce_early(T, V, d, (int)reduction, which); });
     // (loss, state, sums of dx, sums of dw); the sums are empty in the late way
     m.def("linear_ce_forward", [](const Tensor& x, const Tensor& w, const Tensor& target, int64_t ignore, int64_t reduction, bool early) {
-        CrossEntropy r = ce_forward(rows_of(x), rows_of(w), target, ignore, reduction, early, early);
+        CrossEntropy r = ce_forward(rows_of(x), rows_of(w), target.contiguous(), ignore, reduction, early, early);
         if (!early) {
             r.dx_sums = empty({0}, at::kFloat, x.device());
             r.dw_sums = empty({0}, at::kFloat, x.device());

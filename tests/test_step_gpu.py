@@ -259,3 +259,25 @@ def test_compiled_rotary_refuses_a_gradient_of_the_frequencies():
         f(q, freq)
     with torch.no_grad():
         assert torch.equal(f(q, freq), q)
+
+
+@pytest.mark.parametrize("dtype", [torch.int64, torch.int32])
+def test_compiled_loss_of_targets_with_strides(dtype):
+    """A column, every other token, one target for all: read as the eager call reads them."""
+    from cinnamon_b200 import kernels as K
+    g = torch.Generator().manual_seed(6)
+    x, w = torch.randn(90, 64, generator=g).cuda().bfloat16(), torch.randn(300, 64, generator=g).cuda().bfloat16()
+    table = torch.randint(0, 300, (180, 3), generator=g).cuda().to(dtype)
+    call = lambda x, w, t: K.linear_cross_entropy(x, w, t, reduction="none")      # noqa: E731
+    for target in (table[:90, 1], table[::2, 0], table[0, :1].expand(90), table[:90, 2].flip(0)):
+        torch._dynamo.reset()
+        results = []
+        for f in (torch.compile(call, fullgraph=True), call):
+            a, b = x.clone().requires_grad_(True), w.clone().requires_grad_(True)
+            loss = f(a, b, target)
+            results.append([loss.detach(), *torch.autograd.grad(loss.sum(), [a, b])])
+        for got, want in zip(*results):
+            assert torch.equal(got, want)
+    leaf = x.clone().requires_grad_(True)                                # the operator by itself
+    got = torch.ops.cinnamon_b200.linear_ce_fwd(leaf, w, table[:90, 1].long(), -100, 0, False)[0]
+    assert torch.equal(got, call(leaf, w, table[:90, 1]))
