@@ -118,6 +118,23 @@ std::tuple<Tensor, Tensor, Tensor> ce_operands(const Tensor& x_in, const Tensor&
     return {x, w, target_in.reshape({-1}).to(at::kLong).contiguous()};
 }
 
+// The calls below are operators of a compiled graph, which hands over what it is given: everything that the kernels rely on is looked at here.
+void check_flat(const Tensor& x, const Tensor& w) {
+    require(x.is_cuda() && w.is_cuda(), "Inputs must be on CUDA");
+    require(x.device() == w.device(), "linear_cross_entropy: x, weight and target must be on the same device");
+    require(x.dim() == 2 && w.dim() == 2 && x.size(1) == w.size(1) && x.size(1) > 0 && x.size(1) % 8 == 0 && w.size(0) > 0,
+            "linear_cross_entropy: x is (tokens, d) and weight (vocabulary, d), d a multiple of 8");
+    require(x.scalar_type() == w.scalar_type() && (x.scalar_type() == at::kBFloat16 || x.scalar_type() == at::kHalf),
+            "linear_cross_entropy multiplies 16-bit operands");
+}
+void check_part(const Tensor& t, const Tensor& x, at::ScalarType type, int64_t numel) {
+    require(t.device() == x.device() && t.scalar_type() == type && t.numel() == numel && t.is_contiguous(),
+            "linear_cross_entropy: not what the forward left for this backward");
+}
+void check_grad(const Tensor& grad, const Tensor& x, int64_t reduction) {
+    require(grad.device() == x.device() && grad.numel() == (reduction ? 1 : x.size(0)), "linear_cross_entropy: the loss's gradient does not fit it");
+}
+
 }  // namespace
 
 void bind_loss(pybind11::module_& m) {
@@ -125,6 +142,9 @@ void bind_loss(pybind11::module_& m) {
     m.def("linear_ce_early", [](int64_t T, int64_t V, int64_t d, int64_t reduction, int which) { return api.cinn_linear_ce_early(T, V, d, (int)reduction, which); });
     // (loss, state, sums of dx, sums of dw); the sums are empty in the late way
     m.def("linear_ce_forward", [](const Tensor& x, const Tensor& w, const Tensor& target, int64_t ignore, int64_t reduction, bool early) {
+        check_flat(x, w);
+        require(target.device() == x.device(), "linear_cross_entropy: x, weight and target must be on the same device");
+        require(target.scalar_type() == at::kLong && target.dim() == 1 && target.size(0) == x.size(0), "linear_cross_entropy: target has one int64 for every row of x");
         CrossEntropy r = ce_forward(rows_of(x), rows_of(w), target.contiguous(), ignore, reduction, early, early);
         if (!early) {
             r.dx_sums = empty({0}, at::kFloat, x.device());
@@ -134,9 +154,17 @@ void bind_loss(pybind11::module_& m) {
     });
     m.def("linear_ce_finish", [](const Tensor& grad, const Tensor& state, const Tensor& dx_sums, const Tensor& dw_sums, const Tensor& x, const Tensor& w,
                                  int64_t reduction) {
+        check_flat(x, w);
+        check_grad(grad, x, reduction);
+        check_part(state, x, at::kByte, api.cinn_linear_ce_state_bytes(x.size(0)));
+        check_part(dx_sums, x, at::kFloat, api.cinn_linear_ce_early(x.size(0), w.size(0), x.size(1), (int)reduction, 1) / 4);
+        check_part(dw_sums, x, at::kFloat, api.cinn_linear_ce_early(x.size(0), w.size(0), x.size(1), (int)reduction, 2) / 4);
         return ce_finish(grad, state, dx_sums, dw_sums, x.size(0), w.size(0), x.size(1), x.scalar_type(), reduction);
     });
     m.def("linear_ce_backward", [](const Tensor& grad, const Tensor& x, const Tensor& w, const Tensor& state, int64_t reduction, bool want_x, bool want_w) {
+        check_flat(x, w);
+        check_grad(grad, x, reduction);
+        check_part(state, x, at::kByte, api.cinn_linear_ce_state_bytes(x.size(0)));
         return ce_backward(grad, rows_of(x), rows_of(w), state, reduction, want_x, want_w);
     });
     m.def("linear_cross_entropy", [](const Tensor& x_in, const Tensor& w_in, const Tensor& target_in, int64_t ignore, int64_t reduction) {

@@ -310,6 +310,8 @@ def _ce_early(tokens: int, words: int, d: int, reduction: int) -> bool:
 def linear_cross_entropy(x: Tensor, weight: Tensor, target: Tensor, ignore_index: int, reduction: int) -> Tensor:
     """The operands as the native call makes them (csrc/host/loss.cpp), in operations that can be traced; its checks of shapes and types are
     the operators' own."""
+    assert x.is_cuda and weight.is_cuda and target.is_cuda, "linear_cross_entropy: Inputs must be on CUDA"
+    assert x.device == weight.device and x.device == target.device, "linear_cross_entropy: x, weight and target must be on the same device"
     flat = x.reshape(-1, x.shape[-1])
     if torch.is_autocast_enabled("cuda"):
         dtype = torch.get_autocast_dtype("cuda")

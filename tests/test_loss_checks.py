@@ -1,0 +1,33 @@
+"""What ``linear_cross_entropy``'s operators look at before anything reaches a kernel; no GPU is needed for it (tensors without memory stand for those of one)."""
+import pytest
+import torch
+from torch._subclasses.fake_tensor import FakeTensorMode
+
+
+def _operands(T=6, V=20, d=64):
+    x, w = torch.empty(T, d, dtype=torch.bfloat16, device="cuda"), torch.empty(V, d, dtype=torch.bfloat16, device="cuda")
+    return x, w, torch.empty(T, dtype=torch.int64, device="cuda")
+
+
+def test_operators_of_a_compiled_graph_refuse_what_the_kernels_cannot_read():
+    from cinnamon_b200 import kernels as K
+    forward, backward, finish = K._host.linear_ce_forward, K._host.linear_ce_backward, K._host.linear_ce_finish
+    with FakeTensorMode():
+        x, w, t = _operands()
+        here = dict(dtype=torch.bfloat16)
+        for a, b, c, what in [(torch.empty(6, 64, **here), torch.empty(20, 64, **here), torch.empty(6, dtype=torch.int64), "CUDA"),
+                              (x, torch.empty(20, 64, **here), t, "CUDA"), (x, w, torch.empty(6, dtype=torch.int64), "same device"),
+                              (x, w, t[:5], "one int64"), (x, w, t.int(), "one int64"), (x, w, t[:, None], "one int64"), (x, w[:, :56], t, "multiple of 8"),
+                              (x[:, :60], w[:, :60], t, "multiple of 8"), (x, w[:0], t, "multiple of 8"), (x[None], w, t, "multiple of 8"),
+                              (x, w.half(), t, "16-bit"), (x.float(), w.float(), t, "16-bit")]:
+            with pytest.raises(AssertionError, match=what):
+                forward(a, b, c, -100, 1, False)
+        one, each = torch.empty((), device="cuda"), torch.empty(6, device="cuda")
+        state = torch.empty(256 * 6, dtype=torch.uint8, device="cuda")
+        none = torch.empty(0, device="cuda")
+        for grad, reduction, kept, what in [(one.cpu(), 1, state, "gradient"), (each, 1, state, "gradient"), (one, 0, state, "gradient"),
+                                            (one, 1, state[:5], "left for"), (one, 1, state.cpu(), "left for"), (one, 1, state.float(), "left for")]:
+            with pytest.raises(AssertionError, match=what):
+                backward(grad, x, w, kept, reduction, True, True)
+            with pytest.raises(AssertionError, match=what):
+                finish(grad, kept, none, none, x, w, reduction)

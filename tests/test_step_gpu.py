@@ -3,6 +3,8 @@ router of groups in the MoE block, and the head's cross entropy; and the same un
 
 The step through autograd against the step taken apart, every operator called by itself with the gradient that comes back to it: the same bits,
 except behind sparse attention's keys and values, whose gradients are sums in no fixed order."""
+import math
+
 import pytest
 import torch
 import torch.nn as nn
@@ -281,3 +283,24 @@ def test_compiled_loss_of_targets_with_strides(dtype):
     leaf = x.clone().requires_grad_(True)                                # the operator by itself
     got = torch.ops.cinnamon_b200.linear_ce_fwd(leaf, w, table[:90, 1].long(), -100, 0, False)[0]
     assert torch.equal(got, call(leaf, w, table[:90, 1]))
+
+
+def test_compiled_loss_refuses_operands_of_other_devices():
+    from cinnamon_b200 import kernels as K
+    x, w = torch.zeros(5, 64, device="cuda", dtype=torch.bfloat16), torch.zeros(7, 64, device="cuda", dtype=torch.bfloat16)
+    t = torch.zeros(5, device="cuda", dtype=torch.int64)
+    f = torch.compile(lambda x, w, t: K.linear_cross_entropy(x, w, t))
+    for args in ((x, w, t.cpu()), (x, w.cpu(), t), (x.cpu(), w, t)):
+        torch._dynamo.reset()
+        with pytest.raises(Exception, match="Inputs must be on CUDA"):
+            f(*args)
+    for args in ((x, w, t.cpu()), (x, w, t[:4]), (x, w.cpu(), t)):
+        with pytest.raises(AssertionError, match="linear_cross_entropy|Inputs must be on CUDA"):
+            torch.ops.cinnamon_b200.linear_ce_fwd(*args, -100, 1, False)
+    loss, state, sx, sw = torch.ops.cinnamon_b200.linear_ce_fwd(x, w, t, -100, 1, False)
+    assert abs(float(loss) - math.log(7.0)) <= 2.0 ** -20
+    with pytest.raises(AssertionError, match="left for"):
+        torch.ops.cinnamon_b200.linear_ce_bwd(loss, x, w, state[:256], sx, sw, 1, False)
+    with pytest.raises(AssertionError, match="left for"):
+        torch.ops.cinnamon_b200.linear_ce_bwd(loss, x, w, state, sx, sw, 1, True)
+    assert K.device_status() == 0
