@@ -127,45 +127,50 @@ void check_flat(const Tensor& x, const Tensor& w) {
     require(x.scalar_type() == w.scalar_type() && (x.scalar_type() == at::kBFloat16 || x.scalar_type() == at::kHalf),
             "linear_cross_entropy multiplies 16-bit operands");
 }
-void check_part(const Tensor& t, const Tensor& x, at::ScalarType type, int64_t numel) {
-    require(t.device() == x.device() && t.scalar_type() == type && t.numel() == numel && t.is_contiguous(),
+void check_part(const Tensor& t, const at::Device& dev, at::ScalarType type, int64_t numel) {
+    require(t.device() == dev && t.scalar_type() == type && t.numel() == numel && t.is_contiguous(),
             "linear_cross_entropy: not what the forward left for this backward");
 }
-void check_grad(const Tensor& grad, const Tensor& x, int64_t reduction) {
-    require(grad.device() == x.device() && grad.numel() == (reduction ? 1 : x.size(0)), "linear_cross_entropy: the loss's gradient does not fit it");
+void check_grad(const Tensor& grad, const at::Device& dev, int64_t numel) {
+    require(grad.device() == dev && grad.numel() == numel, "linear_cross_entropy: the loss's gradient does not fit it");
 }
 
 }  // namespace
 
 void bind_loss(pybind11::module_& m) {
+    namespace py = pybind11;
     m.def("linear_ce_operands", &ce_operands);
     m.def("linear_ce_early", [](int64_t T, int64_t V, int64_t d, int64_t reduction, int which) { return api.cinn_linear_ce_early(T, V, d, (int)reduction, which); });
-    // (loss, state, sums of dx, sums of dw); the sums are empty in the late way
-    m.def("linear_ce_forward", [](const Tensor& x, const Tensor& w, const Tensor& target, int64_t ignore, int64_t reduction, bool early) {
+    // (loss, state, sums of dx, sums of dw); what is not made is empty: the sums in the late way, and those of a gradient that is not wanted
+    m.def("linear_ce_forward", [](const Tensor& x, const Tensor& w, const Tensor& target, int64_t ignore, int64_t reduction, bool early, bool want_x, bool want_w) {
         check_flat(x, w);
         require(target.device() == x.device(), "linear_cross_entropy: x, weight and target must be on the same device");
         require(target.scalar_type() == at::kLong && target.dim() == 1 && target.size(0) == x.size(0), "linear_cross_entropy: target has one int64 for every row of x");
-        CrossEntropy r = ce_forward(rows_of(x), rows_of(w), target.contiguous(), ignore, reduction, early, early);
-        if (!early) {
-            r.dx_sums = empty({0}, at::kFloat, x.device());
-            r.dw_sums = empty({0}, at::kFloat, x.device());
-        }
-        return std::make_tuple(r.loss, r.state, r.dx_sums, r.dw_sums);
+        CrossEntropy r = ce_forward(rows_of(x), rows_of(w), target.contiguous(), ignore, reduction, early && want_x, early && want_w);
+        auto sums = [&](const Tensor& t) { return t.defined() ? t : empty({0}, at::kFloat, x.device()); };
+        return std::make_tuple(r.loss, r.state, sums(r.dx_sums), sums(r.dw_sums));
+    }, py::arg("x"), py::arg("w"), py::arg("target"), py::arg("ignore"), py::arg("reduction"), py::arg("early"), py::arg("want_x") = true, py::arg("want_w") = true);
+    // (dx, dw) of the early and of the late way; one that is not wanted is empty
+    auto made = [](const std::tuple<Tensor, Tensor>& r, at::ScalarType type, const at::Device& dev) {
+        auto t = [&](const Tensor& g) { return g.defined() ? g : empty({0}, type, dev); };
+        return std::make_tuple(t(std::get<0>(r)), t(std::get<1>(r)));
+    };
+    m.def("linear_ce_finish", [made](const Tensor& grad, const Tensor& state, const Tensor& dx_sums, const Tensor& dw_sums, int64_t T, int64_t V, int64_t d,
+                                 at::ScalarType type, int64_t reduction, bool want_x, bool want_w) {
+        require(state.is_cuda(), "Inputs must be on CUDA");
+        require(T > 0 && V > 0 && d > 0 && d % 8 == 0 && (type == at::kBFloat16 || type == at::kHalf) && (reduction == 1 || reduction == 2),
+                "linear_cross_entropy: early gradients are those of a sum or mean over some tokens");
+        check_grad(grad, state.device(), 1);
+        check_part(state, state.device(), at::kByte, api.cinn_linear_ce_state_bytes(T));
+        if (want_x) check_part(dx_sums, state.device(), at::kFloat, api.cinn_linear_ce_early(T, V, d, (int)reduction, 1) / 4);
+        if (want_w) check_part(dw_sums, state.device(), at::kFloat, api.cinn_linear_ce_early(T, V, d, (int)reduction, 2) / 4);
+        return made(ce_finish(grad, state, want_x ? dx_sums : Tensor(), want_w ? dw_sums : Tensor(), T, V, d, type, reduction), type, state.device());
     });
-    m.def("linear_ce_finish", [](const Tensor& grad, const Tensor& state, const Tensor& dx_sums, const Tensor& dw_sums, const Tensor& x, const Tensor& w,
-                                 int64_t reduction) {
+    m.def("linear_ce_backward", [made](const Tensor& grad, const Tensor& x, const Tensor& w, const Tensor& state, int64_t reduction, bool want_x, bool want_w) {
         check_flat(x, w);
-        check_grad(grad, x, reduction);
-        check_part(state, x, at::kByte, api.cinn_linear_ce_state_bytes(x.size(0)));
-        check_part(dx_sums, x, at::kFloat, api.cinn_linear_ce_early(x.size(0), w.size(0), x.size(1), (int)reduction, 1) / 4);
-        check_part(dw_sums, x, at::kFloat, api.cinn_linear_ce_early(x.size(0), w.size(0), x.size(1), (int)reduction, 2) / 4);
-        return ce_finish(grad, state, dx_sums, dw_sums, x.size(0), w.size(0), x.size(1), x.scalar_type(), reduction);
-    });
-    m.def("linear_ce_backward", [](const Tensor& grad, const Tensor& x, const Tensor& w, const Tensor& state, int64_t reduction, bool want_x, bool want_w) {
-        check_flat(x, w);
-        check_grad(grad, x, reduction);
-        check_part(state, x, at::kByte, api.cinn_linear_ce_state_bytes(x.size(0)));
-        return ce_backward(grad, rows_of(x), rows_of(w), state, reduction, want_x, want_w);
+        check_grad(grad, x.device(), reduction ? 1 : x.size(0));
+        check_part(state, x.device(), at::kByte, api.cinn_linear_ce_state_bytes(x.size(0)));
+        return made(ce_backward(grad, rows_of(x), rows_of(w), state, reduction, want_x, want_w), x.scalar_type(), x.device());
     });
     m.def("linear_cross_entropy", [](const Tensor& x_in, const Tensor& w_in, const Tensor& target_in, int64_t ignore, int64_t reduction) {
         const auto [x, w, target] = ce_operands(x_in, w_in, target_in);

@@ -9,7 +9,7 @@ below wrap forward and backward of the differentiable entry points as opaque nod
   cinnamon_b200::fp8_linear_fwd / fp8_linear_bwd      FP8MatmulFunction   (src/kernels.py:731-794)
   cinnamon_b200::grouped_gemm_fwd / grouped_gemm_bwd  moe_grouped_gemm    (src/kernels.py:526-581; differentiable here)
   cinnamon_b200::sparse_attn_fwd / sparse_attn_bwd    SparseAttentionFunction (src/kernels.py:1189-1289)
-  cinnamon_b200::linear_ce_fwd / linear_ce_bwd        linear_cross_entropy
+  cinnamon_b200::linear_ce_fwd / linear_ce_bwd / linear_ce_finish   linear_cross_entropy
   cinnamon_b200::rotate                               rotary (its derivative is itself, the other way round)
 
 Each operator body runs the very code of the eager ``autograd.Function`` (its ``forward`` / ``backward`` static
@@ -260,43 +260,61 @@ def _up(n, a: int):
 
 
 @torch.library.custom_op("cinnamon_b200::linear_ce_fwd", mutates_args=(), device_types="cuda")
-def linear_ce_fwd(x: Tensor, weight: Tensor, target: Tensor, ignore_index: int, reduction: int, early: bool) -> Tuple[Tensor, Tensor, Tensor, Tensor]:
-    return K._host.linear_ce_forward(x, weight, target, ignore_index, reduction, early)
+def linear_ce_fwd(x: Tensor, weight: Tensor, target: Tensor, ignore_index: int, reduction: int, early: bool, want_x: bool = True,
+                  want_w: bool = True) -> Tuple[Tensor, Tensor, Tensor, Tensor]:
+    """``early``: the sums of the gradients that are wanted are made along the way."""
+    return K._host.linear_ce_forward(x, weight, target, ignore_index, reduction, early, want_x, want_w)
 
 
 @linear_ce_fwd.register_fake
-def _(x, weight, target, ignore_index, reduction, early):
+def _(x, weight, target, ignore_index, reduction, early, want_x=True, want_w=True):
     T, d = x.shape
     state = 256 + 3 * _up(4 * T, 256) + _up(8 * T, 256) if T else 0                # cinn_linear_ce_state_bytes
-    sums = [K._host.linear_ce_early(int(T), weight.shape[0], int(d), reduction, i) // 4 if early else 0 for i in (1, 2)]
+    sums = [K._host.linear_ce_early(int(T), weight.shape[0], int(d), reduction, i) // 4 if early and want else 0 for i, want in ((1, want_x), (2, want_w))]
     e = lambda shape, dt: torch.empty(shape, dtype=dt, device=x.device)                         # noqa: E731
     return e(() if reduction else (T,), torch.float32), e((state,), torch.uint8), e((sums[0],), torch.float32), e((sums[1],), torch.float32)
 
 
 @torch.library.custom_op("cinnamon_b200::linear_ce_bwd", mutates_args=(), device_types="cuda")
-def linear_ce_bwd(grad: Tensor, x: Tensor, weight: Tensor, state: Tensor, dx_sums: Tensor, dw_sums: Tensor, reduction: int,
-                  early: bool) -> Tuple[Tensor, Tensor]:
-    if early:
-        return K._host.linear_ce_finish(grad, state, dx_sums, dw_sums, x, weight, reduction)
-    return K._host.linear_ce_backward(grad, x, weight, state, reduction, True, True)
+def linear_ce_bwd(grad: Tensor, x: Tensor, weight: Tensor, state: Tensor, reduction: int, want_x: bool, want_w: bool) -> Tuple[Tensor, Tensor]:
+    return K._host.linear_ce_backward(grad, x, weight, state, reduction, want_x, want_w)
 
 
 @linear_ce_bwd.register_fake
-def _(grad, x, weight, state, dx_sums, dw_sums, reduction, early):
-    return (torch.empty(x.shape, dtype=x.dtype, device=x.device), torch.empty(weight.shape, dtype=weight.dtype, device=x.device))
+def _(grad, x, weight, state, reduction, want_x, want_w):
+    return (torch.empty(x.shape if want_x else (0,), dtype=x.dtype, device=x.device),
+            torch.empty(weight.shape if want_w else (0,), dtype=weight.dtype, device=x.device))
+
+
+@torch.library.custom_op("cinnamon_b200::linear_ce_finish", mutates_args=(), device_types="cuda")
+def linear_ce_finish(grad: Tensor, state: Tensor, dx_sums: Tensor, dw_sums: Tensor, tokens: int, words: int, d: int, dtype: torch.dtype, reduction: int,
+                     want_x: bool, want_w: bool) -> Tuple[Tensor, Tensor]:
+    """The backward of the early way, which reads neither operand (they need not be kept for it)."""
+    return K._host.linear_ce_finish(grad, state, dx_sums, dw_sums, tokens, words, d, dtype, reduction, want_x, want_w)
+
+
+@linear_ce_finish.register_fake
+def _(grad, state, dx_sums, dw_sums, tokens, words, d, dtype, reduction, want_x, want_w):
+    return (torch.empty((tokens, d) if want_x else (0,), dtype=dtype, device=state.device),
+            torch.empty((words, d) if want_w else (0,), dtype=dtype, device=state.device))
 
 
 def _ce_setup(ctx, inputs, output):
-    x, weight, _, _, ctx.reduction, ctx.early = inputs
-    ctx.save_for_backward(x, weight, *output[1:])
+    x, weight, _, _, ctx.reduction, ctx.early, _, _ = inputs
+    ctx.of = (x.shape[0], *weight.shape, x.dtype)
+    ctx.save_for_backward(*(output[1:] if ctx.early else (x, weight, output[1])))
     ctx.set_materialize_grads(False)
 
 
 def _ce_backward(ctx, grad, *ignored):
     if grad is None:
-        return None, None, None, None, None, None
-    gx, gw = torch.ops.cinnamon_b200.linear_ce_bwd(grad, *ctx.saved_tensors, ctx.reduction, ctx.early)
-    return gx, gw, None, None, None, None
+        return (None,) * 8
+    want_x, want_w = ctx.needs_input_grad[:2]
+    if ctx.early:
+        gx, gw = torch.ops.cinnamon_b200.linear_ce_finish(grad, *ctx.saved_tensors, *ctx.of, ctx.reduction, want_x, want_w)
+    else:
+        gx, gw = torch.ops.cinnamon_b200.linear_ce_bwd(grad, *ctx.saved_tensors, ctx.reduction, want_x, want_w)
+    return (gx if want_x else None, gw if want_w else None) + (None,) * 6
 
 
 linear_ce_fwd.register_autograd(_ce_backward, setup_context=_ce_setup)
@@ -325,9 +343,9 @@ def linear_cross_entropy(x: Tensor, weight: Tensor, target: Tensor, ignore_index
         "linear_cross_entropy multiplies 16-bit operands: x and weight must both be bfloat16 or both float16 (or autocast must make them so)"
     # the gradients' sums have sizes that only known ones give: a call that is traced for any number of tokens makes them in its backward
     known = has_static_value(flat.shape[0]) and has_static_value(weight.shape[0]) and has_static_value(flat.shape[1])
-    early = (known and flat.requires_grad and weight.requires_grad and torch.is_grad_enabled()
-             and _ce_early(flat.shape[0], weight.shape[0], flat.shape[1], reduction))
-    loss = torch.ops.cinnamon_b200.linear_ce_fwd(flat, weight, target.reshape(-1).long(), ignore_index, reduction, early)[0]
+    want_x, want_w = (torch.is_grad_enabled() and t.requires_grad for t in (flat, weight))
+    early = known and (want_x or want_w) and _ce_early(flat.shape[0], weight.shape[0], flat.shape[1], reduction)
+    loss = torch.ops.cinnamon_b200.linear_ce_fwd(flat, weight, target.reshape(-1).long(), ignore_index, reduction, early, want_x, want_w)[0]
     return loss if reduction else loss.view(target.shape)
 
 

@@ -29,5 +29,12 @@ def test_operators_of_a_compiled_graph_refuse_what_the_kernels_cannot_read():
                                             (one, 1, state[:5], "left for"), (one, 1, state.cpu(), "left for"), (one, 1, state.float(), "left for")]:
             with pytest.raises(AssertionError, match=what):
                 backward(grad, x, w, kept, reduction, True, True)
+        for grad, reduction, kept, what in [(one.cpu(), 1, state, "gradient"), (each, 1, state, "gradient"), (one, 0, state, "sum or mean"),
+                                            (one, 1, state[:5], "left for"), (one, 1, state.cpu(), "CUDA"), (one, 1, state.float(), "left for")]:
             with pytest.raises(AssertionError, match=what):
-                finish(grad, kept, none, none, x, w, reduction)
+                finish(grad, kept, none, none, 6, 20, 64, torch.bfloat16, reduction, True, True)
+        for shape in ((0, 20, 64), (6, 0, 64), (6, 20, 63)):
+            with pytest.raises(AssertionError, match="sum or mean"):
+                finish(one, state, none, none, *shape, torch.bfloat16, 1, True, True)
+        with pytest.raises(AssertionError, match="sum or mean"):
+            finish(one, state, none, none, 6, 20, 64, torch.float32, 1, True, True)

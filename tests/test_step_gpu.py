@@ -300,7 +300,38 @@ def test_compiled_loss_refuses_operands_of_other_devices():
     loss, state, sx, sw = torch.ops.cinnamon_b200.linear_ce_fwd(x, w, t, -100, 1, False)
     assert abs(float(loss) - math.log(7.0)) <= 2.0 ** -20
     with pytest.raises(AssertionError, match="left for"):
-        torch.ops.cinnamon_b200.linear_ce_bwd(loss, x, w, state[:256], sx, sw, 1, False)
+        torch.ops.cinnamon_b200.linear_ce_bwd(loss, x, w, state[:256], 1, True, True)
     with pytest.raises(AssertionError, match="left for"):
-        torch.ops.cinnamon_b200.linear_ce_bwd(loss, x, w, state, sx, sw, 1, True)
+        torch.ops.cinnamon_b200.linear_ce_finish(loss, state, sx, sw, 5, 7, 64, x.dtype, 1, True, True)
     assert K.device_status() == 0
+
+
+@pytest.mark.parametrize("reduction", ["mean", "none"])
+@pytest.mark.parametrize("frozen", ["x", "weight", "neither"])
+@pytest.mark.parametrize("T,d", [(150, 100), (2100, 1030)])             # (the second: a mean's gradients are made in the forward)
+def test_compiled_loss_with_one_side_frozen(T, d, frozen, reduction):
+    """The eager call's bits, and neither time nor memory for the gradient that nobody asked for."""
+    from cinnamon_b200 import kernels as K
+    g = torch.Generator().manual_seed(7)
+    V = 40000
+    x, w = torch.randn(T, d, generator=g).cuda(), (torch.randn(V, d, generator=g) * 0.1).cuda()
+    target = torch.randint(0, V, (T,), generator=g).cuda()
+    target[::9] = -100
+    call = lambda x, w: K.linear_cross_entropy(x, w, target, reduction=reduction)      # noqa: E731
+    up = torch.randn((T,) if reduction == "none" else (), generator=g).cuda()
+    results, most = [], []
+    for compiled in (False, True):
+        torch._dynamo.reset()
+        f = torch.compile(call, fullgraph=True) if compiled else call
+        a, b = x.bfloat16().requires_grad_(frozen != "x"), w.bfloat16().requires_grad_(frozen != "weight")
+        leaves = [t for t in (a, b) if t.requires_grad]
+        torch.autograd.grad(f(a, b), leaves, up)
+        torch.cuda.synchronize()
+        torch.cuda.reset_peak_memory_stats()
+        before = torch.cuda.memory_allocated()
+        loss = f(a, b)
+        results.append([loss.detach(), *torch.autograd.grad(loss, leaves, up)])
+        most.append(torch.cuda.max_memory_allocated() - before)
+    for got, want in zip(results[1], results[0]):
+        assert got.shape == want.shape and torch.equal(got, want)
+    assert most[1] <= most[0] + (4 << 20)                                # (a gradient of this weight: 8 and 82 MB)
