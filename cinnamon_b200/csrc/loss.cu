@@ -73,7 +73,7 @@ struct Params {
     const int* rows;                       // the token of every row in use
     const float2* stat;                    // per row: maximum, log2 of the sum
     const float* grad;                     // the loss's gradient: one number, or one per token
-    const unsigned* grad_max;              // the bits of the largest |gradient| (reduction "none")
+    const unsigned* grad_max;              // the bits of the largest finite |gradient| (reduction "none")
     int mean;
     float log2e;                           // of one unit of the logits as they stand in tensor memory (see growth)
     uint16_t* dz;                          // the piece's (KEEP: what it will be made of), rows of dz_ld (a multiple of 64)
@@ -446,7 +446,11 @@ product_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__
                 if constexpr (MODE == SOFT) {
                     const float2 st = p.stat[own];
                     mx = st.x; sum = st.y;
-                    rel = p.per_row ? (most == 0.0f ? 0.0f : p.grad[p.rows[own]] / most) : 1.0f;
+                    rel = 1.0f;
+                    if (p.per_row) {
+                        const float g = p.grad[p.rows[own]];
+                        rel = most > 0.0f ? g / most : g;              // (0: they are zeros, infinities and NaN)
+                    }
                     if (!BF16) rel *= FP16_SCALE;
                 }
             }
@@ -1024,14 +1028,15 @@ soften_kernel(const Params p) {
     }
 }
 
-// the largest |gradient| among the tokens in use, as bits (a NaN is larger than any number); *out starts at 0
+// the largest finite |gradient| among the tokens in use, as bits; *out starts at 0.  (An infinity or NaN is its own token's affair: related to one, every
+// other token's gradient would be 0 times infinity.)
 __global__ void __launch_bounds__(256)
 grad_max_kernel(const float* __restrict__ grad, const int* __restrict__ slot, int T, unsigned* __restrict__ out) {
     pdl_wait();
     pdl_trigger();
     unsigned most = 0;
     for (int t = blockIdx.x * 256 + threadIdx.x; t < T; t += gridDim.x * 256)
-        if (slot[t] >= 0) most = max(most, __float_as_uint(fabsf(grad[t])));
+        if (slot[t] >= 0 && fabsf(grad[t]) < INFINITY) most = max(most, __float_as_uint(fabsf(grad[t])));
     most = __reduce_max_sync(0xffffffffu, most);
     if ((threadIdx.x & 31) == 0 && most) atomicMax(out, most);
 }

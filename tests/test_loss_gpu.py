@@ -428,3 +428,26 @@ def test_a_few_tokens_lose_nothing_to_dz(T, V, d, ignored, reduction, dtype):
     _, _, dx, dx_tol, dw, dw_tol = _oracle(x, w, target, per, few=True)
     _within(gx, dx, dx_tol, "dx")
     _within(gw, dw, dw_tol, "dw")
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("T,ignored", [(40, 0.0), (300, 0.3), (2300, 0.1)])
+def test_infinite_gradients_are_their_own_tokens(T, ignored, dtype):
+    """One token's infinite or NaN gradient leaves the others' rows as they are."""
+    x, w, target = _inputs(T, 500, 136, dtype, seed=T, ignored=ignored)
+    bad = torch.tensor([5, 9, 17], device="cuda")
+    target[bad] = 3
+    others = torch.ones(T, dtype=torch.bool, device="cuda")
+    others[bad] = False
+    grad = torch.randn(T, generator=torch.Generator().manual_seed(1)).cuda()
+    for rest in (grad, torch.zeros_like(grad)):
+        clean, dirty = rest.clone(), rest.clone()
+        clean[bad] = 0.0
+        dirty[5], dirty[9], dirty[17] = float("inf"), float("nan"), float("-inf")
+        want, got = _run(x, w, target, clean, reduction="none"), _run(x, w, target, dirty, reduction="none")
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1][others], want[1][others])
+        assert not torch.isfinite(got[1][bad]).any() and not torch.isfinite(got[2]).any()
+        if ignored:                                                    # (an ignored token's gradient is nobody's)
+            dirty = clean.clone()
+            dirty[target == -100] = float("inf")
+            assert all(torch.equal(a, b) for a, b in zip(_run(x, w, target, dirty, reduction="none"), want))
