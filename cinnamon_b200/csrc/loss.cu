@@ -10,7 +10,7 @@
 //   late    The words in pieces; a piece's product is made again, turned into dz in the epilogue and rounded to the operands' type
 //           (bf16, or fp16 times 2^14, so that small probabilities keep their bits), and two products over the piece add up dx
 //           (fp32, in L2) and write the piece's rows of dW.  2 T V d forward and 6 T V d backward, one 2 T V d more than with kept logits.
-//   early   The tokens in pieces; a piece's e^(z - maximum of its 128 words) is written in fp16 by the forward's product, turned into dz by one
+//   early   The tokens in pieces; a piece's e^(z - maximum of its 128 words) is written in fp16, times 2^15, by the forward's product, turned into dz by one
 //           pass over it once the sums are known, and the two products add up dx and dW in fp32, all in the forward.  What is left for the
 //           backward is the loss's gradient, one number, and the one rounding.  6 T V d in all.  The sums stay until the backward, and a
 //           loss whose gradient is never asked for has cost three times as much.  For sums and means over many and wide rows (early_pays).
@@ -51,6 +51,10 @@ constexpr int C_BYTES = EPI * BOXES * BOX;
 constexpr size_t SMEM_Z = (size_t)STAGES_Z * 2 * SIDE + 256 + 1024, SMEM_G = (size_t)STAGES_G * 2 * SIDE + C_BYTES + 256 + 1024;
 constexpr int GROUP = 16;                  // tiles of tokens that meet a run of words before the next ones do (L2)
 constexpr int SCAN = 1024;                 // tokens per CTA of the passes that gather
+// Of the exponentials that the early way keeps in fp16: the largest of 128 words is 1, and so becomes 2^15.  Words down to 2^-29 of it (20 nats) keep all
+// their bits and those down to 2^-40 (27 nats) some; unscaled, fp16's smallest numbers began at 2^-14 (10 nats) and a rare word's row of dW was
+// zero from 17 nats on.
+constexpr float KEPT_SCALE = 32768.0f;
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float FP16_SCALE = 16384.0f;     // of dz in fp16: the smallest probability with all its bits is then 2^-28
 
@@ -359,7 +363,7 @@ __device__ __forceinline__ uint64_t pair2(float a, float b) {
 }
 
 // The logits' product: A = x, B = W, both K-major.  STATS leaves maxima and sums of its runs, SOFT dz of the piece, KEEP both maxima and sums, and
-// e^(z - maximum) in fp16, of each half tile.  xg: x's rows in use, gathered; read in x's place where some token is ignored.  Bound by the tensor cores
+// e^(z - maximum) in fp16 (times KEPT_SCALE), of each half tile.  xg: x's rows in use, gathered; read in x's place where some token is ignored.  Bound by the tensor cores
 // (active 87.6 % of STATS at 8192 x 32000 x 512, 74 % of SOFT, which also writes dz) and, in long calls, by the power that they draw.
 template <int MODE, bool BF16>
 __global__ void __launch_bounds__(THREADS, 1)
@@ -518,7 +522,7 @@ product_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__
                         }
                     }
                     const float base = top == -INFINITY ? 0.0f : top;
-                    const uint64_t minus = pair2(-base, -base), scale = pair2(p.log2e, p.log2e);
+                    const uint64_t minus = pair2(-base, -base), scale = pair2(p.log2e, p.log2e), kept = pair2(KEPT_SCALE, KEPT_SCALE);
                     float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
                     for (int c = 0; c < COLS / 32; ++c) {
@@ -549,6 +553,12 @@ product_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__
                         const int col = nt * N + h * COLS + c * 32;
                         if (col < p.dz_ld) {
                             uint32_t v[16];
+#pragma unroll
+                            for (int j = 0; j < 32; j += 2)
+                                asm("{\n\t.reg .b64 a;\n\t"
+                                    "mov.b64 a, {%0, %1};\n\t"
+                                    "mul.rn.f32x2 a, a, %2;\n\t"
+                                    "mov.b64 {%0, %1}, a;\n\t}" : "+r"(z[j]), "+r"(z[j + 1]) : "l"(kept));
 #pragma unroll
                             for (int j = 0; j < 16; ++j) v[j] = pack2<false>(__uint_as_float(z[2 * j]), __uint_as_float(z[2 * j + 1]));
                             store32(p.dz + (int64_t)row * p.dz_ld + col, v);
@@ -1012,7 +1022,7 @@ soften_kernel(const Params p) {
         const int row = (int)(i / per), at = (int)(i - (int64_t)row * per) * 32 + lane;
         if (at >= vecs) continue;
         const float2 st = p.stat[p.t0 + row];
-        const float f = exp2_approx((p.tile_max[(int64_t)(at / 16) * p.part_ld + row] - st.x) * p.log2e - st.y);
+        const float f = exp2_approx((p.tile_max[(int64_t)(at / 16) * p.part_ld + row] - st.x) * p.log2e - st.y) * (1.0f / KEPT_SCALE);
         uint4* q = reinterpret_cast<uint4*>(p.dz + (int64_t)row * p.dz_ld) + at;
         uint4 v = *q;
         uint32_t* h = &v.x;

@@ -451,3 +451,35 @@ def test_infinite_gradients_are_their_own_tokens(T, ignored, dtype):
             dirty = clean.clone()
             dirty[target == -100] = float("inf")
             assert all(torch.equal(a, b) for a, b in zip(_run(x, w, target, dirty, reduction="none"), want))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("T,V,d", [(2304, 512, 1024), (2050, 500, 1040)])
+def test_rare_words_beside_a_likely_one(T, V, d, dtype):
+    """Gradients made in the forward: rows of dW of words that are 8 to 24 nats less likely than the best of their 128 neighbours, each against its
+    own size.  The exponentials are held in fp16 relative to that best one, times 2^15: an error of 2^-11 of each, and at least 2^-40 of the best one
+    (half of fp16's smallest step, 2^-25)."""
+    from cinnamon_b200 import kernels as K
+    assert K._host.linear_ce_early(T, V, d, 2, 0) == 1
+    g = torch.Generator().manual_seed(V)
+    u = HALF_STEP[dtype]
+    along = torch.full((d,), d ** -0.5)
+    x = (8 * along + 0.3 * torch.randn(T, d, generator=g)).to(dtype).cuda()
+    less = 8 + 16 * torch.rand(V, generator=g)
+    less[::128] = torch.arange((V + 127) // 128).float()                # the likely ones, one in 128
+    w = (-less[:, None] / 8 * along + 0.02 * torch.randn(V, d, generator=g)).to(dtype).cuda()
+    target = (torch.randint(0, (V + 127) // 128, (T,), generator=g) * 128).cuda()
+    target[7::50] = -100
+    grad = torch.ones(T, device="cuda")
+    _, _, dx, dx_tol, dw, dw_tol = _oracle(x, w, target, grad)
+    use = target >= 0
+    p = torch.softmax(x[use].double() @ w.double().t(), -1)
+    best = torch.nn.functional.pad(p, (0, -V % 128)).unflatten(1, (-1, 128)).amax(-1).repeat_interleave(128, 1)[:, :V]
+    e = (1 + u) * (2.0 ** -11 * p + 2.0 ** -40 * best)
+    dw_tol = dw_tol + e.t() @ x[use].double().abs() * (1 + u)
+    dx_tol[use] += e @ w.double().abs() * (1 + u)
+    _, gx, gw = _run(x, w, target, reduction="sum")
+    _within(gx, dx, dx_tol, "grad_x")
+    _within(gw, dw, dw_tol, "grad_w")
+    rare = (less > 17) & (less < 20)
+    assert rare.sum() > 20 and (dw_tol[rare].norm(dim=1) <= 0.1 * dw[rare].norm(dim=1)).all()
