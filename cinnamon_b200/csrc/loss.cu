@@ -1250,6 +1250,13 @@ static int check_shapes(const void* x, int64_t ldx, const void* w, int64_t ldw, 
     return CINN_OK;
 }
 
+// store32 writes pieces of 32 bytes into the workspace (whose parts lie 256 bytes apart); the state's widest elements are of 8
+static int check_scratch(const void* state, const void* workspace) {
+    CINN_CHECK_ARG((reinterpret_cast<uintptr_t>(workspace) & 31) == 0 && (reinterpret_cast<uintptr_t>(state) & 7) == 0,
+                   "linear_ce: the workspace must be 32-byte aligned and the state 8-byte aligned");
+    return CINN_OK;
+}
+
 static int gather(const void* x, int64_t ldx, const Plan& r, const State& s, void* xg, int64_t half, cudaStream_t st) {
     launch_dependent(gather_kernel, dim3(grid_for((half + r.T) * (r.d / 8), 256)), dim3(256), 0, st, static_cast<const uint4*>(x), ldx / 8,
                      (int)r.T, (int)(r.d / 8), s.n_valid, s.rows, static_cast<uint4*>(xg), (int)half);
@@ -1410,6 +1417,7 @@ int linear_ce_forward(const void* x, int64_t ldx, const void* w, int64_t ldw, in
         return CINN_OK;
     }
     CINN_CHECK_ARG(target && state && workspace, "linear_ce: null pointer");
+    if ((rc = ce::check_scratch(state, workspace))) return rc;
     const ce::Plan r = ce::make_plan(T, V, d, early);
     int64_t need = 0;
     const ce::Forward f = ce::carve_forward(workspace, r, &need);
@@ -1424,6 +1432,8 @@ int linear_ce_finish(int dtype, const float* grad, int64_t T, int64_t V, int64_t
                      const float* dw_sums, void* dx, void* dw, cudaStream_t st) {
     CINN_CHECK_ARG((dtype == CINN_BF16 || dtype == CINN_F16) && T > 0 && V > 0 && d > 0 && d % 8 == 0 && (reduction == 1 || reduction == 2), "linear_ce finish: bad arguments");
     CINN_CHECK_ARG(grad && state && (!dx || dx_sums) && (!dw || dw_sums), "linear_ce finish: null pointer");
+    int rc = ce::check_scratch(state, nullptr);
+    if (rc) return rc;
     CINN_CHECK_ARG(((reinterpret_cast<uintptr_t>(dx) | reinterpret_cast<uintptr_t>(dw) | reinterpret_cast<uintptr_t>(dx_sums) |
                      reinterpret_cast<uintptr_t>(dw_sums)) & 15) == 0, "linear_ce finish: pointers must be 16-byte aligned");
     const ce::Plan r = ce::make_plan(T, V, d, true);
@@ -1431,7 +1441,6 @@ int linear_ce_finish(int dtype, const float* grad, int64_t T, int64_t V, int64_t
     ce::Params p{};
     p.n_valid = s.n_valid; p.grad = grad; p.mean = reduction == 1;
     const bool bf16 = dtype == CINN_BF16;
-    int rc = CINN_OK;
     if (dx) rc = bf16 ? ce::finish<true>(dx_sums, r.dx_splits, r.Tp, T, d, s.slot, p, dx, st) : ce::finish<false>(dx_sums, r.dx_splits, r.Tp, T, d, s.slot, p, dx, st);
     if (rc || !dw) return rc;
     return bf16 ? ce::finish<true>(dw_sums, r.dw_splits, ce::up(V, ce::M), V, d, nullptr, p, dw, st)
@@ -1448,6 +1457,7 @@ int linear_ce_backward(const void* x, int64_t ldx, const void* w, int64_t ldw, i
         return CINN_OK;
     }
     CINN_CHECK_ARG(grad && state && workspace, "linear_ce: null pointer");
+    if ((rc = ce::check_scratch(state, workspace))) return rc;
     CINN_CHECK_ARG(((reinterpret_cast<uintptr_t>(dx) | reinterpret_cast<uintptr_t>(dw)) & 15) == 0, "linear_ce: gradients must be 16-byte aligned");
     const ce::Plan r = ce::make_plan(T, V, d, false);
     int64_t need = 0;

@@ -568,8 +568,8 @@ int cinn_moe_route_static(const float* logits, const float* bias, int64_t n_toke
  * its row of x holds; one whose target is no word (outside [0, V)) has the loss NaN and no part in the gradients.
  * reduction 0: loss (T,), one per token; 1: the mean over the tokens with a target (NaN where there is none), 2: the sum.
  * grad: (T,) or one number, fp32.  dx (T, d) and dw (V, d), contiguous, of the operands' type; either may be NULL.
- * state: cinn_linear_ce_state_bytes(T), written by the forward for the backward.  workspace: scratch of
- * cinn_linear_ce_workspace_bytes(T, V, d, pass) bytes.  Two ways to the gradients:
+ * state: cinn_linear_ce_state_bytes(T), 8-byte aligned, written by the forward for the backward.  workspace: scratch of
+ * cinn_linear_ce_workspace_bytes(T, V, d, pass) bytes, 32-byte aligned; sums and gradients 16-byte aligned.  Two ways to the gradients:
  *   late   the forward with dx_sums and dw_sums NULL (pass 0); cinn_linear_ce_backward multiplies the logits once more, a piece of
  *          the words at a time (pass 4, + 1 with dx, + 2 with dw);
  *   early  reduction 1 or 2: the forward leaves the fp32 sums of one or both gradients (pass 1); cinn_linear_ce_finish multiplies

@@ -195,3 +195,22 @@ int main() {
     return 0;
 }
 """) == 0
+
+
+def test_the_cross_entropy_refuses_pointers_that_its_stores_cannot_write(built):
+    """On the host, before anything is launched: the workspace is written 32 bytes at a time."""
+    from cinnamon_b200 import _lib
+    L, p = _lib.lib, ctypes.c_void_p
+    T, V, d = 4, 16, 8
+
+    def forward(workspace, state):
+        return L.cinn_linear_ce_forward(p(4096), d, p(4096), d, 0, p(4096), -100, T, V, d, 1, p(4096), p(state), None, None, p(workspace), 1 << 40, None)
+
+    def backward(workspace, state):
+        return L.cinn_linear_ce_backward(p(4096), d, p(4096), d, 0, p(4096), T, V, d, 1, p(state), p(4096), p(4096), p(workspace), 1 << 40, None)
+
+    for call in (forward, backward):
+        for workspace, state in ((4096 + 16, 4096), (4096 + 8, 4096), (4096 + 31, 4096), (4096, 4100)):
+            assert call(workspace, state) == _lib.ERR_INVALID and "aligned" in _lib.last_error()
+    assert L.cinn_linear_ce_finish(0, p(4096), T, V, d, 1, p(4100), p(4096), p(4096), p(4096), p(4096), None) == _lib.ERR_INVALID
+    assert "aligned" in _lib.last_error()
