@@ -174,6 +174,7 @@ void bind_loss(pybind11::module_& m) {
     });
     m.def("linear_cross_entropy", [](const Tensor& x_in, const Tensor& w_in, const Tensor& target_in, int64_t ignore, int64_t reduction) {
         const auto [x, w, target] = ce_operands(x_in, w_in, target_in);
+        c10::cuda::CUDAGuard guard(x.device());               // (check_capture asks the current device's stream)
         check_capture("linear_cross_entropy", x_in, w_in);
         const Tensor loss = takes_node(x, w) ? CrossEntropyNode::apply(x, w, target, ignore, reduction)
                                              : ce_forward(rows_of(x), rows_of(w), target, ignore, reduction, false, false).loss;

@@ -58,3 +58,15 @@ def test_kernels_trigger_once_they_hold_their_tensor_memory():
         inside = body[by[1].end():body.index("pdl_trigger()")]
         assert inside.strip() == "" or (inside.strip().startswith("{") and "}" not in inside), (file, name, inside)
     assert seen >= 9
+
+
+def test_native_calls_set_their_device_before_they_ask_for_its_stream():
+    """``check_capture`` judges by the current device's stream, which is another's until the guard stands."""
+    seen = 0
+    for path in sorted(glob.glob(os.path.join(CSRC, "host", "*.cpp"))):
+        text = re.sub(r"//[^\n]*", "", open(path).read())
+        for m in re.finditer(r"check_capture\(", text):
+            seen += 1
+            call = text[text.rindex("m.def(", 0, m.start()):m.start()]
+            assert "CUDAGuard guard(" in call, os.path.basename(path)
+    assert seen >= 3
