@@ -8,12 +8,15 @@
 #pragma once
 #include <torch/extension.h>
 #include <torch/csrc/Exceptions.h>
+#include <torch/csrc/autograd/graph_task.h>
 #include <ATen/autocast_mode.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <exception>
 #include <string>
+#include <unordered_set>
+#include <vector>
 #include "../../../include/cinnamon_b200.h"
 
 namespace cinnhost {
@@ -126,11 +129,38 @@ inline bool differentiates_on_null_stream(const Tensor& t) {
     const auto s = node->stream();
     return s.has_value() && c10::cuda::CUDAStream(*s).stream() == nullptr;
 }
+[[noreturn]] inline void refuse_capture(const char* who) {
+    throw CinnError(std::string(who) + ": a step that is captured with its gradients must not share its inputs with a graph recorded on the "
+                    "default stream that still lives (drop that loss, or record it on a stream of its own)", true);
+}
 template <typename... T>
 void check_capture(const char* who, const T&... t) {
-    if (at::GradMode::is_enabled() && capturing() && (differentiates_on_null_stream(t) || ...))
-        throw CinnError(std::string(who) + ": a step that is captured with its gradients must not share its inputs with a graph recorded on the "
-                        "default stream that still lives (drop that loss, or record it on a stream of its own)", true);
+    if (at::GradMode::is_enabled() && capturing() && (differentiates_on_null_stream(t) || ...)) refuse_capture(who);
+}
+// The same from within a captured backward pass, which is about to go on to the nodes behind the one that runs: a leaf behind a view or a cast has no
+// node of its own that check_capture could have asked.
+inline void check_captured_backward(const char* who) {
+    if (!capturing()) return;
+    const auto here = torch::autograd::get_current_node();
+    if (!here) return;
+    const auto* wanted = torch::autograd::get_current_graph_task_exec_info();       // (empty: all of them)
+    std::vector<torch::autograd::Node*> todo{here.get()};
+    std::unordered_set<torch::autograd::Node*> seen;
+    while (!todo.empty()) {
+        auto* node = todo.back();
+        todo.pop_back();
+        for (const auto& edge : node->next_edges()) {
+            auto* next = edge.function.get();
+            if (!next || !seen.insert(next).second) continue;
+            if (wanted && !wanted->empty()) {
+                const auto it = wanted->find(next);
+                if (it == wanted->end() || !it->second.should_execute()) continue;
+            }
+            const auto s = next->stream();
+            if (s.has_value() && s->device_type() == c10::DeviceType::CUDA && c10::cuda::CUDAStream(*s).stream() == nullptr) refuse_capture(who);
+            todo.push_back(next);
+        }
+    }
 }
 inline float* f32(const Tensor& t);
 Tensor gemm(const Tensor& a, const Tensor& sa, const Tensor& b, int layout, const Tensor& sb, int64_t sbk, int64_t sbn, int64_t M,

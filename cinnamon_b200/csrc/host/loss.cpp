@@ -80,6 +80,7 @@ struct CrossEntropyNode : public torch::autograd::Function<CrossEntropyNode> {
         Tensor dx, dw;
         as_python_error([&] {
             require(!at::GradMode::is_enabled(), "linear_cross_entropy has no second derivative (create_graph=True)");
+            check_captured_backward("linear_cross_entropy");
             const int64_t reduction = ctx->saved_data["reduction"].toInt();
             const bool want_x = ctx->needs_input_grad(0), want_w = ctx->needs_input_grad(1);
             if (ctx->saved_data["early"].toBool()) {

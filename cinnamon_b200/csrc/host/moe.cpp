@@ -171,6 +171,7 @@ struct RouteNode : public torch::autograd::Function<RouteNode> {
             require(!at::GradMode::is_enabled(), "moe_route has no second derivative (create_graph=True)");
             const Tensor& logits = s[0];
             c10::cuda::CUDAGuard guard(logits.device());
+            check_captured_backward("moe_route");
             const int64_t T = logits.size(0), E = logits.size(1);
             Tensor g[3];
             for (int i = 0; i < 3; ++i)

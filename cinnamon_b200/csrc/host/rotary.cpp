@@ -76,6 +76,7 @@ struct RotaryNode : public torch::autograd::Function<RotaryNode> {
         as_python_error([&] {
             require(!at::GradMode::is_enabled(), "rotary has no second derivative (create_graph=True)");
             c10::cuda::CUDAGuard guard(s[0].device());
+            check_captured_backward("rotary");
             const Form f{ctx->saved_data["start"].toInt(), ctx->saved_data["magnitude"].toDouble(), ctx->saved_data["interleaved"].toBool()};
             r = turned(ctx->needs_input_grad(0) ? grads[0] : Tensor(), grads.size() > 1 && ctx->needs_input_grad(1) ? grads[1] : Tensor(), s[0], s[1], f, true);
         });

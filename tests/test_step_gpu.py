@@ -3,6 +3,7 @@ router of groups in the MoE block, and the head's cross entropy; and the same un
 
 The step through autograd against the step taken apart, every operator called by itself with the gradient that comes back to it: the same bits,
 except behind sparse attention's keys and values, whose gradients are sums in no fixed order."""
+import gc
 import math
 
 import pytest
@@ -335,3 +336,58 @@ def test_compiled_loss_with_one_side_frozen(T, d, frozen, reduction):
     for got, want in zip(results[1], results[0]):
         assert got.shape == want.shape and torch.equal(got, want)
     assert most[1] <= most[0] + (4 << 20)                                # (a gradient of this weight: 8 and 82 MB)
+
+
+@pytest.mark.parametrize("op", ["loss", "rotary", "route", "route_reference"])
+@pytest.mark.parametrize("everything", [False, True])
+def test_capture_beside_a_living_graph_of_a_leaf_behind_views(op, everything):
+    """A leaf behind a transpose, a slice or a product has its node on the default stream as well: the captured backward is refused before it gets there.
+    A captured forward alone, and a backward that ends in front of the leaf, go through."""
+    from cinnamon_b200 import kernels as K
+    g = torch.Generator().manual_seed(4)
+    x, w = (torch.randn(40, 96, generator=g).cuda().bfloat16().requires_grad_(True) for _ in range(2))
+    q = torch.randn(1, 40, 2, 64, generator=g).cuda().requires_grad_(True)
+    target, positions, bias = torch.arange(40, device="cuda"), torch.arange(40, device="cuda"), torch.zeros(64, device="cuda")
+    freq, _ = K.rotary_frequencies(32, device="cuda")
+    shown = {"loss": lambda: (x[:, 8:72] * 2, w.narrow(1, 16, 64)), "rotary": lambda: (q.transpose(1, 2) * 1.0,),
+             "route": lambda: (x[:, :64],), "route_reference": lambda: (x[:, :64],)}[op]
+    calls = {"loss": lambda a, b: K.linear_cross_entropy(a, b, target), "rotary": lambda a: K.rotary(a, None, positions, freq)[0].sum(),
+             "route": lambda a: K.moe_route(a, bias, 2, scores="softmax")["top_gates"].sum(), "route_reference": lambda a: K.moe_route(a, bias, 2)["top_gates"].sum()}
+    call = lambda: calls[op](*shown())                                   # noqa: E731
+    leaves = [q] if op == "rotary" else [x] if op.startswith("route") else [x, w]
+
+    def back(loss):
+        if not everything:
+            return torch.autograd.grad(loss, leaves)
+        loss.backward()
+        return [t.grad for t in leaves]
+    earlier = call()
+    want = torch.autograd.grad(earlier, leaves, retain_graph=True)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        with pytest.raises(AssertionError, match="default stream"):
+            with torch.cuda.graph(torch.cuda.CUDAGraph(), stream=side):
+                back(call())
+        forward, inner = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+        with torch.cuda.graph(forward, stream=side):
+            loss = call().detach()
+        with torch.cuda.graph(inner, stream=side):
+            parts = shown()
+            between = torch.autograd.grad(calls[op](*parts), parts)
+        del earlier, parts
+        gc.collect()                                                     # (the refused step's graph, in its exception's frames)
+        for t in leaves:
+            t.grad = None
+        torch.autograd.grad(call(), leaves)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            got = back(call())
+    torch.cuda.current_stream().wait_stream(side)
+    for g in (forward, inner, graph):
+        g.replay()
+    torch.cuda.synchronize()
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
+    assert torch.equal(loss, call().detach()) and all(t.abs().sum() > 0 for t in between)
+    assert K.device_status() == 0
