@@ -1207,6 +1207,8 @@ static Backward carve_backward(void* mem, const Plan& r, bool want_dx, bool want
 // sum off below its last bit: half such a bit, about 0.36 2^-23 of the sum (mantissas spread as logarithms are); and after k of K steps the sum is z k / K
 // on average, whatever the order.  That makes 0.36 K 2^-24 of z.  Measured, in units of K 2^-24, d from 256 to 7168: bf16 0.25 to 0.28 for the words that a
 // softmax is made of, 0.29 to 0.42 for z of 12 to 30, scattered by a tenth of that; fp16 0.3 and, its products having more bits to lose, 0.5 to 1.1.
+// Those are operands with normally distributed elements.  Where nothing is cut off (few non-zeros in a row, or a coarse grid) the factor is itself the error: at d =
+// 7168 it is 8e-6 of a logit, 2.4e-4 of the loss where logits are 30.  It stays below the bound of any fp32 sum of d / 16 steps, d / 16 2^-24.
 static float growth(int64_t d) { return 1.0f + 0.3f * (float)(d / 16) * 0x1p-24f; }
 
 template <auto KERN, size_t SMEM_BYTES, typename... A>

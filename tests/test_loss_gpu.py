@@ -483,3 +483,23 @@ def test_rare_words_beside_a_likely_one(T, V, d, dtype):
     _within(gw, dw, dw_tol, "grad_w")
     rare = (less > 17) & (less < 20)
     assert rare.sum() > 20 and (dw_tol[rare].norm(dim=1) <= 0.1 * dw[rare].norm(dim=1)).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("T,V,d", [(200, 300, 7168), (70, 5000, 1040), (300, 300, 64)])
+def test_sums_that_lose_nothing(T, V, d, dtype):
+    """Sixteen non-zeros on a coarse grid in each row: the tensor cores' sums are exact, and the factor of 1 + 0.3 d / 16 2^-24 that makes good for what
+    such sums lose on average is itself the error, of that much of the largest logit; beside it the exponentials' 2^-20 and the fp32 of
+    logits and loss, 2^-22."""
+    g = torch.Generator().manual_seed(d)
+    at = torch.arange(16) * (d // 16) + 3
+    x, w = torch.zeros(T, d), torch.zeros(V, d)
+    x[:, at] = torch.randint(-8, 9, (T, 16), generator=g).float() / 4
+    w[:, at] = torch.randint(-16, 17, (V, 16), generator=g).float() / 8
+    x, w, target = x.to(dtype).cuda(), w.to(dtype).cuda(), torch.randint(0, V, (T,), generator=g).cuda()
+    z = x.double() @ w.double().t()
+    want = torch.logsumexp(z, -1) - z.gather(1, target[:, None])[:, 0]
+    tol = 0.3 * (d // 16) * 2.0 ** -24 * z.abs().amax(-1) + 2.0 ** -20 + 2.0 ** -22 * (want + z.abs().amax(-1))
+    assert z.max() > 10
+    loss, _, _ = _run(x, w, target, torch.ones(T, device="cuda"), reduction="none")
+    _within(loss, want, tol, "loss")
