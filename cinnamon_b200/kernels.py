@@ -847,10 +847,12 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, target: torch.Te
                          reduction: str = "mean") -> torch.Tensor:
     """``F.cross_entropy(F.linear(x, weight).float(), target, ...)`` of an output projection (the reference's ``lm_head`` and
     loss, src/train.py:338-376) without the logits in memory: forward and both gradients are made from ``x`` and ``weight``
-    tile by tile.  Beside inputs and gradients a call holds a piece of the logits' gradient at a time: 512 MiB, or 256 words for more than a
-    million tokens.  A mean or sum over 2048 rows or more of 1024 or more whose gradients are wanted makes them in the forward, in three products in
-    place of four: it holds 1.25 GiB meanwhile and the gradients' fp32 sums until its backward (where these are 8 GiB at most), and under
-    ``torch.no_grad()`` none of it.
+    tile by tile.  Beside inputs and gradients a call holds a copy of ``x``'s rows and up to 70 MiB (some 40 bytes a token where that is more); in the
+    backward also a piece of the logits' gradient (512 MiB, or 256 words of it for more than a million tokens) and ``x``'s gradient in fp32; and from one to the
+    other 20 bytes a token.  Operands that are cast (under autocast, anew in every call) or padded (rows of no multiple of 8) are copies as well.
+    A mean or sum over 2048 rows or more of 1024 or more whose gradients are wanted makes them in the forward, in three products in
+    place of four: it holds 1.27 GiB meanwhile (or 256 rows of the logits' gradient, of over 2.6 million words) and the wanted gradients in fp32 (``x``'s in up to 16 parts to
+    be added, over vocabularies that leave a piece few rows) until its backward, where these are 8 GiB at most, and under ``torch.no_grad()`` none of it.
 
     ``x`` (..., d) and ``weight`` (vocabulary, d): both bfloat16 or both float16; under autocast they are cast to its type as for
     ``F.linear``.  ``target`` (...): int64 or int32.  A target equal to ``ignore_index`` takes its token out: loss 0, a
