@@ -503,3 +503,35 @@ def test_sums_that_lose_nothing(T, V, d, dtype):
     assert z.max() > 10
     loss, _, _ = _run(x, w, target, torch.ones(T, device="cuda"), reduction="none")
     _within(loss, want, tol, "loss")
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_operands_changed_in_place_after_the_forward(dtype):
+    """Gradients made in the forward are those of the values it was called with, whatever the operands and targets hold by the time of the backward; made in the
+    backward, they are refused."""
+    from cinnamon_b200 import kernels as K
+    T, V, d = 2300, 700, 1032
+    x, w, target = _inputs(T, V, d, dtype, seed=77, ignored=0.2)
+    want = _run(x, w, target, reduction="sum")
+    for side in (None, 0, 1):                                            # (a frozen one too)
+        a, b, t = x.clone().requires_grad_(side != 0), w.clone().requires_grad_(side != 1), target.clone()
+        leaves = [v for v in (a, b) if v.requires_grad]
+        loss = K.linear_cross_entropy(a, b, t, reduction="sum")
+        with torch.no_grad():
+            a.normal_(), b.zero_(), t.fill_(1)
+        got = torch.autograd.grad(loss, leaves)
+        assert torch.equal(loss.detach(), want[0])
+        for v, g in zip(got, [want[1 + i] for i in range(2) if i != side]):
+            assert torch.equal(v, g)
+    up = torch.ones(T, device="cuda")
+    want = _run(x, w, target, up, reduction="none")
+    for changed in range(3):
+        a, b, t = x.clone().requires_grad_(True), w.clone().requires_grad_(True), target.clone()
+        loss = K.linear_cross_entropy(a, b, t, reduction="none")
+        with torch.no_grad():
+            (a, b, t)[changed].zero_()
+        if changed == 2:                                                 # (the backward reads its own copy of the targets)
+            assert torch.equal(torch.autograd.grad(loss, a, up)[0], want[1])
+            continue
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            torch.autograd.grad(loss, [a, b], up)
