@@ -370,7 +370,12 @@ def _rotate_setup(ctx, inputs, output):
 
 
 def _rotate_backward(ctx, grads):
-    out = torch.ops.cinnamon_b200.rotate(list(grads), *ctx.saved_tensors, ctx.interleaved, ctx.start, ctx.magnitude, not ctx.inverse)
+    wanted = [g is not None and bool(n) for g, n in zip(grads, ctx.needs_input_grad[0])]
+    out = [None] * len(grads)
+    if any(wanted):
+        turned = iter(torch.ops.cinnamon_b200.rotate([g for g, w in zip(grads, wanted) if w], *ctx.saved_tensors, ctx.interleaved, ctx.start, ctx.magnitude,
+                                                     not ctx.inverse))
+        out = [next(turned) if w else None for w in wanted]
     return out, None, None, None, None, None, None
 
 

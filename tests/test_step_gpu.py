@@ -391,3 +391,30 @@ def test_capture_beside_a_living_graph_of_a_leaf_behind_views(op, everything):
         assert torch.equal(a, b)
     assert torch.equal(loss, call().detach()) and all(t.abs().sum() > 0 for t in between)
     assert K.device_status() == 0
+
+
+@pytest.mark.parametrize("frozen", [0, 1, None])
+def test_compiled_rotary_with_one_side_frozen(frozen):
+    """The eager call's bits, and no gradient for the side that takes none (heads of other lengths: `start` counts from each one's end)."""
+    from cinnamon_b200 import kernels as K
+    g = torch.Generator().manual_seed(8)
+    q, k = torch.randn(2, 8, 600, 96, generator=g).bfloat16().cuda(), torch.randn(2, 4, 600, 160, generator=g).bfloat16().cuda()
+    freq, positions = K.rotary_frequencies(32, device="cuda")[0], torch.arange(600, device="cuda")
+    call = lambda q, k: K.rotary(q, k, positions, freq, start=-32)       # noqa: E731
+    results, most = [], []
+    for compiled in (False, True):
+        torch._dynamo.reset()
+        f = torch.compile(call, fullgraph=True) if compiled else call
+        a, b = (t.clone().requires_grad_(i != frozen) for i, t in enumerate((q, k)))
+        leaves = [t for t in (a, b) if t.requires_grad]
+        torch.autograd.grad(f(a, b), leaves, [q, k])
+        out = f(a, b)
+        torch.cuda.synchronize()
+        torch.cuda.reset_peak_memory_stats()
+        before = torch.cuda.memory_allocated()
+        grads = torch.autograd.grad(out, leaves, [q, k])
+        most.append(torch.cuda.max_memory_allocated() - before)
+        results.append([*(t.detach() for t in out), *grads])
+    for got, want in zip(results[1], results[0]):
+        assert got.shape == want.shape and torch.equal(got, want)
+    assert most[1] <= most[0] + (1 << 20)                                # (a gradient of these: 1.8 and 1.5 MB)
