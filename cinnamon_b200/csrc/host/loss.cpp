@@ -140,7 +140,6 @@ void check_grad(const Tensor& grad, const at::Device& dev, int64_t numel) {
 
 void bind_loss(pybind11::module_& m) {
     namespace py = pybind11;
-    m.def("linear_ce_operands", &ce_operands);
     m.def("linear_ce_early", [](int64_t T, int64_t V, int64_t d, int64_t reduction, int which) { return api.cinn_linear_ce_early(T, V, d, (int)reduction, which); });
     // (loss, state, sums of dx, sums of dw); what is not made is empty: the sums in the late way, and those of a gradient that is not wanted
     m.def("linear_ce_forward", [](const Tensor& x, const Tensor& w, const Tensor& target, int64_t ignore, int64_t reduction, bool early, bool want_x, bool want_w) {
