@@ -332,12 +332,15 @@ __device__ __forceinline__ void largest_keys(const uint32_t (&k)[VPL], uint32_t 
     }
 }
 
-// What bounds it are the integer units, at half the rate of the floating-point ones: selections, comparisons, minima.  So a lane's VPL
+// What it is made of are integer instructions at half the rate of the floating-point ones: selections, comparisons, minima.  So a lane's VPL
 // neighbouring experts are keys that need little of them: score + bias, made positive by a common offset, is a float whose bits are in order
 // as they are, and its last bits are the expert's number in the lane (the lower one larger).  A lane keeps its eight largest, sorted; should
 // one run out of them, the token is chosen in 64 bits.  A round is one reduction, a vote and a shift of the winner's keys.  8 of 256 experts,
 // 32768 tokens, 46 us, 760 instructions a token, 16 of them a round.  (All keys of a lane unsorted, with a look through the winner's: 1280
-// and 83 us; 1024 experts, all 32 keys of a lane sorted: 281 us in all, like this 110.)
+// and 83 us; 1024 experts, all 32 keys of a lane sorted: 281 us in all, like this 110.)  What bounds it now is latency: of 63 thousand active cycles at that size a
+// scheduler issues in 42 thousand and the integer pipe works in 31 thousand; 30 of 40 warps are resident, and a warp waits for a token's logits with
+// none of the next one's on their way.  32 of more experts than 32 always go through route_exact, since the list has no place for the one behind
+// the last (4096 tokens to 32 of 64 32 us, to 31 of them 26).
 //
 // Errors of the quick scores.  Sigmoid: the exponent's rounding is |x| 2^-24 of e^-x, its part in the score s (1 - s) |x| 2^-24 < 2^-26, and
 // ex2, the sum and rcp add less than 2^-22: two scores are sure to be in order when they are 2^-20 apart, and HIDDEN of the key: what
