@@ -495,7 +495,7 @@ route_form_kernel(const L* __restrict__ logits, const float* __restrict__ bias, 
             for (; n < 32; ++n) {
                 const uint32_t next = take(n);
                 if (v_last - __uint_as_float(next) > wide) break;
-                if (next == 0u) { unsure = n < E; break; }
+                if (next == 0u) { unsure = unsure || n < E; break; }           // (where all are taken, one of them may have been no key)
             }
             if (n == 32 && top_k < E) unsure = true;                           // (more of them than lanes)
             if (__any_sync(0xffffffffu, more && best[0] == 0u)) unsure = true;

@@ -391,3 +391,34 @@ def test_outputs_changed_in_place_before_the_backward(gates, scores, renormalise
         got = back()
         assert torch.equal(got, want) if gates == "top_gates" else (got == 0).all()
     assert K.device_status() == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("scores", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("E,n_groups", [(1, 1), (2, 1), (3, 1), (8, 2), (24, 4), (32, 1), (32, 8)])
+@pytest.mark.parametrize("kind", ["banned", "all banned", "underflow", "equal"])
+def test_all_experts_are_chosen(kind, E, n_groups, scores):
+    """As many as there are: banned experts come last, each once, and so do those whose score is 0 in fp32."""
+    from cinnamon_b200 import kernels as K
+    T = 300
+    g = torch.Generator().manual_seed(E)
+    logits = torch.zeros(T, E) if kind == "equal" else torch.randn(T, E, generator=g)
+    if kind == "underflow":
+        logits[torch.rand(T, E, generator=g) < 0.5] -= 110.0
+    for low in (float("-inf"), -1e31, torch.finfo(torch.float32).min):
+        bias = torch.full((E,), low if kind == "all banned" else 0.0)
+        if kind in ("banned", "equal"):
+            bias[::2] = low
+        bias = None if kind == "underflow" and low != -1e31 else bias.cuda()
+        x = logits.cuda().requires_grad_(True)
+        r = K.moe_route(x, bias, E, scores=scores, n_groups=n_groups, top_groups=n_groups, renormalise=False)
+        s, top = _choose(logits, bias, E, scores, n_groups, n_groups)
+        want = dict(top_experts=top.int(), counts=torch.full((E,), T), sorted_experts=torch.arange(E).repeat_interleave(T),
+                    token_indices=torch.arange(T).repeat(E))
+        for name, w in want.items():
+            assert torch.equal(r[name].cpu(), w), name
+        gates = s.gather(1, top)
+        assert ((r["top_gates"].detach().double().cpu() - gates).abs() <= 2.0 ** -18 * gates + 2.0 ** -126).all()
+        grad, = torch.autograd.grad(r["top_gates"].sum(), x)
+        assert torch.isfinite(grad).all()
+    assert K.device_status() == 0
