@@ -9,9 +9,11 @@
 // the angle is exact to 2^-53 of the frequency times the position.  The top two bits (rounded) are the quadrant, and the rest,
 // within an eighth of a turn, goes to sincospif in fp32.
 //
-// Every element is read and written once, and where up to half of a head is rotated that is what bounds it.  Whole heads in 16 bits are bound by shared memory:
-// cosines and sines are read anew for every head, 8 bytes a pair, neighbouring lanes 64 bytes apart on the same banks (queries of 32 and keys of 8 heads
-// x 4 x 4096 positions x 128 in bf16, 336 MB in and out: 128 of 128 rotated 78 us, 4.3 TB/s, interleaved 84; 64 of 128 57 us, 5.9 TB/s).  A CTA takes jobs of up to 24 KiB (a few positions of a sequence and some of
+// Every element is read and written once, and where up to half of a head is rotated that is what bounds it.  Whole heads in 16 bits are bound by
+// shared memory: cosines and sines are read anew for every head, 8 bytes a pair, neighbouring lanes 64 bytes apart on the same banks (32 query and
+// 8 key heads x 4 x 4096 positions x 128 in bf16, 336 MB in and out: 128 of 128 rotated 78 us, 4.3 TB/s, interleaved 84; 64 of 128 57 us, 5.9 TB/s).
+//
+// A CTA takes jobs of up to 24 KiB (a few positions of a sequence and some of
 // their heads), two of them on their way into shared memory by TMA while a third is turned in place and leaves the same way.  A job is
 // one box of a tensor map over (part of a head, parts, heads, positions, sequences), so any strides of whole 16 bytes are one instruction of one
 // thread: with loads and stores of the threads' own, resident CTAs did not keep enough bytes in flight (queries and keys of 32 x 8
